@@ -19,7 +19,9 @@ OBJDIR = os.path.join(HERE, "lib", "obj")
 SO = os.path.join(LIBDIR, "libcozo_gpu.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-fno-fast-math",
-         "-Wall", "-Wno-unused-function", "-Wno-unused-variable", "-Wno-unused-but-set-variable"]
+         "-Wall", "-Wno-unused-function", "-Wno-unused-variable", "-Wno-unused-but-set-variable",
+         # no v_pk_*_f32: some of their forms have given wrong results on gfx950 (the host pass does not know the feature and says so)
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _sources():
