@@ -1,0 +1,144 @@
+// gemm_nt.h -- the matrix-core loop that the dense operators share:  C[m][n] = sum_k A[m][k] * B[n][k],  both operands with k
+// contiguous.  A workgroup owns a BM x BN tile; what happens to the accumulators is the caller's epilogue.
+//
+// * k goes in steps of 128 bytes per row (64 bf16 / 32 f32): a step of A and B goes straight from memory into LDS (16 bytes a lane, no
+//   registers in between), two steps are kept, the next one is on its way while the matrix cores work on this one.
+// * LDS rows are 128 bytes = 8 pieces of 16; piece p of row r lies at place p ^ (r & 7), so that the 32 rows a matrix instruction reads
+//   at one k spread over all banks.  The copy into LDS writes lanes in order, so it is the lane's GLOBAL address that is permuted.
+// * operand layout of the 32 x 32 matrix instructions: lane l holds row l % 32 and the k that belong to half l / 32; as both
+//   operands are read alike, which k those are does not matter: a half is a 16-byte piece (8 bf16 = one 32x32x16 instruction, 4 f32 =
+//   four 32x32x2 ones).
+// * accumulators: register r of lane l is C[8 (r / 4) + 4 (l / 32) + r % 4][l % 32] of its 32 x 32 tile.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+namespace gemm {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+struct Bf16 {
+    typedef __bf16 T;
+    static constexpr uint32_t kStep = 64;  // elements of a 128-byte step
+};
+struct F32 {
+    typedef float T;
+    static constexpr uint32_t kStep = 32;
+};
+
+__device__ __forceinline__ void mma(Bf16, const u32x4 &a, const u32x4 &b, f32x16 &c) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ void mma(F32, const u32x4 &a, const u32x4 &b, f32x16 &c) {
+    const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+    for (int j = 0; j < 4; j++) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j], y[j], c, 0, 0, 0);
+}
+
+// rows of one operand as a workgroup sees them; rows past the last one are read as the last one (the epilogue drops them)
+struct Operand {
+    const char *base;
+    uint64_t ld;     // bytes
+    uint32_t rows;
+};
+
+template <class E, int BM, int BN, int WM, int WN>
+struct Tile {
+    static constexpr int kThreads = 64 * WM * WN;
+    static constexpr int MT = BM / WM / 32, NT = BN / WN / 32;
+    static constexpr int kBytes = (BM + BN) * 128;  // LDS of one step
+    static constexpr int kLds = 2 * kBytes;
+    static constexpr int NA = BM * 8 / kThreads, NB = BN * 8 / kThreads;  // 16-byte pieces a thread copies per step
+    static_assert(MT * WM * 32 == BM && NT * WN * 32 == BN, "waves cover the tile");
+    static_assert(NA * kThreads == BM * 8 && NB * kThreads == BN * 8, "threads cover the copies");
+
+    f32x16 acc[MT][NT];
+
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < MT; i++)
+#pragma unroll
+            for (int j = 0; j < NT; j++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) acc[i][j][r] = 0.f;
+    }
+    // where this thread's pieces of a tile that starts at row0 come from (k = 0)
+    template <int N>
+    static __device__ __forceinline__ void rows_of(const Operand &o, uint32_t row0, const char *(&src)[N]) {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const uint32_t c = i * kThreads + threadIdx.x, row = c >> 3, piece = (c & 7) ^ (row & 7);
+            src[i] = o.base + (uint64_t)min(row0 + row, o.rows - 1) * o.ld + piece * 16;
+        }
+    }
+    template <int N>
+    static __device__ __forceinline__ void copy(const char *(&src)[N], uint64_t k, char *lds) {
+        const uint32_t wave = threadIdx.x >> 6;
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(src[i] + k),
+                                             (__attribute__((address_space(3))) void *)(lds + (i * kThreads + wave * 64) * 16), 16, 0, 0);
+    }
+    // the copies this wave has in flight are in LDS, and every wave is here
+    static __device__ __forceinline__ void arrived() {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+    }
+    static __device__ __forceinline__ int wave_row() { return (int)(threadIdx.x >> 6) / WN * (BM / WM); }
+    static __device__ __forceinline__ int wave_col() { return (int)(threadIdx.x >> 6) % WN * (BN / WN); }
+
+    __device__ __forceinline__ void step(const char *lds) {
+        const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
+        const char *la = lds + (wave_row() + l32) * 128, *lb = lds + BM * 128 + (wave_col() + l32) * 128;
+#pragma unroll
+        for (int kk = 0; kk < 4; kk++) {
+            const int at = ((2 * kk + half) ^ (l32 & 7)) * 16;
+            u32x4 a[MT], b[NT];
+#pragma unroll
+            for (int i = 0; i < MT; i++) a[i] = *(const u32x4 *)(la + i * 32 * 128 + at);
+#pragma unroll
+            for (int j = 0; j < NT; j++) b[j] = *(const u32x4 *)(lb + j * 32 * 128 + at);
+#pragma unroll
+            for (int i = 0; i < MT; i++)
+#pragma unroll
+                for (int j = 0; j < NT; j++) mma(E{}, a[i], b[j], acc[i][j]);
+        }
+    }
+    // one tile: A rows from m0, B rows from n0, `steps` >= 1 steps from byte k0 of a row on
+    __device__ __forceinline__ void run(const Operand &A, uint32_t m0, const Operand &B, uint32_t n0, uint64_t k0, uint32_t steps, char *lds) {
+        const char *sa[NA], *sb[NB];
+        rows_of(A, m0, sa);
+        rows_of(B, n0, sb);
+        zero();
+        copy(sa, k0, lds);
+        copy(sb, k0, lds + BM * 128);
+        for (uint32_t s = 0; s < steps; s++) {
+            char *cur = lds + (s & 1) * kBytes, *nxt = lds + (~s & 1) * kBytes;
+            arrived();
+            if (s + 1 < steps) {
+                copy(sa, k0 + (uint64_t)(s + 1) * 128, nxt);
+                copy(sb, k0 + (uint64_t)(s + 1) * 128, nxt + BM * 128);
+            }
+            step(cur);
+        }
+    }
+    // f(row, col, value) over this thread's accumulators, rows and columns within the tile
+    template <class F>
+    __device__ __forceinline__ void each(F f) const {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int i = 0; i < MT; i++)
+#pragma unroll
+            for (int j = 0; j < NT; j++)
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    f(wave_row() + i * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3), wave_col() + j * 32 + (lane & 31), acc[i][j][r]);
+    }
+};
+
+}  // namespace gemm

@@ -1,0 +1,546 @@
+// softmax_xent.hip -- softmax cross entropy over a whole table and its gradient (arithmetic: include/cozo_gpu.h).
+//
+// Forward: one matrix product per (table tile, query tile) with the softmax's running maximum and sum as its epilogue.  The TABLE rows are
+// the product's m and the queries its n: a lane's accumulators then belong to one query, so maximum and sum run in the lane and lanes are
+// joined once, at the end of a workgroup's stretch of the table.  Stretches are joined in a second launch.
+// Gradient, a piece of the table at a time:  P = grad_loss scale (softmax - onehot) of the piece is computed again and stored in both
+// orders, then  dW = P^T Q  is written and  dq += P W  goes to per-stretch partial sums (each added to by one workgroup only, in
+// a fixed order: no atomics).
+#include <algorithm>
+#include <cmath>
+
+#include "call.h"
+#include "gemm_nt.h"
+
+using gemm::Bf16;
+using gemm::F32;
+using gemm::Operand;
+
+namespace {
+
+constexpr uint32_t kMaxDim = 8192;
+constexpr float kLog2e = 1.44269504088896340736f;
+
+__device__ __forceinline__ float up(float x) { return x; }
+__device__ __forceinline__ float up(__bf16 x) { return (float)x; }
+template <typename T>
+__device__ __forceinline__ T down(float x) { return (T)x; }
+__device__ __forceinline__ bool has_answer(uint32_t y, uint32_t V) { return y < V; }
+// what exponents are taken relative to: a maximum of -inf (nothing seen yet, or nothing but -inf) or +inf is no reference
+__device__ __forceinline__ float reference(float m) { return fabsf(m) < __builtin_inff() ? m : 0.f; }
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// rows [r0, r0 + n) of x, their first dim elements and zeros up to ldo, one 16-byte aligned row behind the other
+template <typename T>
+__global__ void __launch_bounds__(256)
+xent_pack_kernel(const T *__restrict__ x, uint64_t ld, uint32_t n, uint32_t dim, T *__restrict__ out, uint32_t ldo) {
+    const uint64_t total = (uint64_t)n * ldo;
+    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (uint64_t)gridDim.x * 256) {
+        const uint32_t r = (uint32_t)(i / ldo), c = (uint32_t)(i - (uint64_t)r * ldo);
+        out[i] = c < dim ? x[r * ld + c] : (T)0.f;
+    }
+}
+
+// out[d][r] = x[r][d] for d < dim, r < n, and zeros up to row length ldo; rows whose target is no row of the table are zeros too when
+// targets are given (what such a query holds, NaN included, must not reach a product with its zero weight)
+template <typename T>
+__global__ void __launch_bounds__(256)
+xent_transpose_kernel(const T *__restrict__ x, uint64_t ld, uint32_t n, uint32_t dim, const uint32_t *__restrict__ targets, uint32_t V,
+                      T *__restrict__ out, uint64_t ldo) {
+    __shared__ T tile[64][64 + 4 / sizeof(T)];
+    const uint32_t r0 = blockIdx.x * 64, d0 = blockIdx.y * 64;
+    const uint32_t c = threadIdx.x & 63, q = threadIdx.x >> 6;
+    for (uint32_t i = q; i < 64; i += 4) {
+        const uint32_t r = r0 + i, d = d0 + c;
+        T v = (T)0.f;
+        if (r < n && d < dim && (!targets || has_answer(targets[r], V))) v = x[r * ld + d];
+        tile[i][c] = v;
+    }
+    __syncthreads();
+    for (uint32_t i = q; i < 64; i += 4) {
+        const uint32_t d = d0 + i, r = r0 + c;
+        if (d < dim && r < ldo) out[(uint64_t)d * ldo + r] = tile[c][i];
+    }
+}
+
+template <class E, int BM, int BN, int WM, int WN>
+__global__ void __launch_bounds__(64 * WM * WN)
+xent_forward_kernel(Operand W, uint32_t v0, Operand Q, uint32_t steps, float scale2, uint32_t n_tiles, uint32_t tiles_per_part,
+                    uint32_t part0, float2 *__restrict__ parts) {
+    typedef gemm::Tile<E, BM, BN, WM, WN> G;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int lane = threadIdx.x & 63;
+    const uint32_t qt = (Q.rows + BN - 1) / BN;
+    const uint32_t n0 = blockIdx.x % qt * BN, part = blockIdx.x / qt;
+    const uint32_t t0 = part * tiles_per_part, t1 = min(n_tiles, t0 + tiles_per_part);
+    float m[G::NT], l[G::NT];
+#pragma unroll
+    for (int j = 0; j < G::NT; j++) m[j] = -__builtin_inff(), l[j] = 0.f;
+    G g;
+    for (uint32_t t = t0; t < t1; t++) {
+        g.run(W, t * BM, Q, n0, 0, steps, lds);
+        const uint32_t left = W.rows - t * BM;  // rows of this tile that exist
+#pragma unroll
+        for (int j = 0; j < G::NT; j++) {
+            float top = m[j];
+#pragma unroll
+            for (int i = 0; i < G::MT; i++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const uint32_t row = G::wave_row() + i * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+                    const float z = row < left ? g.acc[i][j][r] * scale2 : -__builtin_inff();
+                    g.acc[i][j][r] = z;
+                    top = fmaxf(top, z);
+                }
+            const float ref = reference(top);
+            float sum = l[j] * exp2_(m[j] - ref);
+            if (m[j] == -__builtin_inff()) sum = l[j];
+#pragma unroll
+            for (int i = 0; i < G::MT; i++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) sum += exp2_(g.acc[i][j][r] - ref);
+            m[j] = top;
+            l[j] = sum;
+        }
+        __syncthreads();  // LDS is free for the next tile
+    }
+    // lanes that hold the same query: the two halves, then the waves along m
+    float2 *red = (float2 *)lds;  // [WM][BN]
+#pragma unroll
+    for (int j = 0; j < G::NT; j++) {
+        const float mo = __shfl_xor(m[j], 32, 64), lo = __shfl_xor(l[j], 32, 64);
+        const float top = fmaxf(m[j], mo), ref = reference(top);
+        const float sum = (m[j] == -__builtin_inff() ? l[j] : l[j] * exp2_(m[j] - ref)) + (mo == -__builtin_inff() ? lo : lo * exp2_(mo - ref));
+        if (lane < 32) red[(threadIdx.x >> 6) / WN * BN + G::wave_col() + j * 32 + lane] = make_float2(top, sum);
+    }
+    __syncthreads();
+    for (uint32_t c = threadIdx.x; c < BN; c += G::kThreads) {
+        if (n0 + c >= Q.rows) break;
+        float2 a = red[c];
+#pragma unroll
+        for (int w = 1; w < WM; w++) {
+            const float2 b = red[w * BN + c];
+            const float top = fmaxf(a.x, b.x), ref = reference(top);
+            a.y = (a.x == -__builtin_inff() ? a.y : a.y * exp2_(a.x - ref)) + (b.x == -__builtin_inff() ? b.y : b.y * exp2_(b.x - ref));
+            a.x = top;
+        }
+        parts[(uint64_t)(part0 + part) * Q.rows + n0 + c] = a;
+    }
+}
+
+// one wave per query: the stretches joined, the answer's logit, the loss.  f64: a handful of operations per query
+template <typename T>
+__global__ void __launch_bounds__(256)
+xent_join_kernel(const float2 *__restrict__ parts, uint32_t n_parts, const T *__restrict__ q, uint64_t ldq, const T *__restrict__ w,
+                 uint64_t ldw, uint32_t Tn, uint32_t V, uint32_t dim, const uint32_t *__restrict__ targets, float scale,
+                 float *__restrict__ loss, float *__restrict__ lse) {
+    const uint32_t t = blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (t >= Tn) return;
+    float top = -__builtin_inff();
+    for (uint32_t p = lane; p < n_parts; p += 64) top = fmaxf(top, parts[(uint64_t)p * Tn + t].x);
+    for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    const float ref = reference(top);
+    double sum = 0.0;
+    for (uint32_t p = lane; p < n_parts; p += 64) {
+        const float2 a = parts[(uint64_t)p * Tn + t];
+        sum += a.x == -__builtin_inff() ? (double)a.y : (double)a.y * exp2((double)a.x - (double)ref);
+    }
+    const uint32_t y = targets[t];
+    double z = 0.0;
+    if (has_answer(y, V))
+        for (uint32_t d = lane; d < dim; d += 64) z = fma((double)up(q[t * ldq + d]), (double)up(w[y * ldw + d]), z);
+    for (int o = 32; o; o >>= 1) {
+        sum += __shfl_xor(sum, o, 64);
+        z += __shfl_xor(z, o, 64);
+    }
+    if (lane) return;
+    const double e = ((double)ref + log2(sum)) * 0.69314718055994530942;
+    lse[t] = (float)e;
+    loss[t] = y == CZ_NONE ? 0.f : y < V ? (float)(e - (double)scale * z) : __builtin_nanf("");
+}
+
+// P of a piece: p[t][v] and pt[v][t], zeros where the piece or the queries end
+template <class E, int BM, int BN, int WM, int WN>
+__global__ void __launch_bounds__(64 * WM * WN)
+xent_weights_kernel(Operand W, uint32_t v0, uint32_t V, Operand Q, uint32_t steps, float scale, const uint32_t *__restrict__ targets,
+                    const float *__restrict__ lse, const float *__restrict__ grad_loss, typename E::T *__restrict__ p, uint64_t ldp,
+                    typename E::T *__restrict__ pt, uint32_t ldt) {
+    typedef gemm::Tile<E, BM, BN, WM, WN> G;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const uint32_t qt = (ldt + BN - 1) / BN;
+    const uint32_t n0 = blockIdx.x % qt * BN, m0 = blockIdx.x / qt * BM;
+    const int lane = threadIdx.x & 63;
+    G g;
+    g.run(W, m0, Q, n0, 0, steps, lds);
+    const float scale2 = scale * kLog2e;
+#pragma unroll
+    for (int j = 0; j < G::NT; j++) {
+        const uint32_t t = n0 + G::wave_col() + j * 32 + (lane & 31);
+        const uint32_t y = t < Q.rows ? targets[t] : CZ_NONE;
+        const bool on = t < Q.rows && has_answer(y, V);
+        const float l2 = on ? lse[t] * kLog2e : 0.f, weight = on ? grad_loss[t] * scale : 0.f;
+#pragma unroll
+        for (int i = 0; i < G::MT; i++)
+#pragma unroll
+            for (int r4 = 0; r4 < 4; r4++) {
+                const uint32_t v = m0 + G::wave_row() + i * 32 + 8 * r4 + 4 * (lane >> 5);
+                typename E::T o[4];
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    float x = exp2_(fmaf(g.acc[i][j][4 * r4 + r], scale2, -l2));
+                    if (v0 + v + r == y) x -= 1.f;
+                    o[r] = down<typename E::T>(on && v + r < W.rows ? x * weight : 0.f);
+                }
+                if (t < Q.rows && p) {
+                    typedef typename E::T T4 __attribute__((ext_vector_type(4)));
+                    *(T4 *)(p + t * ldp + v) = T4{o[0], o[1], o[2], o[3]};
+                }
+                if (t < ldt && pt)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) pt[(uint64_t)(v + r) * ldt + t] = o[r];
+            }
+    }
+}
+
+// grad_table rows of a piece: pt [rows][ldt] . qt [dim][ldt]^T
+template <class E, int BM, int BN, int WM, int WN>
+__global__ void __launch_bounds__(64 * WM * WN)
+xent_table_grad_kernel(Operand Pt, Operand Qt, uint32_t steps, typename E::T *__restrict__ out, uint32_t dim) {
+    typedef gemm::Tile<E, BM, BN, WM, WN> G;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const uint32_t nt = (dim + BN - 1) / BN;
+    const uint32_t n0 = blockIdx.x % nt * BN, m0 = blockIdx.x / nt * BM;
+    G g;
+    g.run(Pt, m0, Qt, n0, 0, steps, lds);
+    g.each([&](uint32_t r, uint32_t c, float v) {
+        if (m0 + r < Pt.rows && n0 + c < dim) out[(uint64_t)(m0 + r) * dim + n0 + c] = down<typename E::T>(v);
+    });
+}
+
+// partial sums of grad_queries: part s gets p [T][k of stretch s] . wt [dim][k]^T, added to what the earlier pieces left there
+template <class E, int BM, int BN, int WM, int WN>
+__global__ void __launch_bounds__(64 * WM * WN)
+xent_query_grad_kernel(Operand P, Operand Wt, uint32_t steps, uint32_t steps_per_part, int add, float *__restrict__ parts, uint32_t dim) {
+    typedef gemm::Tile<E, BM, BN, WM, WN> G;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const uint32_t nt = (dim + BN - 1) / BN, mt = (P.rows + BM - 1) / BM;
+    const uint32_t n0 = blockIdx.x % nt * BN, m0 = blockIdx.x / nt % mt * BM, s = blockIdx.x / (nt * mt);
+    const uint32_t s0 = s * steps_per_part, s1 = min(steps, s0 + steps_per_part);
+    float *out = parts + (uint64_t)s * P.rows * dim;
+    G g;
+    if (s0 < s1) g.run(P, m0, Wt, n0, (uint64_t)s0 * 128, s1 - s0, lds);
+    else g.zero();
+    g.each([&](uint32_t r, uint32_t c, float v) {
+        if (m0 + r < P.rows && n0 + c < dim) {
+            float *o = out + (uint64_t)(m0 + r) * dim + n0 + c;
+            *o = add ? *o + v : v;
+        }
+    });
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+xent_sum_parts_kernel(const float *__restrict__ parts, uint32_t n_parts, uint64_t n, uint32_t dim, const uint32_t *__restrict__ targets,
+                      uint32_t V, T *__restrict__ out) {
+    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (uint64_t)gridDim.x * 256) {
+        float a = 0.f;
+        for (uint32_t p = 0; p < n_parts; p++) a += parts[p * n + i];
+        if (targets && !has_answer(targets[i / dim], V)) a = 0.f;  // (zero weights times a row that is not finite)
+        out[i] = down<T>(a);
+    }
+}
+
+// ---- host side -------------------------------------------------------------------------------------------------------
+uint64_t up_to(uint64_t x, uint64_t m) { return (x + m - 1) / m * m; }
+
+struct Shape {
+    uint32_t T, V, dim;
+    uint64_t ldq, ldw;
+    bool bf16;
+    uint32_t es() const { return bf16 ? 2 : 4; }
+    uint32_t kstep() const { return 128 / es(); }
+    uint32_t kp() const { return (uint32_t)up_to(dim, kstep()); }
+    uint32_t tp() const { return (uint32_t)up_to(T, kstep()); }
+};
+
+struct Plan {
+    uint32_t piece;        // table rows worked on at a time
+    uint32_t parts;        // forward: stretches of the whole table; backward: partial sums of grad_queries
+    uint32_t tiles_per_part;  // forward, tiles of a stretch
+    void *q, *w;           // packed copies (unaligned rows or a dim that is no multiple of a step), or null
+    void *qt, *wt, *p, *pt;
+    float2 *stats;
+    float *dq;
+    size_t bytes;
+};
+
+constexpr int kBM = 128, kBN = 128, kWM = 2, kWN = 2;
+
+// rows that the matrix loop can read where they are
+bool direct(const void *x, uint64_t ld, uint32_t dim, uint32_t es) {
+    return (reinterpret_cast<uintptr_t>(x) & 15) == 0 && ld * es % 16 == 0 && dim * es % 128 == 0;
+}
+
+Plan make_plan(const Shape &s, bool grad, void *ws) {
+    // the scratch asked for covers packed copies whether or not a call needs them: alignment is not known here
+    Plan pl{};
+    const uint64_t es = s.es(), kp = s.kp(), tp = s.tp();
+    const uint64_t budget = 128ull << 20;
+    const uint64_t per_row = es * (grad ? std::max<uint64_t>(tp, kp) : kp);
+    pl.piece = (uint32_t)std::min<uint64_t>(up_to(s.V, 256), std::max<uint64_t>(1024, budget / per_row / 1024 * 1024));
+    cz::Carve c(ws);
+    pl.q = c.take<uint8_t>((uint64_t)s.T * kp * es);
+    pl.w = c.take<uint8_t>((uint64_t)pl.piece * kp * es);
+    if (!grad) {
+        const uint32_t qt = (s.T + kBN - 1) / kBN;
+        // forward goes over the table piece by piece only where it has to be packed; the stretches are those of a piece either way
+        const uint32_t tiles = (std::min(s.V, pl.piece) + kBM - 1) / kBM;
+        pl.parts = std::max(1u, std::min(tiles, 1024 / qt));
+        pl.tiles_per_part = (tiles + pl.parts - 1) / pl.parts;
+        pl.parts = (tiles + pl.tiles_per_part - 1) / pl.tiles_per_part;
+        pl.stats = c.take<float2>((uint64_t)pl.parts * ((s.V + pl.piece - 1) / pl.piece) * s.T);
+    } else {
+        pl.qt = c.take<uint8_t>(s.dim * tp * es);
+        pl.wt = c.take<uint8_t>((uint64_t)s.dim * pl.piece * es);
+        pl.p = c.take<uint8_t>((uint64_t)s.T * pl.piece * es);
+        pl.pt = c.take<uint8_t>(pl.piece * tp * es);
+        const uint32_t tiles = ((s.T + kBM - 1) / kBM) * ((s.dim + kBN - 1) / kBN);
+        pl.parts = std::max(1u, std::min({512 / tiles, 64u, pl.piece / 1024}));
+        pl.dq = c.take<float>((uint64_t)pl.parts * s.T * s.dim);
+    }
+    pl.bytes = c.used();
+    return pl;
+}
+
+int launched(const char *what) {
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return cz::set_error(CZ_E_HIP, "%s: %s", what, hipGetErrorString(e));
+    return CZ_OK;
+}
+uint32_t grid_of(uint64_t items) { return (uint32_t)std::min<uint64_t>((items + 255) / 256, 1u << 16); }
+
+template <typename T>
+void pack(const T *x, uint64_t ld, uint32_t n, uint32_t dim, void *out, uint32_t ldo, hipStream_t stream) {
+    hipLaunchKernelGGL(xent_pack_kernel<T>, dim3(grid_of((uint64_t)n * ldo)), dim3(256), 0, stream, x, ld, n, dim, (T *)out, ldo);
+}
+
+template <class K>
+int allow_lds(K kernel, int bytes) {
+    if (bytes > 65536) CZ_HIP(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    return CZ_OK;
+}
+
+template <class E>
+int forward(const Shape &s, const Plan &pl, const void *q_, const void *w_, const uint32_t *targets, float scale, float *loss, float *lse,
+            hipStream_t stream) {
+    typedef typename E::T T;
+    typedef gemm::Tile<E, kBM, kBN, kWM, kWN> G;
+    const T *q = (const T *)q_, *w = (const T *)w_;
+    const uint32_t es = s.es(), kp = s.kp();
+    Operand Q{(const char *)q, s.ldq * es, s.T};
+    if (!direct(q, s.ldq, s.dim, es)) {
+        pack(q, s.ldq, s.T, s.dim, pl.q, kp, stream);
+        Q = Operand{(const char *)pl.q, (uint64_t)kp * es, s.T};
+    }
+    const bool wd = direct(w, s.ldw, s.dim, es);
+    auto kernel = xent_forward_kernel<E, kBM, kBN, kWM, kWN>;
+    int rc = allow_lds(kernel, G::kLds);
+    if (rc) return rc;
+    uint32_t parts = 0;
+    for (uint32_t v0 = 0; v0 < s.V; v0 += pl.piece) {
+        const uint32_t nv = std::min(pl.piece, s.V - v0);
+        Operand W{(const char *)(w + v0 * s.ldw), s.ldw * es, nv};
+        if (!wd) {
+            pack(w + v0 * s.ldw, s.ldw, nv, s.dim, pl.w, kp, stream);
+            W = Operand{(const char *)pl.w, (uint64_t)kp * es, nv};
+        }
+        const uint32_t tiles = (nv + kBM - 1) / kBM, here = (tiles + pl.tiles_per_part - 1) / pl.tiles_per_part;
+        hipLaunchKernelGGL(kernel, dim3(here * ((s.T + kBN - 1) / kBN)), dim3(G::kThreads), G::kLds, stream, W, v0, Q, kp / s.kstep(),
+                           scale * kLog2e, tiles, pl.tiles_per_part, parts, pl.stats);
+        parts += here;
+    }
+    hipLaunchKernelGGL(xent_join_kernel<T>, dim3((s.T + 3) / 4), dim3(256), 0, stream, pl.stats, parts, q, s.ldq, w, s.ldw, s.T, s.V, s.dim,
+                       targets, scale, loss, lse);
+    return launched("cz_softmax_xent");
+}
+
+template <class E>
+int backward(const Shape &s, const Plan &pl, const void *q_, const void *w_, const uint32_t *targets, float scale, const float *lse,
+             const float *grad_loss, void *dq, void *dw, hipStream_t stream) {
+    typedef typename E::T T;
+    typedef gemm::Tile<E, kBM, kBN, kWM, kWN> G;
+    const T *q = (const T *)q_, *w = (const T *)w_;
+    const uint32_t es = s.es(), kp = s.kp(), tp = s.tp();
+    Operand Q{(const char *)q, s.ldq * es, s.T};
+    if (!direct(q, s.ldq, s.dim, es)) {
+        pack(q, s.ldq, s.T, s.dim, pl.q, kp, stream);
+        Q = Operand{(const char *)pl.q, (uint64_t)kp * es, s.T};
+    }
+    const bool wd = direct(w, s.ldw, s.dim, es);
+    auto weights = xent_weights_kernel<E, kBM, kBN, kWM, kWN>;
+    auto table_grad = xent_table_grad_kernel<E, kBM, kBN, kWM, kWN>;
+    auto query_grad = xent_query_grad_kernel<E, kBM, kBN, kWM, kWN>;
+    int rc;
+    if ((rc = allow_lds(weights, G::kLds)) || (rc = allow_lds(table_grad, G::kLds)) || (rc = allow_lds(query_grad, G::kLds))) return rc;
+    const uint32_t dt = (s.dim + 63) / 64;
+    if (dw)
+        hipLaunchKernelGGL(xent_transpose_kernel<T>, dim3((tp + 63) / 64, dt), dim3(256), 0, stream, q, s.ldq, s.T, s.dim, targets, s.V,
+                           (T *)pl.qt, (uint64_t)tp);
+    for (uint32_t v0 = 0; v0 < s.V; v0 += pl.piece) {
+        const uint32_t nv = std::min(pl.piece, s.V - v0), vp = (uint32_t)up_to(nv, kBM);
+        const T *wv = w + v0 * s.ldw;
+        Operand W{(const char *)wv, s.ldw * es, nv};
+        if (!wd) {
+            pack(wv, s.ldw, nv, s.dim, pl.w, kp, stream);
+            W = Operand{(const char *)pl.w, (uint64_t)kp * es, nv};
+        }
+        hipLaunchKernelGGL(weights, dim3(vp / kBM * ((tp + kBN - 1) / kBN)), dim3(G::kThreads), G::kLds, stream, W, v0, s.V, Q,
+                           kp / s.kstep(), scale, targets, lse, grad_loss, dq ? (T *)pl.p : nullptr, (uint64_t)vp,
+                           dw ? (T *)pl.pt : nullptr, tp);
+        if (dw) {
+            const Operand Pt{(const char *)pl.pt, (uint64_t)tp * es, nv}, Qt{(const char *)pl.qt, (uint64_t)tp * es, s.dim};
+            hipLaunchKernelGGL(table_grad, dim3(vp / kBM * ((s.dim + kBN - 1) / kBN)), dim3(G::kThreads), G::kLds, stream, Pt, Qt,
+                               tp / s.kstep(), (T *)dw + (uint64_t)v0 * s.dim, s.dim);
+        }
+        if (dq) {
+            hipLaunchKernelGGL(xent_transpose_kernel<T>, dim3((vp + 63) / 64, dt), dim3(256), 0, stream, wv, s.ldw, nv, s.dim,
+                               (const uint32_t *)nullptr, 0u, (T *)pl.wt, (uint64_t)vp);
+            const Operand P{(const char *)pl.p, (uint64_t)vp * es, s.T}, Wt{(const char *)pl.wt, (uint64_t)vp * es, s.dim};
+            const uint32_t steps = vp / s.kstep(), per = (steps + pl.parts - 1) / pl.parts;
+            const uint32_t tiles = ((s.T + kBM - 1) / kBM) * ((s.dim + kBN - 1) / kBN);
+            hipLaunchKernelGGL(query_grad, dim3(tiles * pl.parts), dim3(G::kThreads), G::kLds, stream, P, Wt, steps, per, v0 ? 1 : 0, pl.dq, s.dim);
+        }
+    }
+    if (dq)
+        hipLaunchKernelGGL(xent_sum_parts_kernel<T>, dim3(grid_of((uint64_t)s.T * s.dim)), dim3(256), 0, stream, pl.dq, pl.parts,
+                           (uint64_t)s.T * s.dim, s.dim, targets, s.V, (T *)dq);
+    return launched("cz_softmax_xent_grad");
+}
+
+int check_shape(uint32_t T, uint32_t V, uint32_t dim, int elem) {
+    if (elem != CZ_ELEM_F32 && elem != CZ_ELEM_BF16) return cz::set_error(CZ_E_INVALID, "unknown element type %d", elem);
+    if (dim == 0 || dim > kMaxDim) return cz::set_error(CZ_E_UNSUPPORTED, "dim must be in 1..%u", kMaxDim);
+    if (V == 0) return cz::set_error(CZ_E_INVALID, "a softmax over no rows");
+    if (V >= 0x80000000u || T >= (1u << 24)) return cz::set_error(CZ_E_UNSUPPORTED, "fewer than 2^31 rows and 2^24 queries");
+    return CZ_OK;
+}
+
+// what forward and backward check alike; host arrays are staged
+int prepare_call(Shape &s, int elem, uint32_t flags, const void *&queries, const void *&table, const uint32_t *&targets, cz::HostStage &stage) {
+    int rc = check_shape(s.T, s.V, s.dim, elem);
+    if (rc) return rc;
+    s.bf16 = elem == CZ_ELEM_BF16;
+    if (s.ldq < s.dim || s.ldw < s.dim) return cz::set_error(CZ_E_INVALID, "ldq or ldw is smaller than dim");
+    rc = cz::ensure_device();
+    if (rc || s.T == 0) return rc;
+    if (!queries || !table || !targets) return cz::set_error(CZ_E_INVALID, "null buffer");
+    const uint32_t es = s.es();
+    if (flags & CZ_DEVICE_PTRS) {
+        if ((reinterpret_cast<uintptr_t>(queries) | reinterpret_cast<uintptr_t>(table)) % es || reinterpret_cast<uintptr_t>(targets) % 4)
+            return cz::set_error(CZ_E_INVALID, "an array is not aligned to its elements");
+        if ((rc = cz::check_device_ptr(queries, "queries")) || (rc = cz::check_device_ptr(table, "table"))) return rc;
+        return cz::check_device_ptr(targets, "targets");
+    }
+    for (uint32_t t = 0; t < s.T; t++)
+        if (targets[t] != CZ_NONE && targets[t] >= s.V) return cz::set_error(CZ_E_INVALID, "targets[%u] = %u is no row of %u", t, targets[t], s.V);
+    const uint8_t *q = (const uint8_t *)queries, *w = (const uint8_t *)table;
+    if ((rc = stage.in(q, ((uint64_t)(s.T - 1) * s.ldq + s.dim) * es, &q)) || (rc = stage.in(w, ((uint64_t)(s.V - 1) * s.ldw + s.dim) * es, &w)) ||
+        (rc = stage.in(targets, s.T, &targets)))
+        return rc;
+    queries = q;
+    table = w;
+    return CZ_OK;
+}
+
+}  // namespace
+
+extern "C" uint64_t cz_softmax_xent_workspace(uint32_t T, uint32_t V, uint32_t dim, int elem, int grad) {
+    if (check_shape(T, V, dim, elem)) return 0;
+    if (T == 0) return 256;
+    return make_plan(Shape{T, V, dim, dim, dim, elem == CZ_ELEM_BF16}, grad != 0, nullptr).bytes;
+}
+
+extern "C" int cz_softmax_xent(const void *queries, uint64_t ldq, const void *table, uint64_t ldw, int elem, uint32_t T, uint32_t V,
+                               uint32_t dim, const uint32_t *targets, float scale, float *loss, float *lse, void *ws, uint64_t ws_bytes,
+                               uint32_t flags, void *stream_) {
+    hipStream_t stream = (hipStream_t)stream_;
+    cz::HostStage stage(stream);
+    cz::DevBuf<uint8_t> own;
+    Shape s{T, V, dim, ldq, ldw, false};
+    int rc = prepare_call(s, elem, flags, queries, table, targets, stage);
+    if (rc || T == 0) return rc;
+    if (!loss || !lse) return cz::set_error(CZ_E_INVALID, "null buffer");
+    const bool dev = flags & CZ_DEVICE_PTRS;
+    if (dev) {
+        if ((reinterpret_cast<uintptr_t>(loss) | reinterpret_cast<uintptr_t>(lse)) & 3)
+            return cz::set_error(CZ_E_INVALID, "an array is not aligned to its elements");
+        if ((rc = cz::check_device_ptr(loss, "loss")) || (rc = cz::check_device_ptr(lse, "lse"))) return rc;
+    } else {
+        if ((rc = stage.out(loss, T, &loss)) || (rc = stage.out(lse, T, &lse))) return rc;
+        ws = nullptr;
+    }
+    void *base = nullptr;
+    if ((rc = cz::scratch_of(ws, ws_bytes, make_plan(s, false, nullptr).bytes, own, &base))) return rc;
+    const Plan pl = make_plan(s, false, base);
+    rc = s.bf16 ? forward<Bf16>(s, pl, queries, table, targets, scale, loss, lse, stream)
+                : forward<F32>(s, pl, queries, table, targets, scale, loss, lse, stream);
+    if (rc) return rc;
+    if (!dev) return stage.finish();
+    if (own.p) CZ_HIP(hipStreamSynchronize(stream));
+    return CZ_OK;
+}
+
+extern "C" int cz_softmax_xent_grad(const void *queries, uint64_t ldq, const void *table, uint64_t ldw, int elem, uint32_t T, uint32_t V,
+                                    uint32_t dim, const uint32_t *targets, float scale, const float *lse, const float *grad_loss,
+                                    void *grad_queries, void *grad_table, void *ws, uint64_t ws_bytes, uint32_t flags, void *stream_) {
+    hipStream_t stream = (hipStream_t)stream_;
+    cz::HostStage stage(stream);
+    cz::DevBuf<uint8_t> own;
+    Shape s{T, V, dim, ldq, ldw, false};
+    const bool dev = flags & CZ_DEVICE_PTRS;
+    int rc = prepare_call(s, elem, flags, queries, table, targets, stage);
+    if (rc || (!grad_queries && !grad_table)) return rc;
+    const uint32_t es = s.es();
+    if (T == 0) {  // the table's gradient is written whole all the same
+        if (!grad_table) return CZ_OK;
+        if (!dev) {
+            std::fill_n((uint8_t *)grad_table, (size_t)V * dim * es, (uint8_t)0);
+            return CZ_OK;
+        }
+        if ((rc = cz::check_device_ptr(grad_table, "grad_table"))) return rc;
+        if (s.bf16)
+            hipLaunchKernelGGL(xent_sum_parts_kernel<__bf16>, dim3(grid_of((uint64_t)V * dim)), dim3(256), 0, stream, (const float *)nullptr, 0u,
+                               (uint64_t)V * dim, dim, (const uint32_t *)nullptr, V, (__bf16 *)grad_table);
+        else
+            hipLaunchKernelGGL(xent_sum_parts_kernel<float>, dim3(grid_of((uint64_t)V * dim)), dim3(256), 0, stream, (const float *)nullptr, 0u,
+                               (uint64_t)V * dim, dim, (const uint32_t *)nullptr, V, (float *)grad_table);
+        return launched("cz_softmax_xent_grad");
+    }
+    if (!lse || !grad_loss) return cz::set_error(CZ_E_INVALID, "null buffer");
+    if (dev) {
+        if ((reinterpret_cast<uintptr_t>(lse) | reinterpret_cast<uintptr_t>(grad_loss)) & 3 ||
+            (reinterpret_cast<uintptr_t>(grad_queries) | reinterpret_cast<uintptr_t>(grad_table)) % es)
+            return cz::set_error(CZ_E_INVALID, "an array is not aligned to its elements");
+        if ((rc = cz::check_device_ptr(lse, "lse")) || (rc = cz::check_device_ptr(grad_loss, "grad_loss")) ||
+            (rc = cz::check_device_ptr(grad_queries, "grad_queries")) || (rc = cz::check_device_ptr(grad_table, "grad_table")))
+            return rc;
+    } else {
+        uint8_t *dq = (uint8_t *)grad_queries, *dw = (uint8_t *)grad_table;
+        if ((rc = stage.in(lse, T, &lse)) || (rc = stage.in(grad_loss, T, &grad_loss)) ||
+            (dq && (rc = stage.out(dq, (size_t)T * dim * es, &dq))) || (dw && (rc = stage.out(dw, (size_t)V * dim * es, &dw))))
+            return rc;
+        grad_queries = dq;
+        grad_table = dw;
+        ws = nullptr;
+    }
+    void *base = nullptr;
+    if ((rc = cz::scratch_of(ws, ws_bytes, make_plan(s, true, nullptr).bytes, own, &base))) return rc;
+    const Plan pl = make_plan(s, true, base);
+    rc = s.bf16 ? backward<Bf16>(s, pl, queries, table, targets, scale, lse, grad_loss, grad_queries, grad_table, stream)
+                : backward<F32>(s, pl, queries, table, targets, scale, lse, grad_loss, grad_queries, grad_table, stream);
+    if (rc) return rc;
+    if (!dev) return stage.finish();
+    if (own.p) CZ_HIP(hipStreamSynchronize(stream));
+    return CZ_OK;
+}

@@ -281,6 +281,71 @@ int cz_knn_bruteforce(cz_hnsw_index *ix, const float *queries, uint32_t B, uint3
                       double *out_dist, uint32_t flags, void *stream);
 
 /* =====================================================================================
+ * 4-bit rows: a table of vectors in an eighth of its f32 bytes, its products with queries and the exhaustive k-NN over it.
+ * The reference has no narrower form than F32 (VecElementType, parse/sys.rs); these stand beside cz_distance_batch and
+ * cz_knn_bruteforce for tables that are scanned whole.
+ *
+ * The form.  A row is cut into groups of `group` (32 | 64 | 128) consecutive elements, the last group filled up with zeros.
+ *   m = max |x| of the group;  scale = bf16(m / 7), 0 when m < 2^-60;  code = clamp(rint(x * (1 / scale)), -7, 7) in f32 arithmetic,
+ *   round to nearest even;  the row stands for  code * scale.
+ *   codes   u8 [n][groups * group / 2]  two's complement nibbles, element 2j in the low and 2j + 1 in the high half of byte j;
+ *                                        codes a caller makes may also hold -8; the padding's codes are ignored
+ *   scales  bf16 bits [n][groups]        finite, >= 0
+ *   sqnorms f32 [n]                      sum (code * scale)^2, summed in f64 (a row that is not all zeros never gets 0)
+ * with groups = ceil(dim / group).  `codes` is 16-byte aligned.  dim <= 8192.  A NaN or an infinity in a vector gives its group a
+ * scale that is not finite: the row's distances are then NaN or infinite like the vector's own.
+ *
+ * `ws` / `ws_bytes`: device scratch of at least cz_q4_workspace() bytes, 256-byte aligned, used by this call alone until its work on
+ * `stream` is done; with it and CZ_DEVICE_PTRS a call only enqueues work (it allocates nothing, waits for nothing and may be
+ * captured into a graph).  ws = NULL: the library allocates, waits and frees.  Device pointers have to be on the selected GPU.
+ * ===================================================================================== */
+typedef enum { CZ_ELEM_F32 = 0, CZ_ELEM_BF16 = 1 } cz_elem; /* element type of rows and queries */
+
+/* vectors [n] rows of `dim` elements of type `elem` (cz_elem), `ld` elements apart (ld >= dim)   [all dev-able] */
+int cz_q4_quantize(const void *vectors, int elem, uint32_t n, uint32_t dim, uint64_t ld, uint32_t group, uint8_t *codes,
+                   uint16_t *scales, float *sqnorms, uint32_t flags, void *stream);
+/* out f32 [m][dim]: the rows that rows[0..m) name, or all n of them (rows = NULL, m = n).  A number that is no row gives a row of
+ * NaN (host pointers: CZ_E_INVALID).                                                         [all dev-able] */
+int cz_q4_dequantize(const uint8_t *codes, const uint16_t *scales, uint32_t n, uint32_t dim, uint32_t group, const uint32_t *rows,
+                     uint32_t m, float *out, uint32_t flags, void *stream);
+/* bytes of `ws` for cz_q4_dots (k = 0) or cz_q4_knn of these sizes; 0 when the sizes are refused */
+uint64_t cz_q4_workspace(uint32_t n, uint32_t dim, uint32_t group, uint32_t B, uint32_t k);
+/* out f32 [B][n] = queries . rows: the matrix-vector product (B = 1) and its few-column form.  queries f32 [B][dim].  Products are
+ * summed in 32 bits or more; a query with a NaN or an infinity gives NaN.                    [all dev-able] */
+int cz_q4_dots(const uint8_t *codes, const uint16_t *scales, uint32_t n, uint32_t dim, uint32_t group, const float *queries,
+               uint32_t B, float *out, void *ws, uint64_t ws_bytes, uint32_t flags, void *stream);
+/* exact k-NN over the 4-bit rows (exact: of the rows as they stand, not of the vectors they were made from).  Distances are the
+ * reference's (runtime/hnsw.rs:66-109) between a query and a row, evaluated in f64; the k smallest, ties to the lower row number,
+ * NaN last.  has_radius: distance > radius is left out.  Outputs like cz_hnsw_search_batch: out_ids [B][k] CZ_NONE padded,
+ * out_dist [B][k] f64 (infinity padded), out_count [B].  1 <= k <= 1024.                     [all dev-able] */
+int cz_q4_knn(int metric, const uint8_t *codes, const uint16_t *scales, const float *sqnorms, uint32_t n, uint32_t dim,
+              uint32_t group, const float *queries, uint32_t B, uint32_t k, int has_radius, double radius, uint32_t *out_ids,
+              double *out_dist, uint32_t *out_count, void *ws, uint64_t ws_bytes, const volatile uint8_t *poison, uint32_t flags,
+              void *stream);
+
+/* =====================================================================================
+ * Softmax cross entropy over a whole table: the loss that trains the vectors an index holds (a query's answer against every
+ * other row), and its gradient.  The logits are never kept: the loss goes over the table once with a running maximum and sum, the
+ * gradient works through it in pieces.
+ *   z[t][v] = scale * queries[t] . table[v]       lse[t] = log sum_v exp z[t][v]       loss[t] = lse[t] - z[t][targets[t]]
+ * targets[t] = CZ_NONE: no row answers the query, its loss and gradient are 0.  A target that is no row gives a NaN loss and is
+ * otherwise treated like CZ_NONE (host pointers: CZ_E_INVALID).
+ *   queries [T] rows of `dim` elements, ldq apart; table [V] rows, ldw apart; both of type `elem`; 1 <= dim <= 8192, V >= 1.
+ * Products and sums are f32 (f32 products stay f32; bf16 products are exact).
+ *   grad:  G[t][v] = grad_loss[t] * (exp(z[t][v] - lse[t]) - [v = targets[t]]);   grad_queries = scale * G . table,
+ *          grad_table = scale * G^T . queries   (contiguous [T][dim] / [V][dim] of type `elem`, each written whole; either may be
+ *          NULL).  For bf16, G is rounded to bf16 before the two products.  grad_loss [T] f32; lse as the forward call gave it.
+ * Results do not depend on the run: no atomics.  ws / ws_bytes as for cz_q4_dots, of cz_softmax_xent_workspace() bytes. [all dev-able]
+ * ===================================================================================== */
+uint64_t cz_softmax_xent_workspace(uint32_t T, uint32_t V, uint32_t dim, int elem, int grad);
+int cz_softmax_xent(const void *queries, uint64_t ldq, const void *table, uint64_t ldw, int elem, uint32_t T, uint32_t V,
+                    uint32_t dim, const uint32_t *targets, float scale, float *loss, float *lse, void *ws, uint64_t ws_bytes,
+                    uint32_t flags, void *stream);
+int cz_softmax_xent_grad(const void *queries, uint64_t ldq, const void *table, uint64_t ldw, int elem, uint32_t T, uint32_t V,
+                         uint32_t dim, const uint32_t *targets, float scale, const float *lse, const float *grad_loss,
+                         void *grad_queries, void *grad_table, void *ws, uint64_t ws_bytes, uint32_t flags, void *stream);
+
+/* =====================================================================================
  * Whole-graph fixed rules   replaces: fixed_rule/algos/ (one .rs per rule) behind `trait FixedRule`
  * (fixed_rule/mod.rs:538-567).  Graphs arrive as the CSR that
  * FixedRuleInputRelation::as_directed_graph builds (fixed_rule/mod.rs:136-200): dense u32 ids in

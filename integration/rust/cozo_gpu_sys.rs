@@ -30,6 +30,9 @@ pub const CZ_L2: c_int = 0;
 pub const CZ_COSINE: c_int = 1;
 pub const CZ_IP: c_int = 2;
 
+pub const CZ_ELEM_F32: c_int = 0;
+pub const CZ_ELEM_BF16: c_int = 1;
+
 #[repr(C)]
 pub struct cz_hnsw_index {
     _private: [u8; 0],
@@ -159,6 +162,26 @@ extern "C" {
                                         out: *mut c_double, flags: u32, stream: *mut c_void) -> c_int;
     pub fn cz_knn_bruteforce(ix: *mut cz_hnsw_index, queries: *const c_float, b: u32, k: u32, out_ids: *mut u32,
                              out_dist: *mut c_double, flags: u32, stream: *mut c_void) -> c_int;
+
+    pub fn cz_q4_quantize(vectors: *const c_void, elem: c_int, n: u32, dim: u32, ld: u64, group: u32, codes: *mut u8,
+                          scales: *mut u16, sqnorms: *mut c_float, flags: u32, stream: *mut c_void) -> c_int;
+    pub fn cz_q4_dequantize(codes: *const u8, scales: *const u16, n: u32, dim: u32, group: u32, rows: *const u32, m: u32,
+                            out: *mut c_float, flags: u32, stream: *mut c_void) -> c_int;
+    pub fn cz_q4_workspace(n: u32, dim: u32, group: u32, B: u32, k: u32) -> u64;
+    pub fn cz_q4_dots(codes: *const u8, scales: *const u16, n: u32, dim: u32, group: u32, queries: *const c_float, B: u32,
+                      out: *mut c_float, ws: *mut c_void, ws_bytes: u64, flags: u32, stream: *mut c_void) -> c_int;
+    pub fn cz_q4_knn(metric: c_int, codes: *const u8, scales: *const u16, sqnorms: *const c_float, n: u32, dim: u32, group: u32,
+                     queries: *const c_float, B: u32, k: u32, has_radius: c_int, radius: c_double, out_ids: *mut u32,
+                     out_dist: *mut c_double, out_count: *mut u32, ws: *mut c_void, ws_bytes: u64, poison: *const u8, flags: u32,
+                     stream: *mut c_void) -> c_int;
+    pub fn cz_softmax_xent_workspace(T: u32, V: u32, dim: u32, elem: c_int, grad: c_int) -> u64;
+    pub fn cz_softmax_xent(queries: *const c_void, ldq: u64, table: *const c_void, ldw: u64, elem: c_int, T: u32, V: u32, dim: u32,
+                           targets: *const u32, scale: c_float, loss: *mut c_float, lse: *mut c_float, ws: *mut c_void,
+                           ws_bytes: u64, flags: u32, stream: *mut c_void) -> c_int;
+    pub fn cz_softmax_xent_grad(queries: *const c_void, ldq: u64, table: *const c_void, ldw: u64, elem: c_int, T: u32, V: u32,
+                                dim: u32, targets: *const u32, scale: c_float, lse: *const c_float, grad_loss: *const c_float,
+                                grad_queries: *mut c_void, grad_table: *mut c_void, ws: *mut c_void, ws_bytes: u64, flags: u32,
+                                stream: *mut c_void) -> c_int;
 
     pub fn cz_pagerank(in_offsets: *const u32, in_sources: *const u32, out_degree: *const u32, n: u32, e: u64,
                        damping: c_float, tolerance: c_double, max_iter: u32, scores: *mut c_float, iters_run: *mut u32,
