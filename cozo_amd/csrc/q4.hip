@@ -16,7 +16,8 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr uint32_t kMaxDim = 8192;
-constexpr uint32_t kMaxBatch = 4096;  // queries of one launch; a larger batch goes in turns through the same scratch
+
+constexpr uint32_t kTile = 64;        // rows that the search looks at together
 
 struct Rows {
     const uint8_t *codes;
@@ -165,30 +166,348 @@ q4_dequantize_kernel(Rows t, const uint32_t *__restrict__ rows, uint32_t m, bool
     }
 }
 
-// ---- products, the simple form: LPR lanes per row, every query in turn ------------------------------------------------
-template <int LPR>
+// ---- products on the matrix cores -------------------------------------------------------------------------------------
+// A row's codes are 8-bit integers for the matrix cores after one mask per nibble (the code in a byte's upper half: 16 times it), so
+// a query becomes integers too: fixed point with 31 bits below its largest element, cut into four balanced 8-bit digits.
+//   v_mfma_i32_16x16x64_i8:  A (16 rows) = 4 queries x 4 digits,  B (16 columns) = 16 table rows,  64 elements at a time.
+// Sums within a group are exact.  Lane l of the result holds the four digits of query l / 16 for table row l % 16: they are joined in
+// the lane (two integer shifts-and-adds, two conversions, one fma) and added to one f32 accumulator with the lane's own row's scale.
+// Rounding: 2^-31 of the query's largest element, and f32 sums over the groups.
+// HBM bound up to about 16 queries: per 512 bytes of codes (16 rows x 64 elements) a wave issues 14 vector instructions and one matrix
+// instruction for each 4 queries.
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kNotFinite = -100000;  // exponent of a query that holds a NaN or an infinity
+
+// the element that byte j of a lane's 16 bytes stands for: a dword of codes unpacks into its even and then its odd elements
+__device__ __forceinline__ int element_of_byte(int j) { return (j & 8) + ((j & 4) ? 2 * (j & 3) + 1 : 2 * (j & 3)); }
+
+// one workgroup per 4 queries: digits [block][step][lane][16 bytes] in the order the matrix instruction reads them, the exponent of the
+// fixed point, the norm
 __global__ void __launch_bounds__(256)
-q4_dots_kernel(Rows t, const float *__restrict__ q, uint32_t B, float *__restrict__ out) {
-    const int sub = threadIdx.x % LPR;
-    const uint64_t r = (uint64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
-    if (r >= t.n) return;
-    for (uint32_t b = 0; b < B; b++) {
-        float a = 0.f;
-        for (uint32_t c = sub; c < t.chunks; c += LPR) {
-            const uint32_t w = *(const uint32_t *)(t.codes + (r * t.chunks + c) * 4);
-            const float s = bf16_to_f32(t.scales[r * t.groups + ((c * 8) >> t.gshift)]);
-            float p = 0.f;
+q4_digits_kernel(const float *__restrict__ q, uint32_t B, uint32_t dim, uint32_t steps, uint32_t *__restrict__ digits,
+                 int *__restrict__ exponent, float *__restrict__ norm) {
+    __shared__ float top[4];
+    __shared__ double sum[4];
+    __shared__ int ex[4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    {
+        const uint32_t b = blockIdx.x * 4 + wave;
+        float m = 0.f;
+        double s2 = 0.0;
+        bool bad = false;
+        if (b < B)
+            for (uint32_t i = lane; i < dim; i += 64) {
+                const float v = q[(uint64_t)b * dim + i];
+                m = fmaxf(m, fabsf(v));
+                bad |= !(fabsf(v) < __builtin_inff());
+                s2 = fma((double)v, (double)v, s2);
+            }
+        if (bad) m = __builtin_inff();
+        for (int o = 32; o; o >>= 1) {
+            m = fmaxf(m, __shfl_xor(m, o, 64));
+            s2 += __shfl_xor(s2, o, 64);
+        }
+        if (lane == 0) {
+            int e = 0;
+            if (m == __builtin_inff()) e = kNotFinite;
+            else if (m > 0.f) (void)frexpf(m, &e);
+            ex[wave] = e;
+            if (b < B) {
+                exponent[b] = e;
+                if (norm) norm[b] = e == kNotFinite ? __builtin_nanf("") : __double2float_ru(sqrt(s2));
+            }
+        }
+    }
+    __syncthreads();
+    // a thread makes the 4 bytes of one dword: step, lane of the instruction, dword
+    for (uint32_t i = threadIdx.x; i < steps * 256; i += 256) {
+        const uint32_t step = i >> 8, l = (i >> 2) & 63, w = i & 3;
+        const uint32_t row = l & 15, b = blockIdx.x * 4 + (row >> 2), digit = row & 3;
+        const int e = ex[row >> 2];
+        uint32_t out = 0;
+        if (b < B && e != kNotFinite)
 #pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (c * 8 + j < t.dim) {
-                    const float qv = q[(uint64_t)b * t.dim + c * 8 + j];
-                    p = fma_((float)code_at(w, j), fabsf(qv) < __builtin_inff() ? qv : __builtin_nanf(""), p);
+            for (int j = 0; j < 4; j++) {
+                const uint32_t el = step * 64 + (l >> 4) * 16 + element_of_byte(4 * w + j);
+                if (el < dim) {
+                    int v = (int)rint(ldexp((double)q[(uint64_t)b * dim + el], 30 - e));
+                    int d = 0;
+                    for (uint32_t k = 0; k <= digit; k++) {
+                        d = ((v + 128) & 255) - 128;
+                        v = (v - d) >> 8;
+                    }
+                    out |= (uint32_t)(d & 255) << (8 * j);
                 }
-            a = fma_(p, s, a);
+            }
+        digits[(uint64_t)blockIdx.x * steps * 256 + i] = out;
+    }
+}
+
+// RT x 16 rows and CT x 4 queries to a wave; the digits of the workgroup's queries stay in LDS while its waves go over the table.
+// Loads run one batch of KU steps ahead, across tiles.
+template <int RT, int CT, int GS>
+struct Product {
+    static constexpr int KU = 2;                     // steps (64 elements) of a batch
+    static constexpr int SC = GS == 5 ? 2 : 1;       // scales of a step
+    struct Batch {
+        u32x2 w[KU][RT];
+        uint16_t s[KU][RT][SC];
+    };
+    float acc[RT][CT];
+
+    __device__ __forceinline__ static void load(Batch &x, const Rows &t, uint64_t row0, uint32_t k, uint32_t steps) {
+        const int lane = threadIdx.x & 63, col = lane & 15, kg = lane >> 4;
+        const uint32_t row_bytes = t.chunks * 4;
+#pragma unroll
+        for (int i = 0; i < RT; i++) {
+            const uint64_t r = min(row0 + 16 * i + col, (uint64_t)t.n - 1);  // (rows past the last one: the caller drops them)
+            const uint8_t *c = t.codes + r * row_bytes;
+            const uint16_t *s = t.scales + r * t.groups;
+#pragma unroll
+            for (int u = 0; u < KU; u++) {
+                const uint32_t step = min(k + u, steps - 1);
+                // (a row of an odd number of 32-groups ends half way through its last step: the digits are 0 there)
+                x.w[u][i] = *(const u32x2 *)(c + min(step * 32 + kg * 8, row_bytes - 8));
+#pragma unroll
+                for (int h = 0; h < SC; h++) {
+                    const uint32_t g = GS == 5 ? step * 2 + h : GS == 6 ? step : step >> 1;
+                    x.s[u][i][h] = s[min(g, t.groups - 1)];
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ static float join(const i32x4 &d) {
+        const int hi = (d[3] << 8) + d[2], lo = (d[1] << 8) + d[0];  // (a digit's sum is at most 16 * 8 * 128 * 128 = 2^21)
+        return fmaf((float)hi, 65536.f, (float)lo);
+    }
+    __device__ __forceinline__ void work(const Batch &x, const u32x4 *lds, uint32_t k, uint32_t steps, i32x4 (&open)[RT][CT]) {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int u = 0; u < KU; u++) {
+            if (k + u >= steps) break;  // (uniform)
+            i32x4 b[RT];
+            float s[RT][SC];
+#pragma unroll
+            for (int i = 0; i < RT; i++) {
+                const uint32_t w0 = x.w[u][i][0], w1 = x.w[u][i][1];
+                b[i] = i32x4{(int)((w0 << 4) & 0xF0F0F0F0u), (int)(w0 & 0xF0F0F0F0u), (int)((w1 << 4) & 0xF0F0F0F0u), (int)(w1 & 0xF0F0F0F0u)};
+#pragma unroll
+                for (int h = 0; h < SC; h++) s[i][h] = bf16_to_f32(x.s[u][i][h]);
+            }
+#pragma unroll
+            for (int c = 0; c < CT; c++) {
+                const u32x4 a4 = lds[(c * steps + k + u) * 64 + lane];
+                const i32x4 a = {(int)a4[0], (int)a4[1], (int)a4[2], (int)a4[3]};
+                if constexpr (GS == 5) {  // two groups in a step: lanes 0-31 hold the elements of the first, 32-63 those of the second
+                    const i32x4 none = {0, 0, 0, 0};
+                    const i32x4 a0 = lane < 32 ? a : none, a1 = lane < 32 ? none : a;
+#pragma unroll
+                    for (int i = 0; i < RT; i++) {
+                        const i32x4 d0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(a0, b[i], none, 0, 0, 0);
+                        const i32x4 d1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(a1, b[i], none, 0, 0, 0);
+                        acc[i][c] = fmaf(join(d0), s[i][0], acc[i][c]);
+                        acc[i][c] = fmaf(join(d1), s[i][1], acc[i][c]);
+                    }
+                } else if constexpr (GS == 6) {
+#pragma unroll
+                    for (int i = 0; i < RT; i++) {
+                        const i32x4 d = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b[i], i32x4{0, 0, 0, 0}, 0, 0, 0);
+                        acc[i][c] = fmaf(join(d), s[i][0], acc[i][c]);
+                    }
+                } else {  // a group is two steps; rows hold whole groups
+#pragma unroll
+                    for (int i = 0; i < RT; i++) {
+                        if (((k + u) & 1) == 0) open[i][c] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b[i], i32x4{0, 0, 0, 0}, 0, 0, 0);
+                        else {
+                            const i32x4 d = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b[i], open[i][c], 0, 0, 0);
+                            acc[i][c] = fmaf(join(d), s[i][0], acc[i][c]);
+                        }
+                    }
+                }
+            }
+        }
+    }
+};
+
+// score of a row for the search: larger is nearer, in f32; a row whose score says nothing reliable is as near as can be (its tile is
+// looked at in f64), a row of zeros has no cosine
+__device__ __forceinline__ float score_of(int metric, float dot, float sq) {
+    float v = dot;
+    if (metric == CZ_COSINE) {
+        if (sq == 0.f) return -__builtin_inff();
+        v = dot * rsqrtf(sq);
+    } else if (metric == CZ_L2) {
+        v = fmaf(2.f, dot, -sq);
+    }
+    const bool sure = sq < __builtin_inff() && (sq >= 1e-30f || metric != CZ_COSINE) && fabsf(v) < __builtin_inff();
+    return sure ? v : __builtin_inff();
+}
+// how far a score may be off: `c` of |q| |x| (the product), for L2 the norm's and the difference's rounding, and what the lower end of
+// the f32 range cuts off
+__device__ __forceinline__ float score_error(int metric, float c, float qnorm, float xnorm) {
+    if (metric == CZ_COSINE) return c * qnorm + 0x1p-140f;
+    if (metric == CZ_IP) return c * qnorm * xnorm + 0x1p-140f;
+    return 2.f * c * qnorm * xnorm + 0x1p-22f * xnorm * xnorm + 0x1p-140f;
+}
+
+struct Near {              // what the search takes from the product kernels instead of the products
+    int metric;
+    const float *sqnorms;
+    float err;             // c of score_error
+    const float *qnorm;    // [B]
+    float *tile_score;     // [B][n_tiles] largest score of a tile
+    float *tile_norm;      // [n_tiles] largest norm of a tile's rows
+    float *best;           // [B][n_best] what some row of a wave's tiles is sure to reach
+    uint32_t n_tiles, n_best;
+};
+
+template <int CT, int GS, bool NEAR>
+__global__ void __launch_bounds__(256)
+q4_product_kernel(Rows t, const u32x4 *__restrict__ digits, const int *__restrict__ exponent, uint32_t B, uint32_t steps, float *__restrict__ out,
+                  Near near) {
+    constexpr int RT = 4;
+    static_assert(RT * 16 == kTile, "a wave's rows are a tile of the search");
+    typedef Product<RT, CT, GS> P;
+    extern __shared__ __attribute__((aligned(16))) char smem_raw[];
+    u32x4 *lds = (u32x4 *)smem_raw;  // [CT][steps][64]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15;
+    const uint32_t c0 = blockIdx.y * CT, blocks4 = (B + 3) / 4;
+    for (uint32_t i = threadIdx.x; i < CT * steps * 64; i += 256) {
+        const uint32_t c = c0 + i / (steps * 64);
+        lds[i] = c < blocks4 ? digits[(uint64_t)c0 * steps * 64 + i] : u32x4{0, 0, 0, 0};
+    }
+    int ex[CT];
+    float best[CT], qn[CT];
+#pragma unroll
+    for (int c = 0; c < CT; c++) {
+        const uint32_t b = (c0 + c) * 4 + (lane >> 4);
+        ex[c] = b < B ? exponent[b] : 0;
+        best[c] = -__builtin_inff();
+        qn[c] = NEAR && b < B ? near.qnorm[b] : 0.f;
+    }
+    __syncthreads();
+    const uint64_t n_tiles = ((uint64_t)t.n + kTile - 1) / kTile, stride = (uint64_t)gridDim.x * 4;
+    uint64_t tile = (uint64_t)blockIdx.x * 4 + wave;
+    typename P::Batch cur, nxt;
+    P p;
+    i32x4 open[RT][CT];
+    if (tile < n_tiles) P::load(cur, t, tile * kTile, 0, steps);
+    while (tile < n_tiles) {
+#pragma unroll
+        for (int i = 0; i < RT; i++)
+#pragma unroll
+            for (int c = 0; c < CT; c++) p.acc[i][c] = 0.f;
+        for (uint32_t k = 0; k < steps; k += P::KU) {
+            const bool more = k + P::KU < steps;
+            const uint64_t nt = more ? tile : tile + stride;
+            if (nt < n_tiles) P::load(nxt, t, nt * kTile, more ? k + P::KU : 0, steps);
+            p.work(cur, lds, k, steps, open);
+            cur = nxt;
+        }
+        float sq[RT], xn = 0.f;
+        if constexpr (NEAR) {
+#pragma unroll
+            for (int i = 0; i < RT; i++) {
+                const uint64_t r = tile * kTile + 16 * i + col;
+                sq[i] = r < t.n ? near.sqnorms[r] : 0.f;
+                if (sq[i] < __builtin_inff()) xn = fmaxf(xn, sq[i]);
+            }
+            for (int o = 1; o < 16; o <<= 1) xn = fmaxf(xn, __shfl_xor(xn, o, 64));
+            xn = sqrtf(xn) * 1.0001f + 1e-22f;  // (a square may be rounded off the f32 range's lower end)
+            if (blockIdx.y == 0 && lane == 0) near.tile_norm[tile] = xn;
         }
 #pragma unroll
-        for (int o = 1; o < LPR; o <<= 1) a += __shfl_xor(a, o, 64);
-        if (sub == 0) out[(uint64_t)b * t.n + r] = a;
+        for (int c = 0; c < CT; c++) {
+            const uint32_t b = (c0 + c) * 4 + (lane >> 4);
+            float top = -__builtin_inff();
+#pragma unroll
+            for (int i = 0; i < RT; i++) {
+                const uint64_t r = tile * kTile + 16 * i + col;
+                const float v = ex[c] == kNotFinite ? __builtin_nanf("") : ldexpf(p.acc[i][c], ex[c] - 34);
+                if constexpr (NEAR) {
+                    if (r < t.n) top = fmaxf(top, score_of(near.metric, v, sq[i]));
+                } else {
+                    if (r < t.n && b < B) out[(uint64_t)b * t.n + r] = v;
+                }
+            }
+            if constexpr (NEAR) {
+                for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+                if (b < B && col == 0) near.tile_score[(uint64_t)b * near.n_tiles + tile] = top;
+                best[c] = fmaxf(best[c], top - score_error(near.metric, near.err, qn[c], xn));
+            }
+        }
+        tile += stride;
+    }
+    if constexpr (NEAR) {
+#pragma unroll
+        for (int c = 0; c < CT; c++) {
+            const uint32_t b = (c0 + c) * 4 + (lane >> 4);
+            if (b < B && col == 0) near.best[(uint64_t)b * near.n_best + blockIdx.x * 4 + wave] = best[c];
+        }
+    }
+}
+
+// order-preserving u32 of an f32; NaN as -inf
+__device__ __forceinline__ uint32_t order_of(float f) {
+    if (f != f) f = -__builtin_inff();
+    const uint32_t u = __float_as_uint(f);
+    return (u >> 31) ? ~u : (u | 0x80000000u);
+}
+
+// need[b]: a score that k rows are sure to reach = the k-th largest of what `n` waves (or, where there are too few of them, tiles) are
+// sure to hold, each a row of its own.  Radix selection, 8 bits at a time.  -inf (every row is looked at) when there are fewer than k or the
+// k-th is not finite.
+__global__ void __launch_bounds__(1024)
+q4_need_kernel(Near near, bool by_tile, uint32_t k, float *__restrict__ need) {
+    __shared__ uint32_t hist[256];
+    __shared__ uint32_t sel[2];
+    const uint32_t b = blockIdx.x, n = by_tile ? near.n_tiles : near.n_best;
+    const float *v = (by_tile ? near.tile_score : near.best) + (uint64_t)b * n;
+    const float qn = near.qnorm[b];
+    if (n < k) {
+        if (threadIdx.x == 0) need[b] = -__builtin_inff();
+        return;
+    }
+    uint32_t prefix = 0, left = k;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        if (threadIdx.x < 256) hist[threadIdx.x] = 0;
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < n; i += 1024) {
+            const float f = by_tile ? v[i] - score_error(near.metric, near.err, qn, near.tile_norm[i]) : v[i];
+            const uint32_t o = order_of(f);
+            if (shift == 24 || (o >> (shift + 8)) == prefix) atomicAdd(&hist[(o >> shift) & 255], 1u);
+        }
+        __syncthreads();
+        if (threadIdx.x < 64) {  // suffix sums over 256 bins, 4 to a lane, from the top
+            const int lane = threadIdx.x;
+            uint32_t h[4], mine = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) mine += h[j] = hist[255 - (4 * lane + j)];
+            uint32_t run = mine;
+            for (int o = 1; o < 64; o <<= 1) {
+                const uint32_t up = __shfl_up(run, o, 64);
+                if (lane >= o) run += up;
+            }
+            uint32_t before = run - mine;
+            if (before < left && left <= run) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    if (before < left && left <= before + h[j]) {
+                        sel[0] = 255 - (4 * lane + j);
+                        sel[1] = left - before;
+                    }
+                    before += h[j];
+                }
+            }
+        }
+        __syncthreads();
+        prefix = (prefix << 8) | sel[0];
+        left = sel[1];
+    }
+    if (threadIdx.x == 0) {
+        const float f = __uint_as_float((prefix >> 31) ? (prefix & 0x7FFFFFFFu) : ~prefix);
+        need[b] = fabsf(f) < __builtin_inff() ? f : -__builtin_inff();
     }
 }
 
@@ -224,12 +543,19 @@ __device__ __forceinline__ double row_distance(int metric, const Rows &t, uint32
     return 1.0 - a;
 }
 
-constexpr uint32_t kTile = 64;  // rows that are looked at together
+// the tiles that a search still has to look at in f64: those whose best score could reach what k rows are sure to reach
+struct Candidates {
+    const float *tile_score;  // [B][n_tiles], or null: all tiles
+    const float *tile_norm;   // [n_tiles]
+    const float *qnorm;       // [B]
+    const float *need;        // [B]
+    float err;
+};
 
-// per (chunk of tiles, query): the k nearest rows of the chunk as a sorted partial list
+// per (chunk of tiles, query): the k nearest rows of the chunk's candidate tiles as a sorted partial list
 template <int LPR>
 __global__ void __launch_bounds__(256)
-q4_scan_kernel(int metric, Rows t, const float *__restrict__ queries, uint32_t k, uint32_t tiles_per_chunk,
+q4_scan_kernel(int metric, Rows t, const float *__restrict__ queries, uint32_t k, uint32_t tiles_per_chunk, Candidates cand,
                uint64_t *__restrict__ part_key, uint32_t *__restrict__ part_id) {
     extern __shared__ __attribute__((aligned(16))) char smem_raw[];
     uint64_t *bkey = (uint64_t *)smem_raw;       // [256]
@@ -237,36 +563,65 @@ q4_scan_kernel(int metric, Rows t, const float *__restrict__ queries, uint32_t k
     double *red = (double *)(tkey + k);           // [4]
     uint32_t *bid = (uint32_t *)(red + 4);        // [256]
     uint32_t *tid_ = bid + 256;                   // [k]
-    float *q = (float *)(tid_ + k);               // [dim]
+    uint32_t *list = tid_ + k;                    // [256] candidate tiles, ascending
+    uint32_t *cnt = list + 256;                   // [4]
+    float *q = (float *)(cnt + 4);                // [dim]
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, sub = tid % LPR;
     const uint32_t b = blockIdx.y;
-    const uint64_t n_tiles = (t.n + kTile - 1) / kTile;
+    const uint32_t n_tiles = (uint32_t)(((uint64_t)t.n + kTile - 1) / kTile);
+    const uint32_t t0 = blockIdx.x * tiles_per_chunk, t1 = (uint32_t)min((uint64_t)n_tiles, (uint64_t)t0 + tiles_per_chunk);
+    const float need = cand.tile_score ? cand.need[b] : 0.f, qn = cand.tile_score ? cand.qnorm[b] : 0.f;
     double qq = 0.0;
-    for (uint32_t i = tid; i < t.dim; i += 256) {
-        const float v = queries[(uint64_t)b * t.dim + i];
-        q[i] = v;
-        qq = fma((double)v, (double)v, qq);
-    }
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) qq += __shfl_xor(qq, o, 64);
-    if (lane == 0) red[wave] = qq;
-    __syncthreads();
-    qq = (red[0] + red[1]) + (red[2] + red[3]);
-    const uint64_t t0 = (uint64_t)blockIdx.x * tiles_per_chunk, t1 = min(n_tiles, t0 + tiles_per_chunk);
+    bool ready = false;
     int tcnt = 0;
-    for (uint64_t r0 = t0 * kTile; r0 < t1 * kTile; r0 += 256) {
-        const uint32_t nb = (uint32_t)min((uint64_t)256, min((uint64_t)t.n, t1 * kTile) - r0);
-        for (int it = 0; it < LPR; it++) {
-            const uint32_t slot = wave * 64 + it * (64 / LPR) + lane / LPR;
-            if (wave * 64 + it * (64 / LPR) >= (int)nb) break;  // (uniform in the wave)
-            const uint32_t r = (uint32_t)(r0 + min(slot, nb - 1));
-            const double d = row_distance<LPR>(metric, t, r, sub, q, qq);
-            if (sub == 0 && slot < nb) {
-                bkey[slot] = dist_key(d);
-                bid[slot] = r;
-            }
+    for (uint32_t tb = t0; tb < t1; tb += 256) {
+        const uint32_t tile = tb + tid;
+        bool want = tile < t1;
+        if (want && cand.tile_score) {
+            const float s = cand.tile_score[(uint64_t)b * n_tiles + tile];
+            want = !(s + score_error(metric, cand.err, qn, cand.tile_norm[tile]) < need);
         }
-        tcnt = topk_merge_batch((int)nb, bkey, bid, tkey, tid_, tcnt, (int)k);
+        const unsigned long long m = __ballot(want);
+        if (lane == 0) cnt[wave] = __popcll(m);
+        __syncthreads();
+        uint32_t at = __popcll(m & ((1ull << lane) - 1ull)), total = 0;
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            if (w < wave) at += cnt[w];
+            total += cnt[w];
+        }
+        if (want) list[at] = tile;
+        __syncthreads();
+        if (total && !ready) {  // the query, once there is something to look at
+            for (uint32_t i = tid; i < t.dim; i += 256) {
+                const float v = queries[(uint64_t)b * t.dim + i];
+                q[i] = v;
+                qq = fma((double)v, (double)v, qq);
+            }
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) qq += __shfl_xor(qq, o, 64);
+            if (lane == 0) red[wave] = qq;
+            __syncthreads();
+            qq = (red[0] + red[1]) + (red[2] + red[3]);
+            ready = true;
+        }
+        for (uint32_t j = 0; j < total; j += 4) {
+            // only the table's last tile can be short, and it is the last of its batch
+            const uint32_t full = min(4u, total - j), last = list[j + full - 1];
+            const uint32_t nb = (full - 1) * kTile + (uint32_t)min((uint64_t)kTile, (uint64_t)t.n - (uint64_t)last * kTile);
+            for (int it = 0; it < LPR; it++) {
+                const uint32_t first = wave * 64 + it * (64 / LPR), slot = first + lane / LPR;
+                if (first >= nb) break;  // (uniform in the wave)
+                const uint32_t safe = min(slot, nb - 1), r = list[j + safe / kTile] * kTile + safe % kTile;
+                const double d = row_distance<LPR>(metric, t, r, sub, q, qq);
+                if (sub == 0 && slot < nb) {
+                    bkey[slot] = dist_key(d);
+                    bid[slot] = r;
+                }
+            }
+            tcnt = topk_merge_batch((int)nb, bkey, bid, tkey, tid_, tcnt, (int)k);
+        }
+        __syncthreads();  // the list is free
     }
     const size_t o = ((size_t)b * gridDim.x + blockIdx.x) * k;
     for (uint32_t i = tid; i < k; i += 256) {
@@ -380,15 +735,77 @@ int launched(const char *what) {
     return CZ_OK;
 }
 
+// the product kernel's launch: digits of the queries, workgroups that stay while their waves go over the table
+struct ProductPlan {
+    uint32_t steps, ct, grid_x, grid_y, n_tiles, lds;
+    u32x4 *digits;
+    int *exponent;
+    float *qnorm;
+};
+ProductPlan product_plan(const Rows &t, uint32_t B, bool near, cz::Carve &c) {
+    ProductPlan p;
+    p.steps = (t.groups << t.gshift) / 64 + ((t.groups << t.gshift) % 64 != 0);
+    p.n_tiles = (uint32_t)(((uint64_t)t.n + kTile - 1) / kTile);
+    const uint32_t blocks4 = (B + 3) / 4;
+    p.ct = blocks4 >= 4 && p.steps * 4 <= 64 ? 4 : blocks4 >= 2 && p.steps * 2 <= 64 ? 2 : 1;
+    p.lds = p.ct * p.steps * 1024;
+    p.grid_y = (blocks4 + p.ct - 1) / p.ct;
+    const uint32_t per_cu = std::max(1u, std::min(4u, 160u * 1024 / p.lds));
+    p.grid_x = std::max(1u, std::min((p.n_tiles + 3) / 4, std::max(1u, 256 * per_cu / p.grid_y)));
+    p.digits = c.take<u32x4>((size_t)blocks4 * p.steps * 64);
+    p.exponent = c.take<int>(B);
+    p.qnorm = near ? c.take<float>(B) : nullptr;
+    return p;
+}
+
+// c of score_error for the digit products.  With |.| the 2-norm and x the row as it stands: the fixed point moves an element by at most
+// 2^-31 of the largest, 2^-31 |q| sqrt(dim) |x| in all; joining the digits and adding `groups` terms rounds by 2^-24 of sums that
+// |q| |x| bounds (three times it, as digits of both signs may cancel); the cosine's reciprocal root, its product and the norm's own
+// rounding are below 2^-21.  A hundredth on top for the bound's own arithmetic.
+float score_error_unit(const Rows &t) {
+    return 1.01f * (3.f * (float)(t.groups + 4) * 0x1p-24f + sqrtf((float)t.dim) * 0x1p-31f + 0x1p-21f);
+}
+
+template <int CT, int GS, bool NEAR>
+int launch_product_as(const Rows &t, const ProductPlan &p, uint32_t B, float *out, const Near &near, hipStream_t stream) {
+    auto kernel = q4_product_kernel<CT, GS, NEAR>;
+    if (p.lds > 65536) CZ_HIP(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.lds));
+    hipLaunchKernelGGL(kernel, dim3(p.grid_x, p.grid_y), dim3(256), p.lds, stream, t, p.digits, p.exponent, B, p.steps, out, near);
+    return CZ_OK;
+}
+template <int CT, bool NEAR>
+int launch_product_ct(const Rows &t, const ProductPlan &p, uint32_t B, float *out, const Near &near, hipStream_t stream) {
+    if (t.gshift == 5) return launch_product_as<CT, 5, NEAR>(t, p, B, out, near, stream);
+    if (t.gshift == 6) return launch_product_as<CT, 6, NEAR>(t, p, B, out, near, stream);
+    return launch_product_as<CT, 7, NEAR>(t, p, B, out, near, stream);
+}
+template <bool NEAR>
+int launch_product(const Rows &t, const ProductPlan &p, const float *q, uint32_t B, float *out, const Near &near, hipStream_t stream) {
+    hipLaunchKernelGGL(q4_digits_kernel, dim3((B + 3) / 4), dim3(256), 0, stream, q, B, t.dim, p.steps, (uint32_t *)p.digits, p.exponent, p.qnorm);
+    if (p.ct == 4) return launch_product_ct<4, NEAR>(t, p, B, out, near, stream);
+    if (p.ct == 2) return launch_product_ct<2, NEAR>(t, p, B, out, near, stream);
+    return launch_product_ct<1, NEAR>(t, p, B, out, near, stream);
+}
+
+// queries of one launch; a larger batch goes in turns through the same scratch (at most 1 GiB of tile scores)
+uint32_t turn_of(const Rows &t) {
+    const uint64_t n_tiles = std::max<uint64_t>(1, ((uint64_t)t.n + kTile - 1) / kTile);
+    return (uint32_t)std::min<uint64_t>(4096, std::max<uint64_t>(64, (1ull << 28) / n_tiles));
+}
+
 struct KnnPlan {
     uint32_t chunks, tiles_per_chunk;
+    bool filtered;         // scores first, f64 distances of the tiles that can hold a result only
     uint64_t *part_key;
     uint32_t *part_id;
+    ProductPlan product;
+    float *tile_score, *tile_norm, *best, *need;
+    uint32_t n_best;
     size_t bytes;
 };
 KnnPlan knn_plan(const Rows &t, uint32_t B, uint32_t k, void *ws) {
-    KnnPlan p;
-    const uint32_t n_tiles = (t.n + kTile - 1) / kTile;
+    KnnPlan p{};
+    const uint32_t n_tiles = (uint32_t)(((uint64_t)t.n + kTile - 1) / kTile);
     // 256 rows are a batch of the list; enough workgroups to fill the chip, few enough lists to join
     uint32_t chunks = std::min((n_tiles + 3) / 4, std::max(1u, 2048 / B));
     chunks = std::max(1u, std::min(chunks, std::max(16u, 65536 / k)));
@@ -398,6 +815,15 @@ KnnPlan knn_plan(const Rows &t, uint32_t B, uint32_t k, void *ws) {
     cz::Carve c(ws);
     p.part_key = c.take<uint64_t>((size_t)B * p.chunks * k);
     p.part_id = c.take<uint32_t>((size_t)B * p.chunks * k);
+    p.filtered = n_tiles >= 4 * (uint64_t)k && n_tiles >= 512;
+    if (p.filtered) {
+        p.product = product_plan(t, B, true, c);
+        p.n_best = p.product.grid_x * 4;
+        p.tile_score = c.take<float>((size_t)B * n_tiles);
+        p.tile_norm = c.take<float>(n_tiles);
+        p.best = c.take<float>((size_t)B * p.n_best);
+        p.need = c.take<float>(B);
+    }
     p.bytes = c.used();
     return p;
 }
@@ -505,7 +931,16 @@ extern "C" uint64_t cz_q4_workspace(uint32_t n, uint32_t dim, uint32_t group, ui
     Rows t;
     if (shape_of_rows(n, dim, group, &t) || k > 1024) return 0;
     if (B == 0 || n == 0) return 256;
-    return k ? std::max<size_t>(256, knn_plan(t, std::min(B, kMaxBatch), k, nullptr).bytes) : 256;
+    const uint32_t turn = turn_of(t);
+    // the last turn of a large batch is smaller and may be laid out differently
+    size_t need = 0;
+    for (const uint32_t nb : {std::min(B, turn), B > turn && B % turn ? B % turn : 0u}) {
+        if (!nb) continue;
+        cz::Carve c(nullptr);
+        if (k == 0) (void)product_plan(t, nb, false, c);
+        need = std::max(need, k ? knn_plan(t, nb, k, nullptr).bytes : c.used());
+    }
+    return need;
 }
 
 extern "C" int cz_q4_dots(const uint8_t *codes, const uint16_t *scales, uint32_t n, uint32_t dim, uint32_t group,
@@ -538,11 +973,13 @@ extern "C" int cz_q4_dots(const uint8_t *codes, const uint16_t *scales, uint32_t
     if ((rc = cz::scratch_of(ws, ws_bytes, cz_q4_workspace(n, dim, group, B, 0), own, &base))) return rc;
     t.codes = codes;
     t.scales = scales;
-    const uint32_t lpr = lanes_per_row(t.chunks);
-#define CZ_Q4_CALL(L)                                                                                                            \
-    hipLaunchKernelGGL((q4_dots_kernel<L>), dim3((n + 256 / L - 1) / (256 / L)), dim3(256), 0, stream, t, queries, B, out)
-    CZ_Q4_LANES(lpr, CZ_Q4_CALL);
-#undef CZ_Q4_CALL
+    const uint32_t turn = turn_of(t);
+    for (uint32_t b0 = 0; b0 < B; b0 += turn) {
+        const uint32_t nb = std::min(turn, B - b0);
+        cz::Carve c(base);
+        const ProductPlan p = product_plan(t, nb, false, c);
+        if ((rc = launch_product<false>(t, p, queries + (size_t)b0 * dim, nb, out + (size_t)b0 * n, Near{}, stream))) return rc;
+    }
     rc = launched("cz_q4_dots");
     if (rc) return rc;
     if (!dev) return stage.finish();
@@ -593,16 +1030,25 @@ extern "C" int cz_q4_knn(int metric, const uint8_t *codes, const uint16_t *scale
     if ((rc = cz::scratch_of(ws, ws_bytes, cz_q4_workspace(n, dim, group, B, k), own, &base))) return rc;
     t.codes = codes;
     t.scales = scales;
-    const size_t smem = 256 * 12 + (size_t)k * 12 + 32 + (size_t)dim * 4;
+    const size_t smem = 256 * 16 + (size_t)k * 12 + 48 + (size_t)dim * 4;
     const uint32_t lpr = lanes_per_row(t.chunks);
-    for (uint32_t b0 = 0; b0 < B; b0 += kMaxBatch) {
-        const uint32_t nb = std::min(kMaxBatch, B - b0);
+    const uint32_t turn = turn_of(t);
+    for (uint32_t b0 = 0; b0 < B; b0 += turn) {
+        const uint32_t nb = std::min(turn, B - b0);
         const float *q = queries + (size_t)b0 * dim;
         KnnPlan p{};
         if (n) {
             p = knn_plan(t, nb, k, base);
+            Candidates cand{};
+            if (p.filtered) {
+                const float err = score_error_unit(t);
+                const Near near{metric, sqnorms, err, p.product.qnorm, p.tile_score, p.tile_norm, p.best, p.product.n_tiles, p.n_best};
+                if ((rc = launch_product<true>(t, p.product, q, nb, nullptr, near, stream))) return rc;
+                hipLaunchKernelGGL(q4_need_kernel, dim3(nb), dim3(1024), 0, stream, near, p.n_best < 4 * k, k, p.need);
+                cand = Candidates{p.tile_score, p.tile_norm, p.product.qnorm, p.need, err};
+            }
 #define CZ_Q4_CALL(L)                                                                                                              \
-    hipLaunchKernelGGL((q4_scan_kernel<L>), dim3(p.chunks, nb), dim3(256), smem, stream, metric, t, q, k, p.tiles_per_chunk,       \
+    hipLaunchKernelGGL((q4_scan_kernel<L>), dim3(p.chunks, nb), dim3(256), smem, stream, metric, t, q, k, p.tiles_per_chunk, cand, \
                        p.part_key, p.part_id)
             CZ_Q4_LANES(lpr, CZ_Q4_CALL);
 #undef CZ_Q4_CALL
