@@ -179,84 +179,80 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kNotFinite = -100000;  // exponent of a query that holds a NaN or an infinity
 
-// the element that byte j of a lane's 16 bytes stands for: a dword of codes unpacks into its even and then its odd elements
-__device__ __forceinline__ int element_of_byte(int j) { return (j & 8) + ((j & 4) ? 2 * (j & 3) + 1 : 2 * (j & 3)); }
+// The element (of a step's 64) that byte j of lane l's 16 bytes stands for.  A lane loads 16 bytes of codes, 32 consecutive elements; lanes
+// 0-31 hold a step's 64, lanes 32-63 the next step's, and a swap of half registers gives every lane 16 of either: the first or the second
+// 16 of its 32.  A dword of codes unpacks into its even and then its odd elements.
+__device__ __forceinline__ int element_of_byte(int l, int j) {
+    return ((l >> 4) & 1) * 32 + (l >> 5) * 16 + (j & 8) + ((j & 4) ? 2 * (j & 3) + 1 : 2 * (j & 3));
+}
 
 // one workgroup per 4 queries: digits [block][step][lane][16 bytes] in the order the matrix instruction reads them, the exponent of the
-// fixed point, the norm
+// fixed point, the norm.  A fixed-point number v has the balanced digits  byte k of (v + 0x00808080), less 128 for the lower three.
 __global__ void __launch_bounds__(256)
 q4_digits_kernel(const float *__restrict__ q, uint32_t B, uint32_t dim, uint32_t steps, uint32_t *__restrict__ digits,
                  int *__restrict__ exponent, float *__restrict__ norm) {
-    __shared__ float top[4];
-    __shared__ double sum[4];
-    __shared__ int ex[4];
+    extern __shared__ __attribute__((aligned(16))) char smem_raw[];
+    uint32_t *fixed = (uint32_t *)smem_raw;  // [4][steps * 64]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    {
-        const uint32_t b = blockIdx.x * 4 + wave;
+    const uint32_t b = blockIdx.x * 4 + wave, width = steps * 64;
+    {   // a wave per query
+        const float *row = q + (uint64_t)min(b, B - 1) * dim;
         float m = 0.f;
         double s2 = 0.0;
         bool bad = false;
-        if (b < B)
-            for (uint32_t i = lane; i < dim; i += 64) {
-                const float v = q[(uint64_t)b * dim + i];
-                m = fmaxf(m, fabsf(v));
-                bad |= !(fabsf(v) < __builtin_inff());
-                s2 = fma((double)v, (double)v, s2);
-            }
+        for (uint32_t i = lane; i < width; i += 64) {
+            const float v = i < dim ? row[i] : 0.f;
+            fixed[wave * width + i] = __float_as_uint(v);
+            m = fmaxf(m, fabsf(v));
+            bad |= !(fabsf(v) < __builtin_inff());
+            s2 = fma((double)v, (double)v, s2);
+        }
         if (bad) m = __builtin_inff();
         for (int o = 32; o; o >>= 1) {
             m = fmaxf(m, __shfl_xor(m, o, 64));
             s2 += __shfl_xor(s2, o, 64);
         }
-        if (lane == 0) {
-            int e = 0;
-            if (m == __builtin_inff()) e = kNotFinite;
-            else if (m > 0.f) (void)frexpf(m, &e);
-            ex[wave] = e;
-            if (b < B) {
-                exponent[b] = e;
-                if (norm) norm[b] = e == kNotFinite ? __builtin_nanf("") : __double2float_ru(sqrt(s2));
-            }
+        int e = 0;
+        if (m == __builtin_inff()) e = kNotFinite;
+        else if (m > 0.f) (void)frexpf(m, &e);
+        if (lane == 0 && b < B) {
+            exponent[b] = e;
+            if (norm) norm[b] = e == kNotFinite ? __builtin_nanf("") : __double2float_ru(sqrt(s2));
+        }
+        const bool on = b < B && e != kNotFinite;
+        for (uint32_t i = lane; i < width; i += 64) {
+            const float v = __uint_as_float(fixed[wave * width + i]);
+            // (a power of two: exact, or below the half step that is rounded away)
+            fixed[wave * width + i] = on ? ((uint32_t)(int)rintf(ldexpf(v, 30 - e)) + 0x00808080u) ^ 0x00808080u : 0u;
         }
     }
     __syncthreads();
     // a thread makes the 4 bytes of one dword: step, lane of the instruction, dword
     for (uint32_t i = threadIdx.x; i < steps * 256; i += 256) {
         const uint32_t step = i >> 8, l = (i >> 2) & 63, w = i & 3;
-        const uint32_t row = l & 15, b = blockIdx.x * 4 + (row >> 2), digit = row & 3;
-        const int e = ex[row >> 2];
+        const uint32_t row = l & 15, shift = (row & 3) * 8;
+        const uint32_t *f = fixed + (row >> 2) * width + step * 64;
         uint32_t out = 0;
-        if (b < B && e != kNotFinite)
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const uint32_t el = step * 64 + (l >> 4) * 16 + element_of_byte(4 * w + j);
-                if (el < dim) {
-                    int v = (int)rint(ldexp((double)q[(uint64_t)b * dim + el], 30 - e));
-                    int d = 0;
-                    for (uint32_t k = 0; k <= digit; k++) {
-                        d = ((v + 128) & 255) - 128;
-                        v = (v - d) >> 8;
-                    }
-                    out |= (uint32_t)(d & 255) << (8 * j);
-                }
-            }
+        for (int j = 0; j < 4; j++) out |= ((f[element_of_byte(l, 4 * w + j)] >> shift) & 255u) << (8 * j);
         digits[(uint64_t)blockIdx.x * steps * 256 + i] = out;
     }
 }
 
 // RT x 16 rows and CT x 4 queries to a wave; the digits of the workgroup's queries stay in LDS while its waves go over the table.
-// Loads run one batch of KU steps ahead, across tiles.
-template <int RT, int CT, int GS>
+// A batch is 256 elements of each row, whole 128-byte lines (read 64 bytes at a time, the lines of 16 waves do not stay in the L1:
+// 1.15 ms instead of 0.76 for one query against 10M x 768, 5.4 TB/s), and loads run one batch ahead, across tiles.  SW: a batch's scales of a row come in one load.
+template <int RT, int CT, int GS, bool SW>
 struct Product {
-    static constexpr int KU = 2;                     // steps (64 elements) of a batch
-    static constexpr int SC = GS == 5 ? 2 : 1;       // scales of a step
+    static constexpr int KU = 4;                     // steps (64 elements) of a batch
+    static constexpr int SC = GS == 5 ? 8 : GS == 6 ? 4 : 2;  // scales of a batch
     struct Batch {
-        u32x2 w[KU][RT];
-        uint16_t s[KU][RT][SC];
+        u32x4 w[KU / 2][RT];
+        uint32_t s[RT][SC / 2];  // two scales to a word
     };
     float acc[RT][CT];
 
-    __device__ __forceinline__ static void load(Batch &x, const Rows &t, uint64_t row0, uint32_t k, uint32_t steps) {
+    __device__ __forceinline__ static void load(Batch &x, const Rows &t, uint64_t row0, uint32_t k) {
         const int lane = threadIdx.x & 63, col = lane & 15, kg = lane >> 4;
         const uint32_t row_bytes = t.chunks * 4;
 #pragma unroll
@@ -265,64 +261,71 @@ struct Product {
             const uint8_t *c = t.codes + r * row_bytes;
             const uint16_t *s = t.scales + r * t.groups;
 #pragma unroll
-            for (int u = 0; u < KU; u++) {
-                const uint32_t step = min(k + u, steps - 1);
-                // (a row of an odd number of 32-groups ends half way through its last step: the digits are 0 there)
-                x.w[u][i] = *(const u32x2 *)(c + min(step * 32 + kg * 8, row_bytes - 8));
+            for (int u = 0; u < KU / 2; u++)  // (where a row ends inside the batch the digits are 0 or the step is not taken)
+                x.w[u][i] = *(const u32x4 *)(c + min((k + 2 * u) * 32 + kg * 16, row_bytes - 16));
+            const uint32_t g0 = GS == 5 ? k * 2 : GS == 6 ? k : k >> 1;
+            if constexpr (SW) {
+                if constexpr (SC == 8) *(u32x4 *)x.s[i] = *(const u32x4 *)(s + g0);
+                else if constexpr (SC == 4) *(u32x2 *)x.s[i] = *(const u32x2 *)(s + g0);
+                else x.s[i][0] = *(const uint32_t *)(s + g0);
+            } else {
 #pragma unroll
-                for (int h = 0; h < SC; h++) {
-                    const uint32_t g = GS == 5 ? step * 2 + h : GS == 6 ? step : step >> 1;
-                    x.s[u][i][h] = s[min(g, t.groups - 1)];
+                for (int h = 0; h < SC / 2; h++) {
+                    const uint32_t a = s[min(g0 + 2 * h, t.groups - 1)], b = s[min(g0 + 2 * h + 1, t.groups - 1)];
+                    x.s[i][h] = a | (b << 16);
                 }
             }
         }
+    }
+    __device__ __forceinline__ static float scale(const Batch &x, int i, int h) {
+        const uint32_t w = x.s[i][h >> 1];
+        return __uint_as_float((h & 1) ? w & 0xFFFF0000u : w << 16);
     }
     __device__ __forceinline__ static float join(const i32x4 &d) {
         const int hi = (d[3] << 8) + d[2], lo = (d[1] << 8) + d[0];  // (a digit's sum is at most 16 * 8 * 128 * 128 = 2^21)
         return fmaf((float)hi, 65536.f, (float)lo);
     }
-    __device__ __forceinline__ void work(const Batch &x, const u32x4 *lds, uint32_t k, uint32_t steps, i32x4 (&open)[RT][CT]) {
+    __device__ __forceinline__ static i32x4 unpack(uint32_t w0, uint32_t w1) {
+        return i32x4{(int)((w0 << 4) & 0xF0F0F0F0u), (int)(w0 & 0xF0F0F0F0u), (int)((w1 << 4) & 0xF0F0F0F0u), (int)(w1 & 0xF0F0F0F0u)};
+    }
+    __device__ __forceinline__ void work(const Batch &x, const u32x4 *lds, uint32_t k, uint32_t steps) {
         const int lane = threadIdx.x & 63;
+        i32x4 open[RT][CT];  // (a group of 128 is two steps of one batch)
 #pragma unroll
         for (int u = 0; u < KU; u++) {
             if (k + u >= steps) break;  // (uniform)
             i32x4 b[RT];
-            float s[RT][SC];
 #pragma unroll
             for (int i = 0; i < RT; i++) {
-                const uint32_t w0 = x.w[u][i][0], w1 = x.w[u][i][1];
-                b[i] = i32x4{(int)((w0 << 4) & 0xF0F0F0F0u), (int)(w0 & 0xF0F0F0F0u), (int)((w1 << 4) & 0xF0F0F0F0u), (int)(w1 & 0xF0F0F0F0u)};
-#pragma unroll
-                for (int h = 0; h < SC; h++) s[i][h] = bf16_to_f32(x.s[u][i][h]);
+                const u32x4 w = x.w[u / 2][i];
+                const u32x2 p = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false), q = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+                b[i] = unpack(p[u & 1], q[u & 1]);
             }
 #pragma unroll
             for (int c = 0; c < CT; c++) {
                 const u32x4 a4 = lds[(c * steps + k + u) * 64 + lane];
-                const i32x4 a = {(int)a4[0], (int)a4[1], (int)a4[2], (int)a4[3]};
-                if constexpr (GS == 5) {  // two groups in a step: lanes 0-31 hold the elements of the first, 32-63 those of the second
-                    const i32x4 none = {0, 0, 0, 0};
-                    const i32x4 a0 = lane < 32 ? a : none, a1 = lane < 32 ? none : a;
+                const i32x4 a = {(int)a4[0], (int)a4[1], (int)a4[2], (int)a4[3]}, none = {0, 0, 0, 0};
+                if constexpr (GS == 5) {  // two groups in a step: lanes 0-15 and 32-47 hold the elements of the first
+                    const bool first = (lane & 16) == 0;
+                    const i32x4 a0 = first ? a : none, a1 = first ? none : a;
 #pragma unroll
                     for (int i = 0; i < RT; i++) {
                         const i32x4 d0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(a0, b[i], none, 0, 0, 0);
                         const i32x4 d1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(a1, b[i], none, 0, 0, 0);
-                        acc[i][c] = fmaf(join(d0), s[i][0], acc[i][c]);
-                        acc[i][c] = fmaf(join(d1), s[i][1], acc[i][c]);
+                        acc[i][c] = fmaf(join(d0), scale(x, i, 2 * u), acc[i][c]);
+                        acc[i][c] = fmaf(join(d1), scale(x, i, 2 * u + 1), acc[i][c]);
                     }
                 } else if constexpr (GS == 6) {
 #pragma unroll
                     for (int i = 0; i < RT; i++) {
-                        const i32x4 d = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b[i], i32x4{0, 0, 0, 0}, 0, 0, 0);
-                        acc[i][c] = fmaf(join(d), s[i][0], acc[i][c]);
+                        const i32x4 d = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b[i], none, 0, 0, 0);
+                        acc[i][c] = fmaf(join(d), scale(x, i, u), acc[i][c]);
                     }
-                } else {  // a group is two steps; rows hold whole groups
+                } else {
 #pragma unroll
                     for (int i = 0; i < RT; i++) {
-                        if (((k + u) & 1) == 0) open[i][c] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b[i], i32x4{0, 0, 0, 0}, 0, 0, 0);
-                        else {
-                            const i32x4 d = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b[i], open[i][c], 0, 0, 0);
-                            acc[i][c] = fmaf(join(d), s[i][0], acc[i][c]);
-                        }
+                        open[i][c] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b[i], (u & 1) ? open[i][c] : none, 0, 0, 0);
+                        if (u & 1) acc[i][c] = fmaf(join(open[i][c]), scale(x, i, u / 2), acc[i][c]);
                     }
                 }
             }
@@ -362,13 +365,16 @@ struct Near {              // what the search takes from the product kernels ins
     uint32_t n_tiles, n_best;
 };
 
-template <int CT, int GS, bool NEAR>
-__global__ void __launch_bounds__(256)
+// workgroups of a CU (of 4 waves, one to a SIMD): what the registers of CT accumulators and two batches leave room for
+constexpr int residents(int ct, int gshift) { return ct == 1 ? (gshift == 5 ? 3 : 4) : ct == 2 && gshift != 5 ? 3 : 2; }
+
+template <int CT, int GS, bool SW, bool NEAR>
+__global__ void __launch_bounds__(256, residents(CT, GS))
 q4_product_kernel(Rows t, const u32x4 *__restrict__ digits, const int *__restrict__ exponent, uint32_t B, uint32_t steps, float *__restrict__ out,
                   Near near) {
     constexpr int RT = 4;
     static_assert(RT * 16 == kTile, "a wave's rows are a tile of the search");
-    typedef Product<RT, CT, GS> P;
+    typedef Product<RT, CT, GS, SW> P;
     extern __shared__ __attribute__((aligned(16))) char smem_raw[];
     u32x4 *lds = (u32x4 *)smem_raw;  // [CT][steps][64]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15;
@@ -391,8 +397,7 @@ q4_product_kernel(Rows t, const u32x4 *__restrict__ digits, const int *__restric
     uint64_t tile = (uint64_t)blockIdx.x * 4 + wave;
     typename P::Batch cur, nxt;
     P p;
-    i32x4 open[RT][CT];
-    if (tile < n_tiles) P::load(cur, t, tile * kTile, 0, steps);
+    if (tile < n_tiles) P::load(cur, t, tile * kTile, 0);
     while (tile < n_tiles) {
 #pragma unroll
         for (int i = 0; i < RT; i++)
@@ -401,8 +406,8 @@ q4_product_kernel(Rows t, const u32x4 *__restrict__ digits, const int *__restric
         for (uint32_t k = 0; k < steps; k += P::KU) {
             const bool more = k + P::KU < steps;
             const uint64_t nt = more ? tile : tile + stride;
-            if (nt < n_tiles) P::load(nxt, t, nt * kTile, more ? k + P::KU : 0, steps);
-            p.work(cur, lds, k, steps, open);
+            if (nt < n_tiles) P::load(nxt, t, nt * kTile, more ? k + P::KU : 0);
+            p.work(cur, lds, k, steps);
             cur = nxt;
         }
         float sq[RT], xn = 0.f;
@@ -469,15 +474,25 @@ q4_need_kernel(Near near, bool by_tile, uint32_t k, float *__restrict__ need) {
         if (threadIdx.x == 0) need[b] = -__builtin_inff();
         return;
     }
+    constexpr int R = 16;  // values a thread keeps; more are read again for each 8 bits
+    uint32_t kept[R];
+    auto value = [&](uint32_t i) { return order_of(by_tile ? v[i] - score_error(near.metric, near.err, qn, near.tile_norm[i]) : v[i]); };
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const uint32_t i = threadIdx.x + r * 1024;
+        kept[r] = i < n ? value(i) : 0u;
+    }
     uint32_t prefix = 0, left = k;
     for (int shift = 24; shift >= 0; shift -= 8) {
         if (threadIdx.x < 256) hist[threadIdx.x] = 0;
         __syncthreads();
-        for (uint32_t i = threadIdx.x; i < n; i += 1024) {
-            const float f = by_tile ? v[i] - score_error(near.metric, near.err, qn, near.tile_norm[i]) : v[i];
-            const uint32_t o = order_of(f);
+        auto count = [&](uint32_t o) {
             if (shift == 24 || (o >> (shift + 8)) == prefix) atomicAdd(&hist[(o >> shift) & 255], 1u);
-        }
+        };
+#pragma unroll
+        for (int r = 0; r < R; r++)
+            if (threadIdx.x + r * 1024 < n) count(kept[r]);
+        for (uint32_t i = threadIdx.x + R * 1024; i < n; i += 1024) count(value(i));
         __syncthreads();
         if (threadIdx.x < 64) {  // suffix sums over 256 bins, 4 to a lane, from the top
             const int lane = threadIdx.x;
@@ -512,35 +527,68 @@ q4_need_kernel(Near near, bool by_tile, uint32_t k, float *__restrict__ need) {
 }
 
 // ---- exact k-NN ------------------------------------------------------------------------------------------------------
-// the f64 distance of one row from the query in LDS, by LPR neighbouring lanes (every lane returns it).  Codes times scales and the
-// products with an f32 are exact in f64; the lanes' sums are joined by a fixed butterfly, so equal rows have equal bits.
-template <int LPR>
-__device__ __forceinline__ double row_distance(int metric, const Rows &t, uint32_t r, int sub, const float *q, double qq) {
-    double a = 0.0, x2 = 0.0;
-    for (uint32_t c = sub; c < t.chunks; c += LPR) {
-        const uint32_t w = *(const uint32_t *)(t.codes + ((uint64_t)r * t.chunks + c) * 4);
-        const double s = (double)bf16_to_f32(t.scales[(uint64_t)r * t.groups + ((c * 8) >> t.gshift)]);
+// the f64 distances of U rows from the query in LDS, by LPR neighbouring lanes (every lane returns them).  A code times an f32 is exact in
+// f64; a lane's 8 codes share a scale, so it is applied once.  The lanes' sums are joined by a fixed butterfly, so equal rows have equal bits.
+template <int LPR, int U>
+__device__ __forceinline__ void row_distances(int metric, const Rows &t, const uint32_t (&r)[U], int sub, const double *q, double qq, double (&out)[U]) {
+    double a[U], x2[U];
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            if (c * 8 + j >= t.dim) break;
-            const double x = (double)code_at(w, j) * s, qv = (double)q[c * 8 + j];
-            if (metric == CZ_L2) {
-                const double d = qv - x;
-                a = fma(d, d, a);
-            } else {
-                a = fma(qv, x, a);
-                x2 = fma(x, x, x2);
+    for (int u = 0; u < U; u++) a[u] = x2[u] = 0.0;
+    for (uint32_t c = sub; c < t.chunks; c += LPR) {
+        uint32_t w[U];
+        double s[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            w[u] = *(const uint32_t *)(t.codes + ((uint64_t)r[u] * t.chunks + c) * 4);
+            s[u] = (double)bf16_to_f32(t.scales[(uint64_t)r[u] * t.groups + ((c * 8) >> t.gshift)]);
+        }
+        const double *qc = q + c * 8;
+        const int left = min(8, (int)t.dim - (int)(c * 8));  // (the last group's padding)
+        if (left < 8)
+#pragma unroll
+            for (int u = 0; u < U; u++) w[u] &= left > 0 ? (1u << (4 * left)) - 1u : 0u;
+        if (metric == CZ_L2) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const double qv = qc[j];
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const double d = fma((double)code_at(w[u], j), -s[u], qv);
+                    // (past the last element the code is 0 and so is the query)
+                    a[u] = fma(d, d, a[u]);
+                }
+            }
+        } else {
+            double p[U];
+            int cc[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) p[u] = 0.0, cc[u] = 0;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const double qv = qc[j];
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const int k = code_at(w[u], j);
+                    p[u] = fma((double)k, qv, p[u]);
+                    cc[u] += k * k;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                a[u] = fma(p[u], s[u], a[u]);
+                x2[u] = fma((double)cc[u], s[u] * s[u], x2[u]);
             }
         }
     }
 #pragma unroll
-    for (int o = 1; o < LPR; o <<= 1) {
-        a += __shfl_xor(a, o, 64);
-        x2 += __shfl_xor(x2, o, 64);
-    }
-    if (metric == CZ_L2) return a;
-    if (metric == CZ_COSINE) return 1.0 - a / sqrt(qq * x2);
-    return 1.0 - a;
+    for (int o = 1; o < LPR; o <<= 1)
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            a[u] += __shfl_xor(a[u], o, 64);
+            x2[u] += __shfl_xor(x2[u], o, 64);
+        }
+#pragma unroll
+    for (int u = 0; u < U; u++) out[u] = metric == CZ_L2 ? a[u] : metric == CZ_COSINE ? 1.0 - a[u] / sqrt(qq * x2[u]) : 1.0 - a[u];
 }
 
 // the tiles that a search still has to look at in f64: those whose best score could reach what k rows are sure to reach
@@ -556,16 +604,16 @@ struct Candidates {
 template <int LPR>
 __global__ void __launch_bounds__(256)
 q4_scan_kernel(int metric, Rows t, const float *__restrict__ queries, uint32_t k, uint32_t tiles_per_chunk, Candidates cand,
-               uint64_t *__restrict__ part_key, uint32_t *__restrict__ part_id) {
+               uint64_t *__restrict__ part_key, uint32_t *__restrict__ part_id, uint32_t *__restrict__ part_count) {
     extern __shared__ __attribute__((aligned(16))) char smem_raw[];
-    uint64_t *bkey = (uint64_t *)smem_raw;       // [256]
+    double *q = (double *)smem_raw;               // [chunks * 8]
+    uint64_t *bkey = (uint64_t *)(q + t.chunks * 8);  // [256]
     uint64_t *tkey = bkey + 256;                  // [k]
     double *red = (double *)(tkey + k);           // [4]
     uint32_t *bid = (uint32_t *)(red + 4);        // [256]
     uint32_t *tid_ = bid + 256;                   // [k]
     uint32_t *list = tid_ + k;                    // [256] candidate tiles, ascending
     uint32_t *cnt = list + 256;                   // [4]
-    float *q = (float *)(cnt + 4);                // [dim]
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, sub = tid % LPR;
     const uint32_t b = blockIdx.y;
     const uint32_t n_tiles = (uint32_t)(((uint64_t)t.n + kTile - 1) / kTile);
@@ -593,10 +641,10 @@ q4_scan_kernel(int metric, Rows t, const float *__restrict__ queries, uint32_t k
         if (want) list[at] = tile;
         __syncthreads();
         if (total && !ready) {  // the query, once there is something to look at
-            for (uint32_t i = tid; i < t.dim; i += 256) {
-                const float v = queries[(uint64_t)b * t.dim + i];
+            for (uint32_t i = tid; i < t.chunks * 8; i += 256) {
+                const double v = i < t.dim ? (double)queries[(uint64_t)b * t.dim + i] : 0.0;
                 q[i] = v;
-                qq = fma((double)v, (double)v, qq);
+                qq = fma(v, v, qq);
             }
 #pragma unroll
             for (int o = 1; o < 64; o <<= 1) qq += __shfl_xor(qq, o, 64);
@@ -609,68 +657,101 @@ q4_scan_kernel(int metric, Rows t, const float *__restrict__ queries, uint32_t k
             // only the table's last tile can be short, and it is the last of its batch
             const uint32_t full = min(4u, total - j), last = list[j + full - 1];
             const uint32_t nb = (full - 1) * kTile + (uint32_t)min((uint64_t)kTile, (uint64_t)t.n - (uint64_t)last * kTile);
-            for (int it = 0; it < LPR; it++) {
-                const uint32_t first = wave * 64 + it * (64 / LPR), slot = first + lane / LPR;
-                if (first >= nb) break;  // (uniform in the wave)
-                const uint32_t safe = min(slot, nb - 1), r = list[j + safe / kTile] * kTile + safe % kTile;
-                const double d = row_distance<LPR>(metric, t, r, sub, q, qq);
-                if (sub == 0 && slot < nb) {
-                    bkey[slot] = dist_key(d);
-                    bid[slot] = r;
+            constexpr int U = 4, AT = 256 / LPR;  // rows of a lane group at a time, lane groups
+            for (uint32_t s0 = 0; s0 < nb; s0 += U * AT) {
+                uint32_t r[U];
+                double d[U];
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const uint32_t safe = min(s0 + u * AT + tid / LPR, nb - 1);
+                    r[u] = list[j + safe / kTile] * kTile + safe % kTile;
                 }
+                row_distances<LPR, U>(metric, t, r, sub, q, qq, d);
+                if (sub == 0)
+#pragma unroll
+                    for (int u = 0; u < U; u++) {
+                        const uint32_t slot = s0 + u * AT + tid / LPR;
+                        if (slot < nb) {
+                            bkey[slot] = dist_key(d[u]);
+                            bid[slot] = r[u];
+                        }
+                    }
             }
             tcnt = topk_merge_batch((int)nb, bkey, bid, tkey, tid_, tcnt, (int)k);
         }
         __syncthreads();  // the list is free
     }
-    const size_t o = ((size_t)b * gridDim.x + blockIdx.x) * k;
-    for (uint32_t i = tid; i < k; i += 256) {
-        const bool have = (int)i < tcnt;
-        part_key[o + i] = have ? tkey[i] : ~0ull;
-        part_id[o + i] = have ? tid_[i] : CZ_NONE;
+    const size_t part = (size_t)b * gridDim.x + blockIdx.x;
+    for (int i = tid; i < tcnt; i += 256) {
+        part_key[part * k + i] = tkey[i];
+        part_id[part * k + i] = tid_[i];
     }
+    if (tid == 0) part_count[part] = (uint32_t)tcnt;
 }
 
 // one workgroup per query: the partial lists joined, the radius cut, the padding
 __global__ void __launch_bounds__(256)
-q4_join_kernel(const uint64_t *__restrict__ part_key, const uint32_t *__restrict__ part_id, uint32_t n_parts, uint32_t k,
-               int has_radius, double radius, uint32_t *__restrict__ out_ids, double *__restrict__ out_dist,
+q4_join_kernel(const uint64_t *__restrict__ part_key, const uint32_t *__restrict__ part_id, const uint32_t *__restrict__ part_count,
+               uint32_t n_parts, uint32_t k, int has_radius, double radius, uint32_t *__restrict__ out_ids, double *__restrict__ out_dist,
                uint32_t *__restrict__ out_count) {
     extern __shared__ __attribute__((aligned(16))) char smem_raw[];
     uint64_t *bkey = (uint64_t *)smem_raw;   // [256]
     uint64_t *tkey = bkey + 256;              // [k]
     uint32_t *bid = (uint32_t *)(tkey + k);   // [256]
     uint32_t *tid_ = bid + 256;               // [k]
-    uint32_t *ctl = tid_ + k;                 // [1]
-    const int tid = threadIdx.x;
+    uint32_t *first = tid_ + k;               // [257] entries of the parts before this one (of 256 parts at a time)
+    uint32_t *ctl = first + 257;              // [5]
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const uint32_t b = blockIdx.x;
-    const size_t total = (size_t)n_parts * k, at = (size_t)b * total;
     int tcnt = 0, fill = 0;
-    if (tid == 0) ctl[0] = 0;
-    __syncthreads();
-    for (size_t e0 = 0; e0 < total; e0 += 256) {
-        // entries that can still enter the list are gathered until 256 could overflow the batch
-        const size_t e = e0 + tid;
-        uint64_t key = ~0ull;
-        uint32_t id = CZ_NONE;
-        if (e < total) {
-            key = part_key[at + e];
-            id = part_id[at + e];
+    if (tid == 0) ctl[4] = 0;
+    for (uint32_t p0 = 0; p0 < n_parts; p0 += 256) {
+        const uint32_t p = p0 + tid;
+        const uint32_t mine = p < n_parts ? part_count[(size_t)b * n_parts + p] : 0;
+        uint32_t run = mine;
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t up = __shfl_up(run, o, 64);
+            if (lane >= o) run += up;
         }
-        const bool want = id != CZ_NONE && (tcnt < (int)k || czh::key_lt(key, id, tkey[k - 1], tid_[k - 1]));
-        const int add = __syncthreads_count(want);
-        if (fill + add > 256) {
-            tcnt = topk_merge_batch(fill, bkey, bid, tkey, tid_, tcnt, (int)k);
-            if (tid == 0) ctl[0] = 0;
-            fill = 0;
-            __syncthreads();
+        __syncthreads();
+        if (lane == 63) ctl[wave] = run;
+        __syncthreads();
+        for (int w = 0; w < wave; w++) run += ctl[w];
+        first[tid] = run - mine;
+        if (tid == 255) first[256] = run;
+        __syncthreads();
+        const uint32_t total = first[256];
+        for (uint32_t e0 = 0; e0 < total; e0 += 256) {
+            // entries that can still enter the list are gathered until 256 could overflow the batch
+            const uint32_t e = e0 + tid;
+            uint64_t key = ~0ull;
+            uint32_t id = CZ_NONE;
+            if (e < total) {
+                uint32_t lo = 0, hi = 256;  // the part: the last one with first <= e
+                while (hi - lo > 1) {
+                    const uint32_t mid = (lo + hi) >> 1;
+                    if (first[mid] <= e) lo = mid;
+                    else hi = mid;
+                }
+                const size_t at = ((size_t)b * n_parts + p0 + lo) * k + (e - first[lo]);
+                key = part_key[at];
+                id = part_id[at];
+            }
+            const bool want = id != CZ_NONE && (tcnt < (int)k || czh::key_lt(key, id, tkey[k - 1], tid_[k - 1]));
+            const int add = __syncthreads_count(want);
+            if (fill + add > 256) {
+                tcnt = topk_merge_batch(fill, bkey, bid, tkey, tid_, tcnt, (int)k);
+                if (tid == 0) ctl[4] = 0;
+                fill = 0;
+                __syncthreads();
+            }
+            if (want) {
+                const uint32_t at = atomicAdd(&ctl[4], 1u);  // (the order within a batch does not matter: entries are ranked)
+                bkey[at] = key;
+                bid[at] = id;
+            }
+            fill += add;
         }
-        if (want) {
-            const uint32_t p = atomicAdd(&ctl[0], 1u);  // (the order within a batch does not matter: entries are ranked)
-            bkey[p] = key;
-            bid[p] = id;
-        }
-        fill += add;
     }
     tcnt = topk_merge_batch(fill, bkey, bid, tkey, tid_, tcnt, (int)k);
     if (tid >= 64) return;
@@ -750,7 +831,7 @@ ProductPlan product_plan(const Rows &t, uint32_t B, bool near, cz::Carve &c) {
     p.ct = blocks4 >= 4 && p.steps * 4 <= 64 ? 4 : blocks4 >= 2 && p.steps * 2 <= 64 ? 2 : 1;
     p.lds = p.ct * p.steps * 1024;
     p.grid_y = (blocks4 + p.ct - 1) / p.ct;
-    const uint32_t per_cu = std::max(1u, std::min(4u, 160u * 1024 / p.lds));
+    const uint32_t per_cu = std::max(1u, std::min((uint32_t)residents((int)p.ct, (int)t.gshift), 160u * 1024 / p.lds));
     p.grid_x = std::max(1u, std::min((p.n_tiles + 3) / 4, std::max(1u, 256 * per_cu / p.grid_y)));
     p.digits = c.take<u32x4>((size_t)blocks4 * p.steps * 64);
     p.exponent = c.take<int>(B);
@@ -766,22 +847,30 @@ float score_error_unit(const Rows &t) {
     return 1.01f * (3.f * (float)(t.groups + 4) * 0x1p-24f + sqrtf((float)t.dim) * 0x1p-31f + 0x1p-21f);
 }
 
-template <int CT, int GS, bool NEAR>
+template <int CT, int GS, bool SW, bool NEAR>
 int launch_product_as(const Rows &t, const ProductPlan &p, uint32_t B, float *out, const Near &near, hipStream_t stream) {
-    auto kernel = q4_product_kernel<CT, GS, NEAR>;
+    auto kernel = q4_product_kernel<CT, GS, SW, NEAR>;
     if (p.lds > 65536) CZ_HIP(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.lds));
     hipLaunchKernelGGL(kernel, dim3(p.grid_x, p.grid_y), dim3(256), p.lds, stream, t, p.digits, p.exponent, B, p.steps, out, near);
     return CZ_OK;
 }
+template <int CT, int GS, bool NEAR>
+int launch_product_gs(const Rows &t, const ProductPlan &p, uint32_t B, float *out, const Near &near, hipStream_t stream) {
+    // whole batches of scales, each row's aligned to the load: rows of whole 128-byte lines of codes
+    const bool sw = t.chunks % 32 == 0 && (reinterpret_cast<uintptr_t>(t.scales) & 15) == 0;
+    return sw ? launch_product_as<CT, GS, true, NEAR>(t, p, B, out, near, stream) : launch_product_as<CT, GS, false, NEAR>(t, p, B, out, near, stream);
+}
 template <int CT, bool NEAR>
 int launch_product_ct(const Rows &t, const ProductPlan &p, uint32_t B, float *out, const Near &near, hipStream_t stream) {
-    if (t.gshift == 5) return launch_product_as<CT, 5, NEAR>(t, p, B, out, near, stream);
-    if (t.gshift == 6) return launch_product_as<CT, 6, NEAR>(t, p, B, out, near, stream);
-    return launch_product_as<CT, 7, NEAR>(t, p, B, out, near, stream);
+    if (t.gshift == 5) return launch_product_gs<CT, 5, NEAR>(t, p, B, out, near, stream);
+    if (t.gshift == 6) return launch_product_gs<CT, 6, NEAR>(t, p, B, out, near, stream);
+    return launch_product_gs<CT, 7, NEAR>(t, p, B, out, near, stream);
 }
 template <bool NEAR>
 int launch_product(const Rows &t, const ProductPlan &p, const float *q, uint32_t B, float *out, const Near &near, hipStream_t stream) {
-    hipLaunchKernelGGL(q4_digits_kernel, dim3((B + 3) / 4), dim3(256), 0, stream, q, B, t.dim, p.steps, (uint32_t *)p.digits, p.exponent, p.qnorm);
+    const uint32_t fixed = p.steps * 1024;  // the four queries' fixed point
+    if (fixed > 65536) CZ_HIP(hipFuncSetAttribute((const void *)q4_digits_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)fixed));
+    hipLaunchKernelGGL(q4_digits_kernel, dim3((B + 3) / 4), dim3(256), fixed, stream, q, B, t.dim, p.steps, (uint32_t *)p.digits, p.exponent, p.qnorm);
     if (p.ct == 4) return launch_product_ct<4, NEAR>(t, p, B, out, near, stream);
     if (p.ct == 2) return launch_product_ct<2, NEAR>(t, p, B, out, near, stream);
     return launch_product_ct<1, NEAR>(t, p, B, out, near, stream);
@@ -797,7 +886,7 @@ struct KnnPlan {
     uint32_t chunks, tiles_per_chunk;
     bool filtered;         // scores first, f64 distances of the tiles that can hold a result only
     uint64_t *part_key;
-    uint32_t *part_id;
+    uint32_t *part_id, *part_count;
     ProductPlan product;
     float *tile_score, *tile_norm, *best, *need;
     uint32_t n_best;
@@ -807,14 +896,14 @@ KnnPlan knn_plan(const Rows &t, uint32_t B, uint32_t k, void *ws) {
     KnnPlan p{};
     const uint32_t n_tiles = (uint32_t)(((uint64_t)t.n + kTile - 1) / kTile);
     // 256 rows are a batch of the list; enough workgroups to fill the chip, few enough lists to join
-    uint32_t chunks = std::min((n_tiles + 3) / 4, std::max(1u, 2048 / B));
+    uint32_t chunks = std::min(n_tiles, std::max(1u, 2048 / B));
     chunks = std::max(1u, std::min(chunks, std::max(16u, 65536 / k)));
     p.tiles_per_chunk = std::max(1u, (n_tiles + chunks - 1) / chunks);
-    p.tiles_per_chunk = (p.tiles_per_chunk + 3) & ~3u;
     p.chunks = std::max(1u, (n_tiles + p.tiles_per_chunk - 1) / p.tiles_per_chunk);
     cz::Carve c(ws);
     p.part_key = c.take<uint64_t>((size_t)B * p.chunks * k);
     p.part_id = c.take<uint32_t>((size_t)B * p.chunks * k);
+    p.part_count = c.take<uint32_t>((size_t)B * p.chunks);
     p.filtered = n_tiles >= 4 * (uint64_t)k && n_tiles >= 512;
     if (p.filtered) {
         p.product = product_plan(t, B, true, c);
@@ -1030,7 +1119,7 @@ extern "C" int cz_q4_knn(int metric, const uint8_t *codes, const uint16_t *scale
     if ((rc = cz::scratch_of(ws, ws_bytes, cz_q4_workspace(n, dim, group, B, k), own, &base))) return rc;
     t.codes = codes;
     t.scales = scales;
-    const size_t smem = 256 * 16 + (size_t)k * 12 + 48 + (size_t)dim * 4;
+    const size_t smem = 256 * 16 + (size_t)k * 12 + 48 + (size_t)t.chunks * 64;
     const uint32_t lpr = lanes_per_row(t.chunks);
     const uint32_t turn = turn_of(t);
     for (uint32_t b0 = 0; b0 < B; b0 += turn) {
@@ -1049,11 +1138,15 @@ extern "C" int cz_q4_knn(int metric, const uint8_t *codes, const uint16_t *scale
             }
 #define CZ_Q4_CALL(L)                                                                                                              \
     hipLaunchKernelGGL((q4_scan_kernel<L>), dim3(p.chunks, nb), dim3(256), smem, stream, metric, t, q, k, p.tiles_per_chunk, cand, \
-                       p.part_key, p.part_id)
+                       p.part_key, p.part_id, p.part_count)
+#define CZ_Q4_ALLOW(L) CZ_HIP(hipFuncSetAttribute((const void *)q4_scan_kernel<L>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem))
+            if (smem > 65536) CZ_Q4_LANES(lpr, CZ_Q4_ALLOW);
             CZ_Q4_LANES(lpr, CZ_Q4_CALL);
 #undef CZ_Q4_CALL
+#undef CZ_Q4_ALLOW
         }
-        hipLaunchKernelGGL(q4_join_kernel, dim3(nb), dim3(256), 256 * 12 + (size_t)k * 12 + 16, stream, p.part_key, p.part_id, p.chunks, k,
+        hipLaunchKernelGGL(q4_join_kernel, dim3(nb), dim3(256), 256 * 16 + (size_t)k * 12 + 32, stream, p.part_key, p.part_id,
+                           p.part_count, p.chunks, k,
                            has_radius, radius, out_ids + (size_t)b0 * k, out_dist + (size_t)b0 * k, out_count + b0);
     }
     rc = launched("cz_q4_knn");
