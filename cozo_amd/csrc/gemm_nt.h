@@ -26,6 +26,10 @@ struct Bf16 {
     typedef __bf16 T;
     static constexpr uint32_t kStep = 64;  // elements of a 128-byte step
 };
+struct F16 {
+    typedef _Float16 T;
+    static constexpr uint32_t kStep = 64;
+};
 struct F32 {
     typedef float T;
     static constexpr uint32_t kStep = 32;
@@ -33,6 +37,9 @@ struct F32 {
 
 __device__ __forceinline__ void mma(Bf16, const u32x4 &a, const u32x4 &b, f32x16 &c) {
     c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ void mma(F16, const u32x4 &a, const u32x4 &b, f32x16 &c) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 __device__ __forceinline__ void mma(F32, const u32x4 &a, const u32x4 &b, f32x16 &c) {
     const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
@@ -47,8 +54,13 @@ struct Operand {
     uint32_t rows;
 };
 
-template <class E, int BM, int BN, int WM, int WN>
+// BM x BN by WM x WN waves.  What bounds it is LDS: a wave reads (BM / WM + BN / WN) * 32 bytes per k of 16 for BM / WM * BN / WN products.
+// Measured with 1024 rows of B, 1M rows of A, k = 768, bf16: 128 x 128 by 2 x 2 904 TFLOP/s, 256 x 256 by 2 x 4 1177 (a library's
+// 8192^3 product: 1537); more steps kept in LDS, fragments read ahead and tiles run into each other gave no more than either.
+template <class E, int BM_, int BN_, int WM_, int WN_>
 struct Tile {
+    typedef E Elem;
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
     static constexpr int kThreads = 64 * WM * WN;
     static constexpr int MT = BM / WM / 32, NT = BN / WN / 32;
     static constexpr int kBytes = (BM + BN) * 128;  // LDS of one step

@@ -5,6 +5,7 @@
 
 #include "call.h"
 #include "distance.h"
+#include "gemm_nt.h"
 #include "topk.h"
 
 using namespace czd;
@@ -453,6 +454,194 @@ q4_product_kernel(Rows t, const u32x4 *__restrict__ digits, const int *__restric
     }
 }
 
+// ---- scores of many queries: an f16 matrix product ----------------------------------------------------------------------
+// For a large batch the search's scores come from a product in f16 (the f64 distances decide, so a score only has to be within a bound that
+// is known): a row's codes become f16 once per 256 queries instead of once per 4, and one matrix instruction does what the digits take four
+// for.  Both sides are scaled by a power of two to a norm of at most 2^8, so that nothing that matters is below f16's normal range:
+//   error <= |q| |x| (2^-11 of rounding the query + sqrt(dim) 2^-20 of what is flushed + dim 2^-24 of the f32 sums)
+// The loop is that of gemm_nt.h with the table's side made in registers: 16 bytes of codes (32 elements) a thread and step, loaded two steps
+// ahead, four packed f16 operations per 4 elements.  1M x 768, 1024 queries: XXX.
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+// the element (of 8) at each place of a 16-byte piece: a dword's nibbles are taken 16 bits apart
+__device__ __forceinline__ uint32_t element_of_place(uint32_t p) { return (p >> 1) + (p & 1) * 4; }
+
+// one wave per query: its f16 form [steps * 64] in the pieces' order, its exponent (value = form * 2^exponent) and norm
+__global__ void __launch_bounds__(256)
+q4_halves_kernel(const float *__restrict__ q, uint32_t B, uint32_t dim, uint32_t steps, _Float16 *__restrict__ out, int *__restrict__ exponent,
+                 float *__restrict__ norm) {
+    const uint32_t b = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63, width = steps * 64;
+    if (b >= B) return;
+    const float *row = q + (uint64_t)b * dim;
+    double s2 = 0.0;
+    for (uint32_t i = lane; i < dim; i += 64) s2 = fma((double)row[i], (double)row[i], s2);
+    for (int o = 32; o; o >>= 1) s2 += __shfl_xor(s2, o, 64);
+    // (beyond 2^96, an infinity or NaN among it: no score, every row is looked at)
+    const bool fine = s2 < 0x1p192;
+    int e = 0;
+    if (fine && s2 > 0.0) {
+        (void)frexp(s2, &e);
+        e = ((e + 1) >> 1) - 8;  // norm < 2^(e + 8)
+    }
+    if (lane == 0) {
+        exponent[b] = e;
+        norm[b] = fine ? __double2float_ru(sqrt(s2)) : __builtin_nanf("");
+    }
+    for (uint32_t i = lane; i < width; i += 64) {
+        const uint32_t el = (i & ~7u) + element_of_place(i & 7);
+        out[(uint64_t)b * width + i] = fine && el < dim ? (_Float16)ldexpf(row[el], -e) : (_Float16)0.f;
+    }
+}
+
+// largest norm of each tile's rows (those that are finite)
+__global__ void __launch_bounds__(256) q4_tile_norm_kernel(const float *__restrict__ sqnorms, uint32_t n, float *__restrict__ tile_norm) {
+    const uint64_t tile = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6), r = tile * kTile + (threadIdx.x & 63);
+    if (tile * kTile >= n) return;
+    const float sq = r < n ? sqnorms[r] : 0.f;
+    float x = sq < __builtin_inff() ? sq : 0.f;
+    for (int o = 32; o; o >>= 1) x = fmaxf(x, __shfl_xor(x, o, 64));
+    if ((threadIdx.x & 63) == 0) tile_norm[tile] = sqrtf(x) * 1.0001f + 1e-22f;
+}
+
+// scores [tile][ldb] of 64-row tiles: a workgroup keeps BN queries and goes over its stretch of the table, BM rows at a time
+template <class G, int GS>
+__global__ void __launch_bounds__(G::kThreads)
+q4_scores_kernel(Rows t, gemm::Operand Q, const int *__restrict__ exponent, uint32_t steps, Near near, float *__restrict__ score, uint32_t ldb,
+                 uint32_t n_blocks, uint32_t blocks_per_part) {
+    constexpr int BM = G::BM, BN = G::BN, TW = G::MT / 2;  // search tiles of a wave
+    static_assert(G::kThreads == 2 * BM, "two threads make a row of a step");
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    float2 *rowf = (float2 *)(lds + G::kLds);  // [BM] factor and addend that turn a product into a score
+    const int tid = threadIdx.x, lane = tid & 63, mine = tid >> 1, half = tid & 1;
+    const uint32_t qt = (Q.rows + BN - 1) / BN, at = blockIdx.x / 8;
+    const uint32_t n0 = at % qt * BN, part = at / qt * 8 + blockIdx.x % 8;  // (a stretch's workgroups on one XCD)
+    const uint32_t k0 = part * blocks_per_part, k1 = min(n_blocks, k0 + blocks_per_part);
+    const uint32_t row_bytes = t.chunks * 4;
+    float best[G::NT], qn[G::NT];
+    int qe[G::NT];
+#pragma unroll
+    for (int j = 0; j < G::NT; j++) {
+        const uint32_t b = min(n0 + G::wave_col() + j * 32 + (lane & 31), Q.rows - 1);
+        best[j] = -__builtin_inff();
+        qn[j] = near.qnorm[b];
+        qe[j] = exponent[b];
+    }
+    const char *src[G::NB];
+    G::rows_of(Q, n0, src);
+    for (uint32_t blk = k0; blk < k1; blk++) {
+        const uint64_t r = (uint64_t)blk * BM + mine, safe = min(r, (uint64_t)t.n - 1);
+        const uint8_t *codes = t.codes + safe * row_bytes;
+        const uint16_t *scales = t.scales + safe * t.groups;
+        u32x4 w;
+        uint16_t sb;
+        auto load = [&](uint32_t s) {
+            w = *(const u32x4 *)(codes + min(s * 32 + half * 16, row_bytes - 16));  // (past the row's end: times zeros of the query)
+            sb = scales[min(GS == 5 ? 2 * s + half : GS == 6 ? s : s >> 1, t.groups - 1)];
+        };
+        load(0);
+        G::copy(src, 0, lds + BM * 128);
+        const float sq = near.sqnorms[safe];
+        int e = 0;
+        const bool finite = sq < __builtin_inff();
+        if (finite && sq > 0.f) {
+            (void)frexpf(sq, &e);
+            e = ((e + 1) >> 1) - 8;
+        }
+        const float down = finite ? ldexpf(1.f, -e) : 0.f;  // (a row that is not finite: zeros, it is looked at anyway)
+        if (half == 0) {
+            float2 f = make_float2(0.f, -__builtin_inff());
+            if (r < t.n) {
+                const bool unsure = !finite || (near.metric == CZ_COSINE && sq > 0.f && sq < 1e-30f);
+                if (unsure) f.y = __builtin_inff();
+                else if (near.metric == CZ_COSINE) {
+                    if (sq > 0.f) f = make_float2(ldexpf(rsqrtf(sq), e), 0.f);
+                } else {
+                    f = near.metric == CZ_IP ? make_float2(ldexpf(1.f, e), 0.f) : make_float2(ldexpf(2.f, e), -sq);
+                }
+            }
+            rowf[mine] = f;
+        }
+        auto store = [&](char *to) {  // the loaded 32 elements as f16, at their places of the operand's row
+            const _Float16 s = (_Float16)(bf16_to_f32(sb) * down);
+            const f16x2 s2 = {finite ? s : (_Float16)0.f, finite ? s : (_Float16)0.f}, off = {(_Float16)1032.f, (_Float16)1032.f};
+#pragma unroll
+            for (int d = 0; d < 4; d++) {
+                const uint32_t u = w[d] ^ 0x88888888u;
+                u32x4 o;
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    const f16x2 h = __builtin_bit_cast(f16x2, ((u >> (4 * x)) & 0x000F000Fu) | 0x64006400u) - off;  // 1024 + code + 8 - 1032
+                    o[x] = __builtin_bit_cast(uint32_t, h * s2);
+                }
+                *(u32x4 *)(to + mine * 128 + (((half * 4 + d) ^ (mine & 7)) * 16)) = o;
+            }
+        };
+        store(lds);
+        if (steps > 1) load(1);
+        G g;
+        g.zero();
+        for (uint32_t s = 0; s < steps; s++) {
+            char *cur = lds + (s & 1) * G::kBytes, *nxt = lds + (~s & 1) * G::kBytes;
+            G::arrived();
+            if (s + 1 < steps) {
+                G::copy(src, (uint64_t)(s + 1) * 128, nxt + BM * 128);
+                store(nxt);
+                if (s + 2 < steps) load(s + 2);
+            }
+            g.step(cur);
+        }
+        float top[G::NT][TW];
+#pragma unroll
+        for (int j = 0; j < G::NT; j++)
+#pragma unroll
+            for (int x = 0; x < TW; x++) top[j][x] = -__builtin_inff();
+#pragma unroll
+        for (int i = 0; i < G::MT; i++)
+#pragma unroll
+            for (int r4 = 0; r4 < 4; r4++) {
+                float2 f[4];
+#pragma unroll
+                for (int x = 0; x < 4; x++) f[x] = rowf[G::wave_row() + i * 32 + 8 * r4 + 4 * (lane >> 5) + x];
+#pragma unroll
+                for (int j = 0; j < G::NT; j++)
+#pragma unroll
+                    for (int x = 0; x < 4; x++)
+                        top[j][i / 2] = fmaxf(top[j][i / 2], fmaf(ldexpf(g.acc[i][j][4 * r4 + x], qe[j]), f[x].x, f[x].y));
+            }
+#pragma unroll
+        for (int x = 0; x < TW; x++) {
+            const uint32_t tile = blk * (BM / kTile) + G::wave_row() / kTile + x;
+            if (tile >= near.n_tiles) break;  // (uniform)
+            const float xn = near.tile_norm[tile];
+#pragma unroll
+            for (int j = 0; j < G::NT; j++) {
+                const uint32_t b = n0 + G::wave_col() + j * 32 + (lane & 31);
+                const float v = fmaxf(top[j][x], __shfl_xor(top[j][x], 32, 64));
+                if (b < Q.rows && lane < 32) score[(uint64_t)tile * ldb + b] = v;
+                best[j] = fmaxf(best[j], v - score_error(near.metric, near.err, qn[j], xn));
+            }
+        }
+        __syncthreads();  // LDS is free for the next rows
+    }
+#pragma unroll
+    for (int j = 0; j < G::NT; j++) {
+        const uint32_t b = n0 + G::wave_col() + j * 32 + (lane & 31);
+        if (b < Q.rows && lane < 32) near.best[(uint64_t)b * near.n_best + part * G::WM + (tid >> 6) / G::WN] = best[j];
+    }
+}
+
+// [rows][ld] -> [cols][rows], 64 x 64 through LDS
+__global__ void __launch_bounds__(256)
+q4_turn_kernel(const float *__restrict__ x, uint32_t rows, uint32_t cols, uint32_t ld, float *__restrict__ out) {
+    __shared__ float tile[64][65];
+    const uint32_t r0 = blockIdx.x * 64, c0 = blockIdx.y * 64, c = threadIdx.x & 63, w = threadIdx.x >> 6;
+    for (uint32_t i = w; i < 64; i += 4)
+        if (r0 + i < rows && c0 + c < cols) tile[i][c] = x[(uint64_t)(r0 + i) * ld + c0 + c];
+    __syncthreads();
+    for (uint32_t i = w; i < 64; i += 4)
+        if (c0 + i < cols && r0 + c < rows) out[(uint64_t)(c0 + i) * rows + r0 + c] = tile[c][i];
+}
+
 // order-preserving u32 of an f32; NaN as -inf
 __device__ __forceinline__ uint32_t order_of(float f) {
     if (f != f) f = -__builtin_inff();
@@ -689,38 +878,65 @@ q4_scan_kernel(int metric, Rows t, const float *__restrict__ queries, uint32_t k
     if (tid == 0) part_count[part] = (uint32_t)tcnt;
 }
 
-// one workgroup per query: the partial lists joined, the radius cut, the padding
+// one workgroup per query: the partial lists joined, the radius cut, the padding.  Merging a full batch of 256 takes some 20 us, so the k-th
+// smallest of 256 lists' heads, which k entries are sure not to be behind, leaves few to merge (one query, 157 lists: 76 -> XXX us).
+constexpr size_t join_lds(size_t k) { return 256 * 24 + k * 12 + 257 * 4 + 8 * 4 + 8; }
 __global__ void __launch_bounds__(256)
 q4_join_kernel(const uint64_t *__restrict__ part_key, const uint32_t *__restrict__ part_id, const uint32_t *__restrict__ part_count,
                uint32_t n_parts, uint32_t k, int has_radius, double radius, uint32_t *__restrict__ out_ids, double *__restrict__ out_dist,
                uint32_t *__restrict__ out_count) {
     extern __shared__ __attribute__((aligned(16))) char smem_raw[];
     uint64_t *bkey = (uint64_t *)smem_raw;   // [256]
-    uint64_t *tkey = bkey + 256;              // [k]
-    uint32_t *bid = (uint32_t *)(tkey + k);   // [256]
-    uint32_t *tid_ = bid + 256;               // [k]
+    uint64_t *hkey = bkey + 256;              // [256] heads of 256 lists
+    uint64_t *tkey = hkey + 256;              // [k]
+    uint64_t *limit_key = tkey + k;           // [1]
+    uint32_t *bid = (uint32_t *)(limit_key + 1);  // [256]
+    uint32_t *hid = bid + 256;                // [256]
+    uint32_t *tid_ = hid + 256;               // [k]
     uint32_t *first = tid_ + k;               // [257] entries of the parts before this one (of 256 parts at a time)
-    uint32_t *ctl = first + 257;              // [5]
+    uint32_t *ctl = first + 257;              // [0..3] waves' sums, [4] batch fill, [5] limit's id
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const uint32_t b = blockIdx.x;
     int tcnt = 0, fill = 0;
-    if (tid == 0) ctl[4] = 0;
+    if (tid == 0) {
+        ctl[4] = 0;
+        ctl[5] = CZ_NONE;
+        limit_key[0] = ~0ull;
+    }
     for (uint32_t p0 = 0; p0 < n_parts; p0 += 256) {
         const uint32_t p = p0 + tid;
-        const uint32_t mine = p < n_parts ? part_count[(size_t)b * n_parts + p] : 0;
+        const size_t list = (size_t)b * n_parts + p;
+        const uint32_t mine = p < n_parts ? part_count[list] : 0;
+        const uint64_t head_key = mine ? part_key[list * k] : ~0ull;
+        const uint32_t head_id = mine ? part_id[list * k] : CZ_NONE;
+        hkey[tid] = head_key;
+        hid[tid] = head_id;
         uint32_t run = mine;
         for (int o = 1; o < 64; o <<= 1) {
             const uint32_t up = __shfl_up(run, o, 64);
             if (lane >= o) run += up;
         }
-        __syncthreads();
         if (lane == 63) ctl[wave] = run;
         __syncthreads();
         for (int w = 0; w < wave; w++) run += ctl[w];
         first[tid] = run - mine;
         if (tid == 255) first[256] = run;
+        if (mine) {
+            uint32_t rank = 0;
+#pragma unroll 8
+            for (int t = 0; t < 256; t++) {
+                const uint64_t other = hkey[t];
+                rank += (uint32_t)((other < head_key) | ((other == head_key) & (hid[t] < head_id)));
+            }
+            if (rank == k - 1 && czh::key_lt(head_key, head_id, limit_key[0], ctl[5])) {  // (ids differ: one thread)
+                limit_key[0] = head_key;
+                ctl[5] = head_id;
+            }
+        }
         __syncthreads();
         const uint32_t total = first[256];
+        const uint64_t last_key = limit_key[0];
+        const uint32_t last_id = ctl[5];
         for (uint32_t e0 = 0; e0 < total; e0 += 256) {
             // entries that can still enter the list are gathered until 256 could overflow the batch
             const uint32_t e = e0 + tid;
@@ -737,7 +953,8 @@ q4_join_kernel(const uint64_t *__restrict__ part_key, const uint32_t *__restrict
                 key = part_key[at];
                 id = part_id[at];
             }
-            const bool want = id != CZ_NONE && (tcnt < (int)k || czh::key_lt(key, id, tkey[k - 1], tid_[k - 1]));
+            const bool want = id != CZ_NONE && !czh::key_lt(last_key, last_id, key, id) &&
+                              (tcnt < (int)k || czh::key_lt(key, id, tkey[k - 1], tid_[k - 1]));
             const int add = __syncthreads_count(want);
             if (fill + add > 256) {
                 tcnt = topk_merge_batch(fill, bkey, bid, tkey, tid_, tcnt, (int)k);
@@ -752,6 +969,7 @@ q4_join_kernel(const uint64_t *__restrict__ part_key, const uint32_t *__restrict
             }
             fill += add;
         }
+        __syncthreads();  // heads, sums and the limit are free
     }
     tcnt = topk_merge_batch(fill, bkey, bid, tkey, tid_, tcnt, (int)k);
     if (tid >= 64) return;
@@ -876,6 +1094,16 @@ int launch_product(const Rows &t, const ProductPlan &p, const float *q, uint32_t
     return launch_product_ct<1, NEAR>(t, p, B, out, near, stream);
 }
 
+// Up to so many queries the digits' product (100 us for each 16 of them at 1M x 768) is the faster way to the scores.
+constexpr uint32_t kDigitQueries = 32;
+using Tile128 = gemm::Tile<gemm::F16, 128, 128, 2, 2>;
+using Tile256 = gemm::Tile<gemm::F16, 256, 256, 2, 4>;
+
+// c of score_error for the f16 product (derived at its kernel); the cosine's own rounding and the bound's as for the digits
+float half_error_unit(const Rows &t) {
+    return 1.01f * (0x1p-11f + sqrtf((float)t.dim) * 0x1p-20f + (float)t.dim * 0x1p-24f + 0x1p-21f);
+}
+
 // queries of one launch; a larger batch goes in turns through the same scratch (at most 1 GiB of tile scores)
 uint32_t turn_of(const Rows &t) {
     const uint64_t n_tiles = std::max<uint64_t>(1, ((uint64_t)t.n + kTile - 1) / kTile);
@@ -888,7 +1116,12 @@ struct KnnPlan {
     uint64_t *part_key;
     uint32_t *part_id, *part_count;
     ProductPlan product;
-    float *tile_score, *tile_norm, *best, *need;
+    int halves;            // scores by the f16 product: 0 no, 1 with 128 x 128 tiles, 2 with 256 x 256
+    uint32_t steps, parts, ldb;
+    _Float16 *q16;
+    int *exponent;
+    float *turned;
+    float *qnorm, *tile_score, *tile_norm, *best, *need;
     uint32_t n_best;
     size_t bytes;
 };
@@ -906,8 +1139,22 @@ KnnPlan knn_plan(const Rows &t, uint32_t B, uint32_t k, void *ws) {
     p.part_count = c.take<uint32_t>((size_t)B * p.chunks);
     p.filtered = n_tiles >= 4 * (uint64_t)k && n_tiles >= 512;
     if (p.filtered) {
-        p.product = product_plan(t, B, true, c);
-        p.n_best = p.product.grid_x * 4;
+        p.steps = (t.groups << t.gshift) / 64 + ((t.groups << t.gshift) % 64 != 0);
+        p.halves = B <= kDigitQueries ? 0 : B <= 128 ? 1 : 2;
+        if (p.halves) {
+            const uint32_t b = p.halves == 2 ? 256 : 128, qt = (B + b - 1) / b, blocks = (t.n + b - 1) / b, resident = p.halves == 2 ? 256 : 512;
+            p.parts = std::max(8u, std::min((blocks + 7) / 8 * 8, resident / qt / 8 * 8));
+            p.n_best = p.parts * 2;
+            p.ldb = (B + 31) / 32 * 32;
+            p.q16 = c.take<_Float16>((size_t)B * p.steps * 64);
+            p.exponent = c.take<int>(B);
+            p.qnorm = c.take<float>(B);
+            p.turned = c.take<float>((size_t)n_tiles * p.ldb);
+        } else {
+            p.product = product_plan(t, B, true, c);
+            p.n_best = p.product.grid_x * 4;
+            p.qnorm = p.product.qnorm;
+        }
         p.tile_score = c.take<float>((size_t)B * n_tiles);
         p.tile_norm = c.take<float>(n_tiles);
         p.best = c.take<float>((size_t)B * p.n_best);
@@ -915,6 +1162,27 @@ KnnPlan knn_plan(const Rows &t, uint32_t B, uint32_t k, void *ws) {
     }
     p.bytes = c.used();
     return p;
+}
+
+template <class G>
+int launch_scores(const Rows &t, const KnnPlan &p, uint32_t B, const Near &near, hipStream_t stream) {
+    const gemm::Operand Q{(const char *)p.q16, (uint64_t)p.steps * 128, B};
+    const uint32_t blocks = (uint32_t)(((uint64_t)t.n + G::BM - 1) / G::BM), lds = G::kLds + G::BM * 8, qt = (B + G::BN - 1) / G::BN;
+    auto kernel = t.gshift == 5 ? q4_scores_kernel<G, 5> : t.gshift == 6 ? q4_scores_kernel<G, 6> : q4_scores_kernel<G, 7>;
+    CZ_HIP(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    hipLaunchKernelGGL(kernel, dim3(p.parts * qt), dim3(G::kThreads), lds, stream, t, Q, p.exponent, p.steps, near, p.turned, p.ldb, blocks,
+                       (blocks + p.parts - 1) / p.parts);
+    return CZ_OK;
+}
+// the scores of every tile, what rows are sure to reach: by digits or in f16
+int launch_near(const Rows &t, const KnnPlan &p, const float *q, uint32_t B, const Near &near, hipStream_t stream) {
+    if (!p.halves) return launch_product<true>(t, p.product, q, B, nullptr, near, stream);
+    hipLaunchKernelGGL(q4_halves_kernel, dim3((B + 3) / 4), dim3(256), 0, stream, q, B, t.dim, p.steps, p.q16, p.exponent, p.qnorm);
+    hipLaunchKernelGGL(q4_tile_norm_kernel, dim3((near.n_tiles + 3) / 4), dim3(256), 0, stream, near.sqnorms, t.n, p.tile_norm);
+    const int rc = p.halves == 2 ? launch_scores<Tile256>(t, p, B, near, stream) : launch_scores<Tile128>(t, p, B, near, stream);
+    if (rc) return rc;
+    hipLaunchKernelGGL(q4_turn_kernel, dim3((near.n_tiles + 63) / 64, (B + 63) / 64), dim3(256), 0, stream, p.turned, near.n_tiles, B, p.ldb, p.tile_score);
+    return CZ_OK;
 }
 
 int check_codes(const uint8_t *codes, const uint16_t *scales) {
@@ -1130,11 +1398,11 @@ extern "C" int cz_q4_knn(int metric, const uint8_t *codes, const uint16_t *scale
             p = knn_plan(t, nb, k, base);
             Candidates cand{};
             if (p.filtered) {
-                const float err = score_error_unit(t);
-                const Near near{metric, sqnorms, err, p.product.qnorm, p.tile_score, p.tile_norm, p.best, p.product.n_tiles, p.n_best};
-                if ((rc = launch_product<true>(t, p.product, q, nb, nullptr, near, stream))) return rc;
+                const float err = p.halves ? half_error_unit(t) : score_error_unit(t);
+                const Near near{metric, sqnorms, err, p.qnorm, p.tile_score, p.tile_norm, p.best, (n + kTile - 1) / kTile, p.n_best};
+                if ((rc = launch_near(t, p, q, nb, near, stream))) return rc;
                 hipLaunchKernelGGL(q4_need_kernel, dim3(nb), dim3(1024), 0, stream, near, p.n_best < 4 * k, k, p.need);
-                cand = Candidates{p.tile_score, p.tile_norm, p.product.qnorm, p.need, err};
+                cand = Candidates{p.tile_score, p.tile_norm, p.qnorm, p.need, err};
             }
 #define CZ_Q4_CALL(L)                                                                                                              \
     hipLaunchKernelGGL((q4_scan_kernel<L>), dim3(p.chunks, nb), dim3(256), smem, stream, metric, t, q, k, p.tiles_per_chunk, cand, \
@@ -1145,7 +1413,7 @@ extern "C" int cz_q4_knn(int metric, const uint8_t *codes, const uint16_t *scale
 #undef CZ_Q4_CALL
 #undef CZ_Q4_ALLOW
         }
-        hipLaunchKernelGGL(q4_join_kernel, dim3(nb), dim3(256), 256 * 16 + (size_t)k * 12 + 32, stream, p.part_key, p.part_id,
+        hipLaunchKernelGGL(q4_join_kernel, dim3(nb), dim3(256), join_lds(k), stream, p.part_key, p.part_id,
                            p.part_count, p.chunks, k,
                            has_radius, radius, out_ids + (size_t)b0 * k, out_dist + (size_t)b0 * k, out_count + b0);
     }

@@ -42,36 +42,55 @@ xent_pack_kernel(const T *__restrict__ x, uint64_t ld, uint32_t n, uint32_t dim,
 }
 
 // out[d][r] = x[r][d] for d < dim, r < n, and zeros up to row length ldo; rows whose target is no row of the table are zeros too when
-// targets are given (what such a query holds, NaN included, must not reach a product with its zero weight)
+// targets are given (what such a query holds, NaN included, must not reach a product with its zero weight).  HBM bound: 64 x 64 through LDS,
+// 16 bytes of a row read and written at a time.  `wide`: rows of x are 16-byte aligned.  ldo is a multiple of 128 bytes.
 template <typename T>
 __global__ void __launch_bounds__(256)
-xent_transpose_kernel(const T *__restrict__ x, uint64_t ld, uint32_t n, uint32_t dim, const uint32_t *__restrict__ targets, uint32_t V,
+xent_transpose_kernel(const T *__restrict__ x, uint64_t ld, bool wide, uint32_t n, uint32_t dim, const uint32_t *__restrict__ targets, uint32_t V,
                       T *__restrict__ out, uint64_t ldo) {
+    constexpr int P = 16 / sizeof(T);  // elements of 16 bytes
+    typedef T Piece __attribute__((ext_vector_type(P)));
     __shared__ T tile[64][64 + 4 / sizeof(T)];
     const uint32_t r0 = blockIdx.x * 64, d0 = blockIdx.y * 64;
-    const uint32_t c = threadIdx.x & 63, q = threadIdx.x >> 6;
-    for (uint32_t i = q; i < 64; i += 4) {
-        const uint32_t r = r0 + i, d = d0 + c;
-        T v = (T)0.f;
-        if (r < n && d < dim && (!targets || has_answer(targets[r], V))) v = x[r * ld + d];
-        tile[i][c] = v;
+#pragma unroll
+    for (uint32_t i = 0; i < 16 / P; i++) {
+        const uint32_t at = i * 256 + threadIdx.x, row = at / (64 / P), c = at % (64 / P) * P, r = r0 + row, d = d0 + c;
+        Piece v;
+#pragma unroll
+        for (int j = 0; j < P; j++) v[j] = (T)0.f;
+        if (r < n && (!targets || has_answer(targets[r], V))) {
+            const T *src = x + r * ld + d;
+            if (wide && d + P <= dim) v = *(const Piece *)src;
+            else
+#pragma unroll
+                for (int j = 0; j < P; j++)
+                    if (d + j < dim) v[j] = src[j];
+        }
+#pragma unroll
+        for (int j = 0; j < P; j++) tile[row][c + j] = v[j];
     }
     __syncthreads();
-    for (uint32_t i = q; i < 64; i += 4) {
-        const uint32_t d = d0 + i, r = r0 + c;
-        if (d < dim && r < ldo) out[(uint64_t)d * ldo + r] = tile[c][i];
+#pragma unroll
+    for (uint32_t i = 0; i < 16 / P; i++) {
+        const uint32_t at = i * 256 + threadIdx.x, row = at / (64 / P), c = at % (64 / P) * P, d = d0 + row, r = r0 + c;
+        if (d >= dim || r >= ldo) continue;
+        Piece v;
+#pragma unroll
+        for (int j = 0; j < P; j++) v[j] = tile[c + j][row];
+        *(Piece *)(out + (uint64_t)d * ldo + r) = v;
     }
 }
 
-template <class E, int BM, int BN, int WM, int WN>
-__global__ void __launch_bounds__(64 * WM * WN)
-xent_forward_kernel(Operand W, uint32_t v0, Operand Q, uint32_t steps, float scale2, uint32_t n_tiles, uint32_t tiles_per_part,
+template <class G>
+__global__ void __launch_bounds__(G::kThreads)
+xent_forward_kernel(Operand W, Operand Q, uint32_t steps, float scale2, uint32_t n_tiles, uint32_t tiles_per_part,
                     uint32_t part0, float2 *__restrict__ parts) {
-    typedef gemm::Tile<E, BM, BN, WM, WN> G;
+    constexpr int BM = G::BM, BN = G::BN, WM = G::WM, WN = G::WN;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int lane = threadIdx.x & 63;
-    const uint32_t qt = (Q.rows + BN - 1) / BN;
-    const uint32_t n0 = blockIdx.x % qt * BN, part = blockIdx.x / qt;
+    // workgroups go round the 8 XCDs: those that share a stretch of the table are put on one, so that its L2 holds the stretch's tile
+    const uint32_t qt = (Q.rows + BN - 1) / BN, at = blockIdx.x / 8;
+    const uint32_t n0 = at % qt * BN, part = at / qt * 8 + blockIdx.x % 8;
     const uint32_t t0 = part * tiles_per_part, t1 = min(n_tiles, t0 + tiles_per_part);
     float m[G::NT], l[G::NT];
 #pragma unroll
@@ -161,12 +180,13 @@ xent_join_kernel(const float2 *__restrict__ parts, uint32_t n_parts, const T *__
 }
 
 // P of a piece: p[t][v] and pt[v][t], zeros where the piece or the queries end
-template <class E, int BM, int BN, int WM, int WN>
-__global__ void __launch_bounds__(64 * WM * WN)
+template <class G>
+__global__ void __launch_bounds__(G::kThreads)
 xent_weights_kernel(Operand W, uint32_t v0, uint32_t V, Operand Q, uint32_t steps, float scale, const uint32_t *__restrict__ targets,
-                    const float *__restrict__ lse, const float *__restrict__ grad_loss, typename E::T *__restrict__ p, uint64_t ldp,
-                    typename E::T *__restrict__ pt, uint32_t ldt) {
-    typedef gemm::Tile<E, BM, BN, WM, WN> G;
+                    const float *__restrict__ lse, const float *__restrict__ grad_loss, typename G::Elem::T *__restrict__ p, uint64_t ldp,
+                    typename G::Elem::T *__restrict__ pt, uint32_t ldt) {
+    typedef typename G::Elem E;
+    constexpr int BM = G::BM, BN = G::BN;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const uint32_t qt = (ldt + BN - 1) / BN;
     const uint32_t n0 = blockIdx.x % qt * BN, m0 = blockIdx.x / qt * BM;
@@ -204,25 +224,25 @@ xent_weights_kernel(Operand W, uint32_t v0, uint32_t V, Operand Q, uint32_t step
 }
 
 // grad_table rows of a piece: pt [rows][ldt] . qt [dim][ldt]^T
-template <class E, int BM, int BN, int WM, int WN>
-__global__ void __launch_bounds__(64 * WM * WN)
-xent_table_grad_kernel(Operand Pt, Operand Qt, uint32_t steps, typename E::T *__restrict__ out, uint32_t dim) {
-    typedef gemm::Tile<E, BM, BN, WM, WN> G;
+template <class G>
+__global__ void __launch_bounds__(G::kThreads)
+xent_table_grad_kernel(Operand Pt, Operand Qt, uint32_t steps, typename G::Elem::T *__restrict__ out, uint32_t dim) {
+    constexpr int BM = G::BM, BN = G::BN;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const uint32_t nt = (dim + BN - 1) / BN;
     const uint32_t n0 = blockIdx.x % nt * BN, m0 = blockIdx.x / nt * BM;
     G g;
     g.run(Pt, m0, Qt, n0, 0, steps, lds);
     g.each([&](uint32_t r, uint32_t c, float v) {
-        if (m0 + r < Pt.rows && n0 + c < dim) out[(uint64_t)(m0 + r) * dim + n0 + c] = down<typename E::T>(v);
+        if (m0 + r < Pt.rows && n0 + c < dim) out[(uint64_t)(m0 + r) * dim + n0 + c] = down<typename G::Elem::T>(v);
     });
 }
 
 // partial sums of grad_queries: part s gets p [T][k of stretch s] . wt [dim][k]^T, added to what the earlier pieces left there
-template <class E, int BM, int BN, int WM, int WN>
-__global__ void __launch_bounds__(64 * WM * WN)
+template <class G>
+__global__ void __launch_bounds__(G::kThreads)
 xent_query_grad_kernel(Operand P, Operand Wt, uint32_t steps, uint32_t steps_per_part, int add, float *__restrict__ parts, uint32_t dim) {
-    typedef gemm::Tile<E, BM, BN, WM, WN> G;
+    constexpr int BM = G::BM, BN = G::BN;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const uint32_t nt = (dim + BN - 1) / BN, mt = (P.rows + BM - 1) / BM;
     const uint32_t n0 = blockIdx.x % nt * BN, m0 = blockIdx.x / nt % mt * BM, s = blockIdx.x / (nt * mt);
@@ -266,16 +286,24 @@ struct Shape {
 
 struct Plan {
     uint32_t piece;        // table rows worked on at a time
-    uint32_t parts;        // forward: stretches of the whole table; backward: partial sums of grad_queries
-    uint32_t tiles_per_part;  // forward, tiles of a stretch
-    void *q, *w;           // packed copies (unaligned rows or a dim that is no multiple of a step), or null
+    uint32_t parts;        // forward: stretches of a piece (a multiple of 8); backward: partial sums of grad_queries
+    int fwd;               // forward's tile: 0 narrow, 1 small, 2 large
+    bool large_p, large_w, large_q;  // backward's tiles: of P, of grad_table, of grad_queries
+    void *q, *w;           // packed copies (unaligned rows or a dim that is no multiple of a step)
     void *qt, *wt, *p, *pt;
     float2 *stats;
     float *dq;
     size_t bytes;
 };
 
-constexpr int kBM = 128, kBN = 128, kWM = 2, kWN = 2;
+// Tiles of the four products.  Large: most products per byte of LDS; small: more workgroups when there are few tiles; and for a few
+// queries a narrow one, which does not spend the f32 matrix cores on columns that are not there.
+template <class E> using Large = gemm::Tile<E, 256, 256, 2, 4>;
+template <class E> using Small = gemm::Tile<E, 128, 128, 2, 2>;
+template <class E> using Narrow = gemm::Tile<E, 128, 32, 4, 1>;
+
+// every tile of `big` x `big` fills the chip's 256 CUs about as well as tiles of half the size would
+bool enough(uint64_t m, uint64_t n) { return ((m + 255) / 256) * ((n + 255) / 256) >= 192 && n > 128 && m > 128; }
 
 // rows that the matrix loop can read where they are
 bool direct(const void *x, uint64_t ld, uint32_t dim, uint32_t es) {
@@ -293,20 +321,23 @@ Plan make_plan(const Shape &s, bool grad, void *ws) {
     pl.q = c.take<uint8_t>((uint64_t)s.T * kp * es);
     pl.w = c.take<uint8_t>((uint64_t)pl.piece * kp * es);
     if (!grad) {
-        const uint32_t qt = (s.T + kBN - 1) / kBN;
-        // forward goes over the table piece by piece only where it has to be packed; the stretches are those of a piece either way
-        const uint32_t tiles = (std::min(s.V, pl.piece) + kBM - 1) / kBM;
-        pl.parts = std::max(1u, std::min(tiles, 1024 / qt));
-        pl.tiles_per_part = (tiles + pl.parts - 1) / pl.parts;
-        pl.parts = (tiles + pl.tiles_per_part - 1) / pl.tiles_per_part;
+        // a table that can be read where it is goes in one piece, another one packed piece by piece: stretches for the larger
+        pl.fwd = s.T <= 32 ? 0 : s.T > 128 && s.V >= 64 * 256 ? 2 : 1;
+        const uint32_t bm = pl.fwd == 2 ? 256 : 128, bn = pl.fwd == 2 ? 256 : pl.fwd == 1 ? 128 : 32;
+        const uint32_t qt = (s.T + bn - 1) / bn, tiles = (s.V + bm - 1) / bm, resident = pl.fwd == 2 ? 256 : pl.fwd == 1 ? 512 : 1024;
+        pl.parts = (uint32_t)up_to(std::max(1u, std::min(tiles, resident / qt)), 8);
         pl.stats = c.take<float2>((uint64_t)pl.parts * ((s.V + pl.piece - 1) / pl.piece) * s.T);
     } else {
         pl.qt = c.take<uint8_t>(s.dim * tp * es);
         pl.wt = c.take<uint8_t>((uint64_t)s.dim * pl.piece * es);
         pl.p = c.take<uint8_t>((uint64_t)s.T * pl.piece * es);
         pl.pt = c.take<uint8_t>(pl.piece * tp * es);
-        const uint32_t tiles = ((s.T + kBM - 1) / kBM) * ((s.dim + kBN - 1) / kBN);
-        pl.parts = std::max(1u, std::min({512 / tiles, 64u, pl.piece / 1024}));
+        const uint32_t nv = std::min(s.V, pl.piece);
+        pl.large_p = enough(nv, tp);
+        pl.large_w = enough(nv, s.dim);
+        pl.large_q = s.T > 128 && s.dim > 128;
+        const uint32_t b = pl.large_q ? 256 : 128, tiles = ((s.T + b - 1) / b) * ((s.dim + b - 1) / b);
+        pl.parts = std::max(1u, std::min({(pl.large_q ? 256 : 512) / tiles, 64u, pl.piece / 1024}));
         pl.dq = c.take<float>((uint64_t)pl.parts * s.T * s.dim);
     }
     pl.bytes = c.used();
@@ -325,91 +356,115 @@ void pack(const T *x, uint64_t ld, uint32_t n, uint32_t dim, void *out, uint32_t
     hipLaunchKernelGGL(xent_pack_kernel<T>, dim3(grid_of((uint64_t)n * ldo)), dim3(256), 0, stream, x, ld, n, dim, (T *)out, ldo);
 }
 
-template <class K>
-int allow_lds(K kernel, int bytes) {
-    if (bytes > 65536) CZ_HIP(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+// a kernel over tiles G, with the LDS that they ask for
+template <class G, class K, class... A>
+int launch(K kernel, uint32_t grid, hipStream_t stream, A... args) {
+    if (G::kLds > 65536) CZ_HIP(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, G::kLds));
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(G::kThreads), G::kLds, stream, args...);
     return CZ_OK;
+}
+uint32_t tiles_of(uint64_t n, int b) { return (uint32_t)((n + b - 1) / b); }
+
+template <class G>
+int forward_piece(const Operand &W, const Operand &Q, uint32_t steps, float scale2, uint32_t parts, uint32_t part0, float2 *stats, hipStream_t stream) {
+    const uint32_t tiles = tiles_of(W.rows, G::BM);
+    return launch<G>(xent_forward_kernel<G>, parts * tiles_of(Q.rows, G::BN), stream, W, Q, steps, scale2, tiles, (tiles + parts - 1) / parts, part0, stats);
 }
 
 template <class E>
 int forward(const Shape &s, const Plan &pl, const void *q_, const void *w_, const uint32_t *targets, float scale, float *loss, float *lse,
             hipStream_t stream) {
     typedef typename E::T T;
-    typedef gemm::Tile<E, kBM, kBN, kWM, kWN> G;
     const T *q = (const T *)q_, *w = (const T *)w_;
-    const uint32_t es = s.es(), kp = s.kp();
+    const uint32_t es = s.es(), kp = s.kp(), steps = kp / s.kstep();
     Operand Q{(const char *)q, s.ldq * es, s.T};
     if (!direct(q, s.ldq, s.dim, es)) {
         pack(q, s.ldq, s.T, s.dim, pl.q, kp, stream);
         Q = Operand{(const char *)pl.q, (uint64_t)kp * es, s.T};
     }
     const bool wd = direct(w, s.ldw, s.dim, es);
-    auto kernel = xent_forward_kernel<E, kBM, kBN, kWM, kWN>;
-    int rc = allow_lds(kernel, G::kLds);
-    if (rc) return rc;
+    const uint32_t piece = wd ? s.V : pl.piece;
     uint32_t parts = 0;
-    for (uint32_t v0 = 0; v0 < s.V; v0 += pl.piece) {
-        const uint32_t nv = std::min(pl.piece, s.V - v0);
+    for (uint32_t v0 = 0; v0 < s.V; v0 += piece) {
+        const uint32_t nv = std::min(piece, s.V - v0);
         Operand W{(const char *)(w + v0 * s.ldw), s.ldw * es, nv};
         if (!wd) {
             pack(w + v0 * s.ldw, s.ldw, nv, s.dim, pl.w, kp, stream);
             W = Operand{(const char *)pl.w, (uint64_t)kp * es, nv};
         }
-        const uint32_t tiles = (nv + kBM - 1) / kBM, here = (tiles + pl.tiles_per_part - 1) / pl.tiles_per_part;
-        hipLaunchKernelGGL(kernel, dim3(here * ((s.T + kBN - 1) / kBN)), dim3(G::kThreads), G::kLds, stream, W, v0, Q, kp / s.kstep(),
-                           scale * kLog2e, tiles, pl.tiles_per_part, parts, pl.stats);
-        parts += here;
+        const int rc = pl.fwd == 2   ? forward_piece<Large<E>>(W, Q, steps, scale * kLog2e, pl.parts, parts, pl.stats, stream)
+                       : pl.fwd == 1 ? forward_piece<Small<E>>(W, Q, steps, scale * kLog2e, pl.parts, parts, pl.stats, stream)
+                                     : forward_piece<Narrow<E>>(W, Q, steps, scale * kLog2e, pl.parts, parts, pl.stats, stream);
+        if (rc) return rc;
+        parts += pl.parts;
     }
     hipLaunchKernelGGL(xent_join_kernel<T>, dim3((s.T + 3) / 4), dim3(256), 0, stream, pl.stats, parts, q, s.ldq, w, s.ldw, s.T, s.V, s.dim,
                        targets, scale, loss, lse);
     return launched("cz_softmax_xent");
 }
 
+template <typename T>
+void transpose(const T *x, uint64_t ld, uint32_t n, uint32_t dim, const uint32_t *targets, uint32_t V, void *out, uint64_t ldo, hipStream_t stream) {
+    const bool wide = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && ld * sizeof(T) % 16 == 0;
+    hipLaunchKernelGGL(xent_transpose_kernel<T>, dim3((uint32_t)((ldo + 63) / 64), (dim + 63) / 64), dim3(256), 0, stream, x, ld, wide, n, dim,
+                       targets, V, (T *)out, ldo);
+}
+
+template <class G>
+int weights_of(const Operand &W, uint32_t v0, uint32_t V, const Operand &Q, uint32_t steps, float scale, const uint32_t *targets, const float *lse,
+               const float *grad_loss, void *p, uint64_t vp, void *pt, uint32_t tp, hipStream_t stream) {
+    typedef typename G::Elem::T T;
+    return launch<G>(xent_weights_kernel<G>, tiles_of(vp, G::BM) * tiles_of(tp, G::BN), stream, W, v0, V, Q, steps, scale, targets, lse, grad_loss,
+                     (T *)p, vp, (T *)pt, tp);
+}
+template <class G>
+int table_grad_of(const Operand &Pt, const Operand &Qt, uint32_t steps, typename G::Elem::T *out, uint32_t dim, hipStream_t stream) {
+    return launch<G>(xent_table_grad_kernel<G>, tiles_of(Pt.rows, G::BM) * tiles_of(dim, G::BN), stream, Pt, Qt, steps, out, dim);
+}
+template <class G>
+int query_grad_of(const Operand &P, const Operand &Wt, uint32_t steps, uint32_t parts, bool add, float *dq, uint32_t dim, hipStream_t stream) {
+    return launch<G>(xent_query_grad_kernel<G>, tiles_of(P.rows, G::BM) * tiles_of(dim, G::BN) * parts, stream, P, Wt, steps,
+                     (steps + parts - 1) / parts, add ? 1 : 0, dq, dim);
+}
+
 template <class E>
 int backward(const Shape &s, const Plan &pl, const void *q_, const void *w_, const uint32_t *targets, float scale, const float *lse,
              const float *grad_loss, void *dq, void *dw, hipStream_t stream) {
     typedef typename E::T T;
-    typedef gemm::Tile<E, kBM, kBN, kWM, kWN> G;
     const T *q = (const T *)q_, *w = (const T *)w_;
-    const uint32_t es = s.es(), kp = s.kp(), tp = s.tp();
+    const uint32_t es = s.es(), kp = s.kp(), tp = s.tp(), steps = kp / s.kstep();
     Operand Q{(const char *)q, s.ldq * es, s.T};
     if (!direct(q, s.ldq, s.dim, es)) {
         pack(q, s.ldq, s.T, s.dim, pl.q, kp, stream);
         Q = Operand{(const char *)pl.q, (uint64_t)kp * es, s.T};
     }
     const bool wd = direct(w, s.ldw, s.dim, es);
-    auto weights = xent_weights_kernel<E, kBM, kBN, kWM, kWN>;
-    auto table_grad = xent_table_grad_kernel<E, kBM, kBN, kWM, kWN>;
-    auto query_grad = xent_query_grad_kernel<E, kBM, kBN, kWM, kWN>;
-    int rc;
-    if ((rc = allow_lds(weights, G::kLds)) || (rc = allow_lds(table_grad, G::kLds)) || (rc = allow_lds(query_grad, G::kLds))) return rc;
-    const uint32_t dt = (s.dim + 63) / 64;
-    if (dw)
-        hipLaunchKernelGGL(xent_transpose_kernel<T>, dim3((tp + 63) / 64, dt), dim3(256), 0, stream, q, s.ldq, s.T, s.dim, targets, s.V,
-                           (T *)pl.qt, (uint64_t)tp);
+    if (dw) transpose(q, s.ldq, s.T, s.dim, targets, s.V, pl.qt, tp, stream);
     for (uint32_t v0 = 0; v0 < s.V; v0 += pl.piece) {
-        const uint32_t nv = std::min(pl.piece, s.V - v0), vp = (uint32_t)up_to(nv, kBM);
+        const uint32_t nv = std::min(pl.piece, s.V - v0), vp = (uint32_t)up_to(nv, 256);
         const T *wv = w + v0 * s.ldw;
         Operand W{(const char *)wv, s.ldw * es, nv};
         if (!wd) {
             pack(wv, s.ldw, nv, s.dim, pl.w, kp, stream);
             W = Operand{(const char *)pl.w, (uint64_t)kp * es, nv};
         }
-        hipLaunchKernelGGL(weights, dim3(vp / kBM * ((tp + kBN - 1) / kBN)), dim3(G::kThreads), G::kLds, stream, W, v0, s.V, Q,
-                           kp / s.kstep(), scale, targets, lse, grad_loss, dq ? (T *)pl.p : nullptr, (uint64_t)vp,
-                           dw ? (T *)pl.pt : nullptr, tp);
+        void *p = dq ? pl.p : nullptr, *pt = dw ? pl.pt : nullptr;
+        int rc = pl.large_p ? weights_of<Large<E>>(W, v0, s.V, Q, steps, scale, targets, lse, grad_loss, p, vp, pt, tp, stream)
+                            : weights_of<Small<E>>(W, v0, s.V, Q, steps, scale, targets, lse, grad_loss, p, vp, pt, tp, stream);
+        if (rc) return rc;
         if (dw) {
             const Operand Pt{(const char *)pl.pt, (uint64_t)tp * es, nv}, Qt{(const char *)pl.qt, (uint64_t)tp * es, s.dim};
-            hipLaunchKernelGGL(table_grad, dim3(vp / kBM * ((s.dim + kBN - 1) / kBN)), dim3(G::kThreads), G::kLds, stream, Pt, Qt,
-                               tp / s.kstep(), (T *)dw + (uint64_t)v0 * s.dim, s.dim);
+            T *out = (T *)dw + (uint64_t)v0 * s.dim;
+            rc = pl.large_w ? table_grad_of<Large<E>>(Pt, Qt, tp / s.kstep(), out, s.dim, stream)
+                            : table_grad_of<Small<E>>(Pt, Qt, tp / s.kstep(), out, s.dim, stream);
+            if (rc) return rc;
         }
         if (dq) {
-            hipLaunchKernelGGL(xent_transpose_kernel<T>, dim3((vp + 63) / 64, dt), dim3(256), 0, stream, wv, s.ldw, nv, s.dim,
-                               (const uint32_t *)nullptr, 0u, (T *)pl.wt, (uint64_t)vp);
+            transpose(wv, s.ldw, nv, s.dim, (const uint32_t *)nullptr, 0u, pl.wt, vp, stream);
             const Operand P{(const char *)pl.p, (uint64_t)vp * es, s.T}, Wt{(const char *)pl.wt, (uint64_t)vp * es, s.dim};
-            const uint32_t steps = vp / s.kstep(), per = (steps + pl.parts - 1) / pl.parts;
-            const uint32_t tiles = ((s.T + kBM - 1) / kBM) * ((s.dim + kBN - 1) / kBN);
-            hipLaunchKernelGGL(query_grad, dim3(tiles * pl.parts), dim3(G::kThreads), G::kLds, stream, P, Wt, steps, per, v0 ? 1 : 0, pl.dq, s.dim);
+            rc = pl.large_q ? query_grad_of<Large<E>>(P, Wt, vp / s.kstep(), pl.parts, v0 != 0, pl.dq, s.dim, stream)
+                            : query_grad_of<Small<E>>(P, Wt, vp / s.kstep(), pl.parts, v0 != 0, pl.dq, s.dim, stream);
+            if (rc) return rc;
         }
     }
     if (dq)
