@@ -1,7 +1,6 @@
 """Arrays of a caller, on the host (numpy) or on the GPU (torch tensors), as the C entry points want them."""
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 
 
@@ -21,18 +20,26 @@ def all_on_gpu(*arrays) -> bool:
     return any(there)
 
 
-@contextlib.contextmanager
-def on_stream(like, stream):
-    """-> the raw stream a call works on: the caller's, or torch's current one on the tensor's device.  Outputs and scratch allocated
-    inside belong to that stream."""
-    import torch
-    with torch.cuda.device(like.device):
-        if stream is None:
-            yield C.c_void_p(torch.cuda.current_stream(like.device).cuda_stream)
-        else:
-            raw = int(stream.cuda_stream) if hasattr(stream, "cuda_stream") else int(stream)
-            # handle 0 is the device's default stream, which ExternalStream does not wrap
-            s = torch.cuda.ExternalStream(raw, device=like.device) if raw else torch.cuda.default_stream(like.device)
-            with torch.cuda.stream(s):
-                yield C.c_void_p(raw)
+class on_stream:
+    """with on_stream(tensor, stream) as raw: the raw stream a call works on -- the caller's (a handle or a torch stream), or torch's
+    current one on the tensor's device.  Outputs and scratch allocated inside belong to that stream."""
 
+    def __init__(self, like, stream):
+        import torch
+        self._inner = None
+        if stream is None:
+            self._raw = torch.cuda.current_stream(like.device).cuda_stream
+        else:
+            self._raw = int(stream.cuda_stream) if hasattr(stream, "cuda_stream") else int(stream)
+            # handle 0 is the device's default stream, which ExternalStream does not wrap
+            s = torch.cuda.ExternalStream(self._raw, device=like.device) if self._raw else torch.cuda.default_stream(like.device)
+            self._inner = torch.cuda.stream(s)
+
+    def __enter__(self):
+        if self._inner is not None:
+            self._inner.__enter__()
+        return C.c_void_p(self._raw)
+
+    def __exit__(self, *exc):
+        if self._inner is not None:
+            self._inner.__exit__(*exc)

@@ -649,18 +649,21 @@ __device__ __forceinline__ uint32_t order_of(float f) {
     return (u >> 31) ? ~u : (u | 0x80000000u);
 }
 
-// need[b]: a score that k rows are sure to reach = the k-th largest of what `n` waves (or, where there are too few of them, tiles) are
+// need[b]: a score that k rows are sure to reach (limit[b]: the distance that goes with it) = the k-th largest of what `n` waves (or, where there are too few of them, tiles) are
 // sure to hold, each a row of its own.  Radix selection, 8 bits at a time.  -inf (every row is looked at) when there are fewer than k or the
 // k-th is not finite.
 __global__ void __launch_bounds__(1024)
-q4_need_kernel(Near near, bool by_tile, uint32_t k, float *__restrict__ need) {
+q4_need_kernel(Near near, bool by_tile, uint32_t k, float *__restrict__ need, double *__restrict__ limit) {
     __shared__ uint32_t hist[256];
     __shared__ uint32_t sel[2];
     const uint32_t b = blockIdx.x, n = by_tile ? near.n_tiles : near.n_best;
     const float *v = (by_tile ? near.tile_score : near.best) + (uint64_t)b * n;
     const float qn = near.qnorm[b];
     if (n < k) {
-        if (threadIdx.x == 0) need[b] = -__builtin_inff();
+        if (threadIdx.x == 0) {
+            need[b] = -__builtin_inff();
+            limit[b] = __builtin_inf();
+        }
         return;
     }
     constexpr int R = 16;  // values a thread keeps; more are read again for each 8 bits
@@ -711,7 +714,13 @@ q4_need_kernel(Near near, bool by_tile, uint32_t k, float *__restrict__ need) {
     }
     if (threadIdx.x == 0) {
         const float f = __uint_as_float((prefix >> 31) ? (prefix & 0x7FFFFFFFu) : ~prefix);
-        need[b] = fabsf(f) < __builtin_inff() ? f : -__builtin_inff();
+        const bool some = fabsf(f) < __builtin_inff();
+        need[b] = some ? f : -__builtin_inff();
+        // a row that k others are nearer than: its distance, with 1e-6 of what it is made of to spare for the arithmetic in between
+        const double q = qn, s = f;
+        double d = near.metric == CZ_COSINE ? 1.0 - s / q + 1e-6 * fabs(s / q) : near.metric == CZ_IP ? 1.0 - s + 1e-6 * fabs(s) : q * q - s + 1e-6 * (q * q + fabs(s));
+        d += 1e-9 * fabs(d) + 1e-12 * (near.metric != CZ_L2);
+        limit[b] = some && d == d ? d : __builtin_inf();
     }
 }
 
@@ -786,6 +795,7 @@ struct Candidates {
     const float *tile_norm;   // [n_tiles]
     const float *qnorm;       // [B]
     const float *need;        // [B]
+    const double *limit;      // [B]
     float err;
 };
 
@@ -801,16 +811,18 @@ q4_scan_kernel(int metric, Rows t, const float *__restrict__ queries, uint32_t k
     double *red = (double *)(tkey + k);           // [4]
     uint32_t *bid = (uint32_t *)(red + 4);        // [256]
     uint32_t *tid_ = bid + 256;                   // [k]
-    uint32_t *list = tid_ + k;                    // [256] candidate tiles, ascending
-    uint32_t *cnt = list + 256;                   // [4]
+    uint32_t *list = tid_ + k;                    // [256] candidate tiles
+    uint32_t *cnt = list + 256;                   // [5]
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, sub = tid % LPR;
     const uint32_t b = blockIdx.y;
     const uint32_t n_tiles = (uint32_t)(((uint64_t)t.n + kTile - 1) / kTile);
     const uint32_t t0 = blockIdx.x * tiles_per_chunk, t1 = (uint32_t)min((uint64_t)n_tiles, (uint64_t)t0 + tiles_per_chunk);
     const float need = cand.tile_score ? cand.need[b] : 0.f, qn = cand.tile_score ? cand.qnorm[b] : 0.f;
+    const double limit = cand.tile_score ? cand.limit[b] : __builtin_inf();
     double qq = 0.0;
     bool ready = false;
     int tcnt = 0;
+    if (tid == 0) cnt[4] = 0;  // rows in the batch
     for (uint32_t tb = t0; tb < t1; tb += 256) {
         const uint32_t tile = tb + tid;
         bool want = tile < t1;
@@ -842,34 +854,40 @@ q4_scan_kernel(int metric, Rows t, const float *__restrict__ queries, uint32_t k
             qq = (red[0] + red[1]) + (red[2] + red[3]);
             ready = true;
         }
-        for (uint32_t j = 0; j < total; j += 4) {
-            // only the table's last tile can be short, and it is the last of its batch
-            const uint32_t full = min(4u, total - j), last = list[j + full - 1];
-            const uint32_t nb = (full - 1) * kTile + (uint32_t)min((uint64_t)kTile, (uint64_t)t.n - (uint64_t)last * kTile);
-            constexpr int U = 4, AT = 256 / LPR;  // rows of a lane group at a time, lane groups
-            for (uint32_t s0 = 0; s0 < nb; s0 += U * AT) {
-                uint32_t r[U];
-                double d[U];
+        constexpr int U = 4, AT = 256 / LPR;  // rows of a lane group at a time, lane groups: 16 to 256 rows
+        const uint32_t rows = total * kTile;
+        for (uint32_t s0 = 0; s0 < rows; s0 += U * AT) {
+            uint32_t r[U];
+            double d[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const uint32_t slot = min(s0 + u * AT + tid / LPR, rows - 1);
+                r[u] = (uint32_t)min((uint64_t)list[slot / kTile] * kTile + slot % kTile, (uint64_t)t.n - 1);
+            }
+            const uint32_t have = cnt[4];
+            row_distances<LPR, U>(metric, t, r, sub, q, qq, d);
+            __syncthreads();  // (everyone has read it)
+            if (have + U * AT > 256) {
+                tcnt = topk_merge_batch((int)have, bkey, bid, tkey, tid_, tcnt, (int)k);
+                if (tid == 0) cnt[4] = 0;
+                __syncthreads();
+            }
+            if (sub == 0)
 #pragma unroll
                 for (int u = 0; u < U; u++) {
-                    const uint32_t safe = min(s0 + u * AT + tid / LPR, nb - 1);
-                    r[u] = list[j + safe / kTile] * kTile + safe % kTile;
-                }
-                row_distances<LPR, U>(metric, t, r, sub, q, qq, d);
-                if (sub == 0)
-#pragma unroll
-                    for (int u = 0; u < U; u++) {
-                        const uint32_t slot = s0 + u * AT + tid / LPR;
-                        if (slot < nb) {
-                            bkey[slot] = dist_key(d[u]);
-                            bid[slot] = r[u];
-                        }
+                    const uint32_t slot = s0 + u * AT + tid / LPR;
+                    if (slot < rows && (uint64_t)list[slot / kTile] * kTile + slot % kTile < t.n && !(d[u] > limit)) {
+                        const uint32_t e = atomicAdd(&cnt[4], 1u);  // (the order does not matter: entries are ranked)
+                        bkey[e] = dist_key(d[u]);
+                        bid[e] = r[u];
                     }
-            }
-            tcnt = topk_merge_batch((int)nb, bkey, bid, tkey, tid_, tcnt, (int)k);
+                }
+            __syncthreads();
         }
         __syncthreads();  // the list is free
     }
+    __syncthreads();
+    tcnt = topk_merge_batch((int)cnt[4], bkey, bid, tkey, tid_, tcnt, (int)k);
     const size_t part = (size_t)b * gridDim.x + blockIdx.x;
     for (int i = tid; i < tcnt; i += 256) {
         part_key[part * k + i] = tkey[i];
@@ -921,7 +939,7 @@ q4_join_kernel(const uint64_t *__restrict__ part_key, const uint32_t *__restrict
         for (int w = 0; w < wave; w++) run += ctl[w];
         first[tid] = run - mine;
         if (tid == 255) first[256] = run;
-        if (mine) {
+        if ((uint32_t)__syncthreads_count(mine != 0) >= k && mine) {
             uint32_t rank = 0;
 #pragma unroll 8
             for (int t = 0; t < 256; t++) {
@@ -1122,14 +1140,17 @@ struct KnnPlan {
     int *exponent;
     float *turned;
     float *qnorm, *tile_score, *tile_norm, *best, *need;
+    double *limit;
     uint32_t n_best;
     size_t bytes;
 };
 KnnPlan knn_plan(const Rows &t, uint32_t B, uint32_t k, void *ws) {
     KnnPlan p{};
     const uint32_t n_tiles = (uint32_t)(((uint64_t)t.n + kTile - 1) / kTile);
-    // 256 rows are a batch of the list; enough workgroups to fill the chip, few enough lists to join
-    uint32_t chunks = std::min(n_tiles, std::max(1u, 2048 / B));
+    p.filtered = n_tiles >= 4 * (uint64_t)k && n_tiles >= 512;
+    // enough workgroups to fill the chip, few enough lists to join
+    uint32_t chunks = std::min(n_tiles, std::max(1u, (p.filtered ? 512 : 2048) / B));
+    if (p.filtered && B > 256) chunks = 2;
     chunks = std::max(1u, std::min(chunks, std::max(16u, 65536 / k)));
     p.tiles_per_chunk = std::max(1u, (n_tiles + chunks - 1) / chunks);
     p.chunks = std::max(1u, (n_tiles + p.tiles_per_chunk - 1) / p.tiles_per_chunk);
@@ -1137,7 +1158,6 @@ KnnPlan knn_plan(const Rows &t, uint32_t B, uint32_t k, void *ws) {
     p.part_key = c.take<uint64_t>((size_t)B * p.chunks * k);
     p.part_id = c.take<uint32_t>((size_t)B * p.chunks * k);
     p.part_count = c.take<uint32_t>((size_t)B * p.chunks);
-    p.filtered = n_tiles >= 4 * (uint64_t)k && n_tiles >= 512;
     if (p.filtered) {
         p.steps = (t.groups << t.gshift) / 64 + ((t.groups << t.gshift) % 64 != 0);
         p.halves = B <= kDigitQueries ? 0 : B <= 128 ? 1 : 2;
@@ -1159,6 +1179,7 @@ KnnPlan knn_plan(const Rows &t, uint32_t B, uint32_t k, void *ws) {
         p.tile_norm = c.take<float>(n_tiles);
         p.best = c.take<float>((size_t)B * p.n_best);
         p.need = c.take<float>(B);
+        p.limit = c.take<double>(B);
     }
     p.bytes = c.used();
     return p;
@@ -1387,7 +1408,7 @@ extern "C" int cz_q4_knn(int metric, const uint8_t *codes, const uint16_t *scale
     if ((rc = cz::scratch_of(ws, ws_bytes, cz_q4_workspace(n, dim, group, B, k), own, &base))) return rc;
     t.codes = codes;
     t.scales = scales;
-    const size_t smem = 256 * 16 + (size_t)k * 12 + 48 + (size_t)t.chunks * 64;
+    const size_t smem = 256 * 16 + (size_t)k * 12 + 64 + (size_t)t.chunks * 64;
     const uint32_t lpr = lanes_per_row(t.chunks);
     const uint32_t turn = turn_of(t);
     for (uint32_t b0 = 0; b0 < B; b0 += turn) {
@@ -1401,8 +1422,8 @@ extern "C" int cz_q4_knn(int metric, const uint8_t *codes, const uint16_t *scale
                 const float err = p.halves ? half_error_unit(t) : score_error_unit(t);
                 const Near near{metric, sqnorms, err, p.qnorm, p.tile_score, p.tile_norm, p.best, (n + kTile - 1) / kTile, p.n_best};
                 if ((rc = launch_near(t, p, q, nb, near, stream))) return rc;
-                hipLaunchKernelGGL(q4_need_kernel, dim3(nb), dim3(1024), 0, stream, near, p.n_best < 4 * k, k, p.need);
-                cand = Candidates{p.tile_score, p.tile_norm, p.qnorm, p.need, err};
+                hipLaunchKernelGGL(q4_need_kernel, dim3(nb), dim3(1024), 0, stream, near, p.n_best < 4 * k, k, p.need, p.limit);
+                cand = Candidates{p.tile_score, p.tile_norm, p.qnorm, p.need, p.limit, err};
             }
 #define CZ_Q4_CALL(L)                                                                                                              \
     hipLaunchKernelGGL((q4_scan_kernel<L>), dim3(p.chunks, nb), dim3(256), smem, stream, metric, t, q, k, p.tiles_per_chunk, cand, \
