@@ -517,6 +517,8 @@ q4_scores_kernel(Rows t, gemm::Operand Q, const int *__restrict__ exponent, uint
     const uint32_t n0 = at % qt * BN, part = at / qt * 8 + blockIdx.x % 8;  // (a stretch's workgroups on one XCD)
     const uint32_t k0 = part * blocks_per_part, k1 = min(n_blocks, k0 + blocks_per_part);
     const uint32_t row_bytes = t.chunks * 4;
+    // of the two waves on a SIMD one makes its rows before and one after its matrix instructions, so that these do not wait for both
+    const bool early = tid < 256;
     float best[G::NT], qn[G::NT];
     int qe[G::NT];
 #pragma unroll
@@ -585,10 +587,16 @@ q4_scores_kernel(Rows t, gemm::Operand Q, const int *__restrict__ exponent, uint
             G::arrived();
             if (s + 1 < steps) {
                 G::copy(src, (uint64_t)(s + 1) * 128, nxt + BM * 128);
+                if (early) {
+                    store(nxt);
+                    if (s + 2 < steps) load(s + 2);
+                }
+            }
+            g.step(cur);
+            if (!early && s + 1 < steps) {
                 store(nxt);
                 if (s + 2 < steps) load(s + 2);
             }
-            g.step(cur);
         }
         float top[G::NT][TW];
 #pragma unroll
@@ -789,6 +797,60 @@ __device__ __forceinline__ void row_distances(int metric, const Rows &t, const u
     for (int u = 0; u < U; u++) out[u] = metric == CZ_L2 ? a[u] : metric == CZ_COSINE ? 1.0 - a[u] / sqrt(qq * x2[u]) : 1.0 - a[u];
 }
 
+// bkey / bid[0 .. nb): a batch of up to 256 entries, no two of one id; tkey / tid_[0 .. tcnt): the list, ascending by (key, id), at most k.
+// Every entry's rank is counted, without a branch, so that the LDS reads of the count run ahead: 3 us for a full batch.  Returns the new
+// length (uniform); starts and ends with a barrier.
+__device__ __forceinline__ int merge_batch(int nb, const uint64_t *bkey, const uint32_t *bid, uint64_t *tkey, uint32_t *tid_, int tcnt, int k) {
+    const int tid = threadIdx.x;
+    __syncthreads();
+    auto before = [&](uint64_t key, uint32_t id) {
+        int c = 0;
+#pragma unroll 8
+        for (int t = 0; t < nb; t++) {
+            const uint64_t o = bkey[t];
+            c += (int)((o < key) | ((o == key) & (bid[t] < id)));
+        }
+        return c;
+    };
+    uint64_t mk = 0, wk[4];
+    uint32_t mi = CZ_NONE, wi[4];
+    int at = k, wat[4];
+    if (tid < nb) {
+        mk = bkey[tid];
+        mi = bid[tid];
+        int lo = 0, hi = tcnt;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (czh::key_lt(tkey[mid], tid_[mid], mk, mi)) lo = mid + 1;
+            else hi = mid;
+        }
+        at = lo + before(mk, mi);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; r++) {  // (k <= 1024)
+        const int j = tid + 256 * r;
+        wat[r] = k;
+        if (j < tcnt) {
+            wk[r] = tkey[j];
+            wi[r] = tid_[j];
+            wat[r] = j + before(wk[r], wi[r]);
+        }
+    }
+    __syncthreads();
+    if (at < k) {
+        tkey[at] = mk;
+        tid_[at] = mi;
+    }
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+        if (wat[r] < k) {
+            tkey[wat[r]] = wk[r];
+            tid_[wat[r]] = wi[r];
+        }
+    __syncthreads();
+    return min(k, tcnt + nb);
+}
+
 // the tiles that a search still has to look at in f64: those whose best score could reach what k rows are sure to reach
 struct Candidates {
     const float *tile_score;  // [B][n_tiles], or null: all tiles
@@ -868,7 +930,7 @@ q4_scan_kernel(int metric, Rows t, const float *__restrict__ queries, uint32_t k
             row_distances<LPR, U>(metric, t, r, sub, q, qq, d);
             __syncthreads();  // (everyone has read it)
             if (have + U * AT > 256) {
-                tcnt = topk_merge_batch((int)have, bkey, bid, tkey, tid_, tcnt, (int)k);
+                tcnt = merge_batch((int)have, bkey, bid, tkey, tid_, tcnt, (int)k);
                 if (tid == 0) cnt[4] = 0;
                 __syncthreads();
             }
@@ -877,9 +939,12 @@ q4_scan_kernel(int metric, Rows t, const float *__restrict__ queries, uint32_t k
                 for (int u = 0; u < U; u++) {
                     const uint32_t slot = s0 + u * AT + tid / LPR;
                     if (slot < rows && (uint64_t)list[slot / kTile] * kTile + slot % kTile < t.n && !(d[u] > limit)) {
-                        const uint32_t e = atomicAdd(&cnt[4], 1u);  // (the order does not matter: entries are ranked)
-                        bkey[e] = dist_key(d[u]);
-                        bid[e] = r[u];
+                        const uint64_t key = dist_key(d[u]);
+                        if (tcnt < (int)k || czh::key_lt(key, r[u], tkey[k - 1], tid_[k - 1])) {
+                            const uint32_t e = atomicAdd(&cnt[4], 1u);  // (the order does not matter: entries are ranked)
+                            bkey[e] = key;
+                            bid[e] = r[u];
+                        }
                     }
                 }
             __syncthreads();
@@ -887,7 +952,7 @@ q4_scan_kernel(int metric, Rows t, const float *__restrict__ queries, uint32_t k
         __syncthreads();  // the list is free
     }
     __syncthreads();
-    tcnt = topk_merge_batch((int)cnt[4], bkey, bid, tkey, tid_, tcnt, (int)k);
+    tcnt = merge_batch((int)cnt[4], bkey, bid, tkey, tid_, tcnt, (int)k);
     const size_t part = (size_t)b * gridDim.x + blockIdx.x;
     for (int i = tid; i < tcnt; i += 256) {
         part_key[part * k + i] = tkey[i];
@@ -896,8 +961,8 @@ q4_scan_kernel(int metric, Rows t, const float *__restrict__ queries, uint32_t k
     if (tid == 0) part_count[part] = (uint32_t)tcnt;
 }
 
-// one workgroup per query: the partial lists joined, the radius cut, the padding.  Merging a full batch of 256 takes some 20 us, so the k-th
-// smallest of 256 lists' heads, which k entries are sure not to be behind, leaves few to merge (one query, 157 lists: 76 -> XXX us).
+// one workgroup per query: the partial lists joined, the radius cut, the padding.  What a list takes in a full batch at a time would be merged for microseconds; the k-th
+// smallest of 256 lists' heads, which k entries are sure not to be behind, leaves few to merge (one query, 157 lists: 76 -> 12 us).
 constexpr size_t join_lds(size_t k) { return 256 * 24 + k * 12 + 257 * 4 + 8 * 4 + 8; }
 __global__ void __launch_bounds__(256)
 q4_join_kernel(const uint64_t *__restrict__ part_key, const uint32_t *__restrict__ part_id, const uint32_t *__restrict__ part_count,
@@ -975,7 +1040,7 @@ q4_join_kernel(const uint64_t *__restrict__ part_key, const uint32_t *__restrict
                               (tcnt < (int)k || czh::key_lt(key, id, tkey[k - 1], tid_[k - 1]));
             const int add = __syncthreads_count(want);
             if (fill + add > 256) {
-                tcnt = topk_merge_batch(fill, bkey, bid, tkey, tid_, tcnt, (int)k);
+                tcnt = merge_batch(fill, bkey, bid, tkey, tid_, tcnt, (int)k);
                 if (tid == 0) ctl[4] = 0;
                 fill = 0;
                 __syncthreads();
@@ -989,7 +1054,7 @@ q4_join_kernel(const uint64_t *__restrict__ part_key, const uint32_t *__restrict
         }
         __syncthreads();  // heads, sums and the limit are free
     }
-    tcnt = topk_merge_batch(fill, bkey, bid, tkey, tid_, tcnt, (int)k);
+    tcnt = merge_batch(fill, bkey, bid, tkey, tid_, tcnt, (int)k);
     if (tid >= 64) return;
     uint32_t done = 0;
     for (uint32_t i0 = 0; i0 < k; i0 += 64) {
@@ -1016,18 +1081,14 @@ q4_join_kernel(const uint64_t *__restrict__ part_key, const uint32_t *__restrict
 }
 
 // ---- host side -------------------------------------------------------------------------------------------------------
-uint32_t lanes_per_row(uint32_t chunks) {
-    uint32_t l = 4;
-    while (l < chunks && l < 64) l <<= 1;
-    return l;
-}
+// lanes that share a row: 16 (a 64-byte piece of its codes), fewer for short rows.  More would spend longer on joining their sums: 64 lanes
+// made the k-NN's f64 distances XXX times as long.
+uint32_t lanes_per_row(uint32_t chunks) { return chunks <= 4 ? 4 : chunks <= 8 ? 8 : 16; }
 #define CZ_Q4_LANES(LPR, CALL)      \
     switch (LPR) {                  \
         case 4: CALL(4); break;     \
         case 8: CALL(8); break;     \
-        case 16: CALL(16); break;   \
-        case 32: CALL(32); break;   \
-        default: CALL(64); break;   \
+        default: CALL(16); break;   \
     }
 
 int shape_of_rows(uint32_t n, uint32_t dim, uint32_t group, Rows *t) {
