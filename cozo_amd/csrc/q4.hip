@@ -530,6 +530,7 @@ q4_scores_kernel(Rows t, gemm::Operand Q, const int *__restrict__ exponent, uint
     }
     const char *src[G::NB];
     G::rows_of(Q, n0, src);
+#pragma unroll 1
     for (uint32_t blk = k0; blk < k1; blk++) {
         const uint64_t r = (uint64_t)blk * BM + mine, safe = min(r, (uint64_t)t.n - 1);
         const uint8_t *codes = t.codes + safe * row_bytes;
@@ -582,15 +583,19 @@ q4_scores_kernel(Rows t, gemm::Operand Q, const int *__restrict__ exponent, uint
         if (steps > 1) load(1);
         G g;
         g.zero();
+#pragma unroll 1
         for (uint32_t s = 0; s < steps; s++) {
             char *cur = lds + (s & 1) * G::kBytes, *nxt = lds + (~s & 1) * G::kBytes;
-            G::arrived();
+            // this step's copies are in LDS; the two loads behind them (codes and scale of the step after) may still be on their way
+            // (__syncthreads would wait for all of them)
+            if (s > 0 && s + 1 < steps) asm volatile("s_waitcnt vmcnt(2) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
             if (s + 1 < steps) {
+                if (early) store(nxt);
+                asm volatile("" ::: "memory");  // (in this order: the wait above counts on it)
                 G::copy(src, (uint64_t)(s + 1) * 128, nxt + BM * 128);
-                if (early) {
-                    store(nxt);
-                    if (s + 2 < steps) load(s + 2);
-                }
+                asm volatile("" ::: "memory");
+                if (early && s + 2 < steps) load(s + 2);
             }
             g.step(cur);
             if (!early && s + 1 < steps) {
