@@ -3,8 +3,8 @@
 //
 // * k goes in steps of 128 bytes per row (64 bf16 / 32 f32): a step of A and B goes straight from memory into LDS (16 bytes a lane, no
 //   registers in between), two steps are kept, the next one is on its way while the matrix cores work on this one.
-// * LDS rows are 128 bytes = 8 pieces of 16; piece p of row r lies at place p ^ (r & 7), so that the 32 rows a matrix instruction reads
-//   at one k spread over all banks.  The copy into LDS writes lanes in order, so it is the lane's GLOBAL address that is permuted.
+// * LDS rows are 128 bytes = 8 pieces of 16; piece p of row r lies at place p ^ (r / 2 & 7): two rows fill the 64 banks, so 16 neighbouring
+//   rows read at one k touch each bank once (p ^ (r & 7), which 32 banks would ask for, counted as many conflicts as reads).  The copy into LDS writes lanes in order, so it is the lane's GLOBAL address that is permuted.
 // * operand layout of the 32 x 32 matrix instructions: lane l holds row l % 32 and the k that belong to half l / 32; as both
 //   operands are read alike, which k those are does not matter: a half is a 16-byte piece (8 bf16 = one 32x32x16 instruction, 4 f32 =
 //   four 32x32x2 ones).
@@ -23,14 +23,17 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 struct Bf16 {
+    static constexpr int kPerPiece = 1;  // matrix instructions of a 16-byte piece
     typedef __bf16 T;
     static constexpr uint32_t kStep = 64;  // elements of a 128-byte step
 };
 struct F16 {
+    static constexpr int kPerPiece = 1;
     typedef _Float16 T;
     static constexpr uint32_t kStep = 64;
 };
 struct F32 {
+    static constexpr int kPerPiece = 4;
     typedef float T;
     static constexpr uint32_t kStep = 32;
 };
@@ -54,9 +57,10 @@ struct Operand {
     uint32_t rows;
 };
 
-// BM x BN by WM x WN waves.  What bounds it is LDS: a wave reads (BM / WM + BN / WN) * 32 bytes per k of 16 for BM / WM * BN / WN products.
-// Measured with 1024 rows of B, 1M rows of A, k = 768, bf16: 128 x 128 by 2 x 2 904 TFLOP/s, 256 x 256 by 2 x 4 1177 (a library's
-// 8192^3 product: 1537); more steps kept in LDS, fragments read ahead and tiles run into each other gave no more than either.
+// BM x BN by WM x WN waves.  Measured with 1024 rows of B, 1M rows of A, k = 768, bf16: 128 x 128 by 2 x 2 900 TFLOP/s (32 bytes of copies
+// a clock and CU; its matrix cores are busy 45 % of the time), 256 x 256 by 2 x 4 1185 (52 %; a library's 8192^3 product: 1537).  Zeros for
+// data run at 1310: the clock under this load is part of the bound.  More and shorter steps kept in LDS, tiles run into each other and a
+// wave priority for the matrix instructions were within 5 % of it either way.
 template <class E, int BM_, int BN_, int WM_, int WN_>
 struct Tile {
     typedef E Elem;
@@ -84,7 +88,7 @@ struct Tile {
     static __device__ __forceinline__ void rows_of(const Operand &o, uint32_t row0, const char *(&src)[N]) {
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            const uint32_t c = i * kThreads + threadIdx.x, row = c >> 3, piece = (c & 7) ^ (row & 7);
+            const uint32_t c = i * kThreads + threadIdx.x, row = c >> 3, piece = (c & 7) ^ ((row >> 1) & 7);
             src[i] = o.base + (uint64_t)min(row0 + row, o.rows - 1) * o.ld + piece * 16;
         }
     }
@@ -104,22 +108,35 @@ struct Tile {
     static __device__ __forceinline__ int wave_row() { return (int)(threadIdx.x >> 6) / WN * (BM / WM); }
     static __device__ __forceinline__ int wave_col() { return (int)(threadIdx.x >> 6) % WN * (BN / WN); }
 
-    __device__ __forceinline__ void step(const char *lds) {
+    __device__ __forceinline__ void fragments(const char *lds, int kk, u32x4 (&a)[MT], u32x4 (&b)[NT]) const {
         const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
         const char *la = lds + (wave_row() + l32) * 128, *lb = lds + BM * 128 + (wave_col() + l32) * 128;
+        const int at = ((2 * kk + half) ^ ((l32 >> 1) & 7)) * 16;
+#pragma unroll
+        for (int j = 0; j < NT; j++) b[j] = *(const u32x4 *)(lb + j * 32 * 128 + at);
+#pragma unroll
+        for (int i = 0; i < MT; i++) a[i] = *(const u32x4 *)(la + i * 32 * 128 + at);
+    }
+    __device__ __forceinline__ void step(const char *lds) {
+        u32x4 a[2][MT], b[2][NT];
+        fragments(lds, 0, a[0], b[0]);
 #pragma unroll
         for (int kk = 0; kk < 4; kk++) {
-            const int at = ((2 * kk + half) ^ (l32 & 7)) * 16;
-            u32x4 a[MT], b[NT];
-#pragma unroll
-            for (int i = 0; i < MT; i++) a[i] = *(const u32x4 *)(la + i * 32 * 128 + at);
-#pragma unroll
-            for (int j = 0; j < NT; j++) b[j] = *(const u32x4 *)(lb + j * 32 * 128 + at);
+            if (kk < 3) fragments(lds, kk + 1, a[(kk + 1) & 1], b[(kk + 1) & 1]);
 #pragma unroll
             for (int i = 0; i < MT; i++)
 #pragma unroll
-                for (int j = 0; j < NT; j++) mma(E{}, a[i], b[j], acc[i][j]);
+                for (int j = 0; j < NT; j++) mma(E{}, a[kk & 1][i], b[kk & 1][j], acc[i][j]);
         }
+        // the next fragments are read between this fragment's matrix instructions, one to one
+        __builtin_amdgcn_sched_group_barrier(0x100, MT + NT, 0);
+#pragma unroll
+        for (int kk = 0; kk < 4; kk++)
+#pragma unroll
+            for (int x = 0; x < MT * NT; x++) {
+                if (kk < 3 && x < MT + NT) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, E::kPerPiece, 0);
+            }
     }
     // one tile: A rows from m0, B rows from n0, `steps` >= 1 steps from byte k0 of a row on
     __device__ __forceinline__ void run(const Operand &A, uint32_t m0, const Operand &B, uint32_t n0, uint64_t k0, uint32_t steps, char *lds) {

@@ -576,7 +576,7 @@ q4_scores_kernel(Rows t, gemm::Operand Q, const int *__restrict__ exponent, uint
                     const f16x2 h = __builtin_bit_cast(f16x2, ((u >> (4 * x)) & 0x000F000Fu) | 0x64006400u) - off;  // 1024 + code + 8 - 1032
                     o[x] = __builtin_bit_cast(uint32_t, h * s2);
                 }
-                *(u32x4 *)(to + mine * 128 + (((half * 4 + d) ^ (mine & 7)) * 16)) = o;
+                *(u32x4 *)(to + mine * 128 + (((half * 4 + d) ^ ((mine >> 1) & 7)) * 16)) = o;
             }
         };
         store(lds);
