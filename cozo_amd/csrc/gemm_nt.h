@@ -50,6 +50,13 @@ __device__ __forceinline__ void mma(F32, const u32x4 &a, const u32x4 &b, f32x16 
     for (int j = 0; j < 4; j++) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j], y[j], c, 0, 0, 0);
 }
 
+// Workgroups go round the 8 XCDs.  The place of this one in an order that gives each XCD a run of neighbours, which read the same rows through
+// its L2.
+__device__ __forceinline__ uint32_t place_in_order() {
+    const uint32_t x = blockIdx.x % 8, per = gridDim.x / 8, rest = gridDim.x % 8;
+    return x * per + min(x, rest) + blockIdx.x / 8;
+}
+
 // rows of one operand as a workgroup sees them; rows past the last one are read as the last one (the epilogue drops them)
 struct Operand {
     const char *base;

@@ -513,8 +513,8 @@ q4_scores_kernel(Rows t, gemm::Operand Q, const int *__restrict__ exponent, uint
     extern __shared__ __attribute__((aligned(16))) char lds[];
     float2 *rowf = (float2 *)(lds + G::kLds);  // [BM] factor and addend that turn a product into a score
     const int tid = threadIdx.x, lane = tid & 63, mine = tid >> 1, half = tid & 1;
-    const uint32_t qt = (Q.rows + BN - 1) / BN, at = blockIdx.x / 8;
-    const uint32_t n0 = at % qt * BN, part = at / qt * 8 + blockIdx.x % 8;  // (a stretch's workgroups on one XCD)
+    const uint32_t qt = (Q.rows + BN - 1) / BN, at = gemm::place_in_order();
+    const uint32_t n0 = at % qt * BN, part = at / qt;
     const uint32_t k0 = part * blocks_per_part, k1 = min(n_blocks, k0 + blocks_per_part);
     const uint32_t row_bytes = t.chunks * 4;
     // of the two waves on a SIMD one makes its rows before and one after its matrix instructions, so that these do not wait for both
@@ -1229,7 +1229,7 @@ KnnPlan knn_plan(const Rows &t, uint32_t B, uint32_t k, void *ws) {
         p.halves = B <= kDigitQueries ? 0 : B <= 128 ? 1 : 2;
         if (p.halves) {
             const uint32_t b = p.halves == 2 ? 256 : 128, qt = (B + b - 1) / b, blocks = (t.n + b - 1) / b, resident = p.halves == 2 ? 256 : 512;
-            p.parts = std::max(8u, std::min((blocks + 7) / 8 * 8, resident / qt / 8 * 8));
+            p.parts = std::max(1u, std::min(blocks, resident / qt));
             p.n_best = p.parts * 2;
             p.ldb = (B + 31) / 32 * 32;
             p.q16 = c.take<_Float16>((size_t)B * p.steps * 64);

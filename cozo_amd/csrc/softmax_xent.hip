@@ -88,9 +88,8 @@ xent_forward_kernel(Operand W, Operand Q, uint32_t steps, float scale2, uint32_t
     constexpr int BM = G::BM, BN = G::BN, WM = G::WM, WN = G::WN;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int lane = threadIdx.x & 63;
-    // workgroups go round the 8 XCDs: those that share a stretch of the table are put on one, so that its L2 holds the stretch's tile
-    const uint32_t qt = (Q.rows + BN - 1) / BN, at = blockIdx.x / 8;
-    const uint32_t n0 = at % qt * BN, part = at / qt * 8 + blockIdx.x % 8;
+    const uint32_t qt = (Q.rows + BN - 1) / BN, at = gemm::place_in_order();
+    const uint32_t n0 = at % qt * BN, part = at / qt;
     const uint32_t t0 = part * tiles_per_part, t1 = min(n_tiles, t0 + tiles_per_part);
     float m[G::NT], l[G::NT];
 #pragma unroll
@@ -189,7 +188,7 @@ xent_weights_kernel(Operand W, uint32_t v0, uint32_t V, Operand Q, uint32_t step
     constexpr int BM = G::BM, BN = G::BN;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const uint32_t qt = (ldt + BN - 1) / BN;
-    const uint32_t n0 = blockIdx.x % qt * BN, m0 = blockIdx.x / qt * BM;
+    const uint32_t at = gemm::place_in_order(), n0 = at % qt * BN, m0 = at / qt * BM;
     const int lane = threadIdx.x & 63;
     G g;
     g.run(W, m0, Q, n0, 0, steps, lds);
@@ -230,7 +229,7 @@ xent_table_grad_kernel(Operand Pt, Operand Qt, uint32_t steps, typename G::Elem:
     constexpr int BM = G::BM, BN = G::BN;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const uint32_t nt = (dim + BN - 1) / BN;
-    const uint32_t n0 = blockIdx.x % nt * BN, m0 = blockIdx.x / nt * BM;
+    const uint32_t at = gemm::place_in_order(), n0 = at % nt * BN, m0 = at / nt * BM;
     G g;
     g.run(Pt, m0, Qt, n0, 0, steps, lds);
     g.each([&](uint32_t r, uint32_t c, float v) {
@@ -245,7 +244,7 @@ xent_query_grad_kernel(Operand P, Operand Wt, uint32_t steps, uint32_t steps_per
     constexpr int BM = G::BM, BN = G::BN;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const uint32_t nt = (dim + BN - 1) / BN, mt = (P.rows + BM - 1) / BM;
-    const uint32_t n0 = blockIdx.x % nt * BN, m0 = blockIdx.x / nt % mt * BM, s = blockIdx.x / (nt * mt);
+    const uint32_t at = gemm::place_in_order(), n0 = at % nt * BN, m0 = at / nt % mt * BM, s = at / (nt * mt);
     const uint32_t s0 = s * steps_per_part, s1 = min(steps, s0 + steps_per_part);
     float *out = parts + (uint64_t)s * P.rows * dim;
     G g;
@@ -286,7 +285,7 @@ struct Shape {
 
 struct Plan {
     uint32_t piece;        // table rows worked on at a time
-    uint32_t parts;        // forward: stretches of a piece (a multiple of 8); backward: partial sums of grad_queries
+    uint32_t parts;        // forward: stretches of a piece; backward: partial sums of grad_queries
     int fwd;               // forward's tile: 0 narrow, 1 small, 2 large
     bool large_p, large_w, large_q;  // backward's tiles: of P, of grad_table, of grad_queries
     void *q, *w;           // packed copies (unaligned rows or a dim that is no multiple of a step)
@@ -325,7 +324,7 @@ Plan make_plan(const Shape &s, bool grad, void *ws) {
         pl.fwd = s.T <= 32 ? 0 : s.T > 128 && s.V >= 64 * 256 ? 2 : 1;
         const uint32_t bm = pl.fwd == 2 ? 256 : 128, bn = pl.fwd == 2 ? 256 : pl.fwd == 1 ? 128 : 32;
         const uint32_t qt = (s.T + bn - 1) / bn, tiles = (s.V + bm - 1) / bm, resident = pl.fwd == 2 ? 256 : pl.fwd == 1 ? 512 : 1024;
-        pl.parts = (uint32_t)up_to(std::max(1u, std::min(tiles, resident / qt)), 8);
+        pl.parts = std::max(1u, std::min(tiles, resident / qt));
         pl.stats = c.take<float2>((uint64_t)pl.parts * ((s.V + pl.piece - 1) / pl.piece) * s.T);
     } else {
         pl.qt = c.take<uint8_t>(s.dim * tp * es);
