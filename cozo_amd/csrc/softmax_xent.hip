@@ -41,13 +41,14 @@ xent_pack_kernel(const T *__restrict__ x, uint64_t ld, uint32_t n, uint32_t dim,
     }
 }
 
-// out[d][r] = x[r][d] for d < dim, r < n, and zeros up to row length ldo; rows whose target is no row of the table are zeros too when
+// out[d][r] = x[r][d] for d < dim, r < n, and zeros up to r = width; rows whose target is no row of the table are zeros too when
 // targets are given (what such a query holds, NaN included, must not reach a product with its zero weight).  HBM bound: 64 x 64 through LDS,
-// 16 bytes of a row read and written at a time.  `wide`: rows of x are 16-byte aligned.  ldo is a multiple of 128 bytes.
+// 16 bytes of a row read and written at a time.  `wide`: rows of x are 16-byte aligned.  width and ldo are
+// multiples of 128 bytes.
 template <typename T>
 __global__ void __launch_bounds__(256)
 xent_transpose_kernel(const T *__restrict__ x, uint64_t ld, bool wide, uint32_t n, uint32_t dim, const uint32_t *__restrict__ targets, uint32_t V,
-                      T *__restrict__ out, uint64_t ldo) {
+                      T *__restrict__ out, uint32_t width, uint64_t ldo) {
     constexpr int P = 16 / sizeof(T);  // elements of 16 bytes
     typedef T Piece __attribute__((ext_vector_type(P)));
     __shared__ T tile[64][64 + 4 / sizeof(T)];
@@ -73,7 +74,7 @@ xent_transpose_kernel(const T *__restrict__ x, uint64_t ld, bool wide, uint32_t 
 #pragma unroll
     for (uint32_t i = 0; i < 16 / P; i++) {
         const uint32_t at = i * 256 + threadIdx.x, row = at / (64 / P), c = at % (64 / P) * P, d = d0 + row, r = r0 + c;
-        if (d >= dim || r >= ldo) continue;
+        if (d >= dim || r >= width) continue;
         Piece v;
 #pragma unroll
         for (int j = 0; j < P; j++) v[j] = tile[c + j][row];
@@ -178,16 +179,16 @@ xent_join_kernel(const float2 *__restrict__ parts, uint32_t n_parts, const T *__
     loss[t] = y == CZ_NONE ? 0.f : y < V ? (float)(e - (double)scale * z) : __builtin_nanf("");
 }
 
-// P of a piece: p[t][v] and pt[v][t], zeros where the piece or the queries end
+// P of a piece: p[t][v] and pt[v][t], zeros where the piece or the queries (up to tp) end
 template <class G>
 __global__ void __launch_bounds__(G::kThreads)
 xent_weights_kernel(Operand W, uint32_t v0, uint32_t V, Operand Q, uint32_t steps, float scale, const uint32_t *__restrict__ targets,
                     const float *__restrict__ lse, const float *__restrict__ grad_loss, typename G::Elem::T *__restrict__ p, uint64_t ldp,
-                    typename G::Elem::T *__restrict__ pt, uint32_t ldt) {
+                    typename G::Elem::T *__restrict__ pt, uint32_t tp, uint64_t ldt) {
     typedef typename G::Elem E;
     constexpr int BM = G::BM, BN = G::BN;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    const uint32_t qt = (ldt + BN - 1) / BN;
+    const uint32_t qt = (tp + BN - 1) / BN;
     const uint32_t at = gemm::place_in_order(), n0 = at % qt * BN, m0 = at / qt * BM;
     const int lane = threadIdx.x & 63;
     G g;
@@ -215,7 +216,7 @@ xent_weights_kernel(Operand W, uint32_t v0, uint32_t V, Operand Q, uint32_t step
                     typedef typename E::T T4 __attribute__((ext_vector_type(4)));
                     *(T4 *)(p + t * ldp + v) = T4{o[0], o[1], o[2], o[3]};
                 }
-                if (t < ldt && pt)
+                if (t < tp && pt)
 #pragma unroll
                     for (int r = 0; r < 4; r++) pt[(uint64_t)(v + r) * ldt + t] = o[r];
             }
@@ -273,6 +274,10 @@ xent_sum_parts_kernel(const float *__restrict__ parts, uint32_t n_parts, uint64_
 // ---- host side -------------------------------------------------------------------------------------------------------
 uint64_t up_to(uint64_t x, uint64_t m) { return (x + m - 1) / m * m; }
 
+// Row length of the matrices in scratch: rows a large power of two apart would all begin in the same few memory channels, and a step of the
+// matrix loop reads the same 128 bytes of 256 rows.
+uint64_t padded(uint64_t n, uint32_t es) { return n + 128 / es; }
+
 struct Shape {
     uint32_t T, V, dim;
     uint64_t ldq, ldw;
@@ -327,10 +332,10 @@ Plan make_plan(const Shape &s, bool grad, void *ws) {
         pl.parts = std::max(1u, std::min(tiles, resident / qt));
         pl.stats = c.take<float2>((uint64_t)pl.parts * ((s.V + pl.piece - 1) / pl.piece) * s.T);
     } else {
-        pl.qt = c.take<uint8_t>(s.dim * tp * es);
-        pl.wt = c.take<uint8_t>((uint64_t)s.dim * pl.piece * es);
-        pl.p = c.take<uint8_t>((uint64_t)s.T * pl.piece * es);
-        pl.pt = c.take<uint8_t>(pl.piece * tp * es);
+        pl.qt = c.take<uint8_t>(s.dim * padded(tp, es) * es);
+        pl.wt = c.take<uint8_t>((uint64_t)s.dim * padded(pl.piece, es) * es);
+        pl.p = c.take<uint8_t>((uint64_t)s.T * padded(pl.piece, es) * es);
+        pl.pt = c.take<uint8_t>(pl.piece * padded(tp, es) * es);
         const uint32_t nv = std::min(s.V, pl.piece);
         pl.large_p = enough(nv, tp);
         pl.large_w = enough(nv, s.dim);
@@ -403,18 +408,19 @@ int forward(const Shape &s, const Plan &pl, const void *q_, const void *w_, cons
 }
 
 template <typename T>
-void transpose(const T *x, uint64_t ld, uint32_t n, uint32_t dim, const uint32_t *targets, uint32_t V, void *out, uint64_t ldo, hipStream_t stream) {
+void transpose(const T *x, uint64_t ld, uint32_t n, uint32_t dim, const uint32_t *targets, uint32_t V, void *out, uint32_t width, uint64_t ldo,
+               hipStream_t stream) {
     const bool wide = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && ld * sizeof(T) % 16 == 0;
-    hipLaunchKernelGGL(xent_transpose_kernel<T>, dim3((uint32_t)((ldo + 63) / 64), (dim + 63) / 64), dim3(256), 0, stream, x, ld, wide, n, dim,
-                       targets, V, (T *)out, ldo);
+    hipLaunchKernelGGL(xent_transpose_kernel<T>, dim3((width + 63) / 64, (dim + 63) / 64), dim3(256), 0, stream, x, ld, wide, n, dim, targets, V,
+                       (T *)out, width, ldo);
 }
 
 template <class G>
 int weights_of(const Operand &W, uint32_t v0, uint32_t V, const Operand &Q, uint32_t steps, float scale, const uint32_t *targets, const float *lse,
-               const float *grad_loss, void *p, uint64_t vp, void *pt, uint32_t tp, hipStream_t stream) {
+               const float *grad_loss, void *p, uint32_t vp, uint64_t ldp, void *pt, uint32_t tp, uint64_t ldt, hipStream_t stream) {
     typedef typename G::Elem::T T;
     return launch<G>(xent_weights_kernel<G>, tiles_of(vp, G::BM) * tiles_of(tp, G::BN), stream, W, v0, V, Q, steps, scale, targets, lse, grad_loss,
-                     (T *)p, vp, (T *)pt, tp);
+                     (T *)p, ldp, (T *)pt, tp, ldt);
 }
 template <class G>
 int table_grad_of(const Operand &Pt, const Operand &Qt, uint32_t steps, typename G::Elem::T *out, uint32_t dim, hipStream_t stream) {
@@ -438,9 +444,11 @@ int backward(const Shape &s, const Plan &pl, const void *q_, const void *w_, con
         Q = Operand{(const char *)pl.q, (uint64_t)kp * es, s.T};
     }
     const bool wd = direct(w, s.ldw, s.dim, es);
-    if (dw) transpose(q, s.ldq, s.T, s.dim, targets, s.V, pl.qt, tp, stream);
+    const uint64_t ldt = padded(tp, es);
+    if (dw) transpose(q, s.ldq, s.T, s.dim, targets, s.V, pl.qt, tp, ldt, stream);
     for (uint32_t v0 = 0; v0 < s.V; v0 += pl.piece) {
         const uint32_t nv = std::min(pl.piece, s.V - v0), vp = (uint32_t)up_to(nv, 256);
+        const uint64_t ldp = padded(vp, es);
         const T *wv = w + v0 * s.ldw;
         Operand W{(const char *)wv, s.ldw * es, nv};
         if (!wd) {
@@ -448,19 +456,19 @@ int backward(const Shape &s, const Plan &pl, const void *q_, const void *w_, con
             W = Operand{(const char *)pl.w, (uint64_t)kp * es, nv};
         }
         void *p = dq ? pl.p : nullptr, *pt = dw ? pl.pt : nullptr;
-        int rc = pl.large_p ? weights_of<Large<E>>(W, v0, s.V, Q, steps, scale, targets, lse, grad_loss, p, vp, pt, tp, stream)
-                            : weights_of<Small<E>>(W, v0, s.V, Q, steps, scale, targets, lse, grad_loss, p, vp, pt, tp, stream);
+        int rc = pl.large_p ? weights_of<Large<E>>(W, v0, s.V, Q, steps, scale, targets, lse, grad_loss, p, vp, ldp, pt, tp, ldt, stream)
+                            : weights_of<Small<E>>(W, v0, s.V, Q, steps, scale, targets, lse, grad_loss, p, vp, ldp, pt, tp, ldt, stream);
         if (rc) return rc;
         if (dw) {
-            const Operand Pt{(const char *)pl.pt, (uint64_t)tp * es, nv}, Qt{(const char *)pl.qt, (uint64_t)tp * es, s.dim};
+            const Operand Pt{(const char *)pl.pt, ldt * es, nv}, Qt{(const char *)pl.qt, ldt * es, s.dim};
             T *out = (T *)dw + (uint64_t)v0 * s.dim;
             rc = pl.large_w ? table_grad_of<Large<E>>(Pt, Qt, tp / s.kstep(), out, s.dim, stream)
                             : table_grad_of<Small<E>>(Pt, Qt, tp / s.kstep(), out, s.dim, stream);
             if (rc) return rc;
         }
         if (dq) {
-            transpose(wv, s.ldw, nv, s.dim, (const uint32_t *)nullptr, 0u, pl.wt, vp, stream);
-            const Operand P{(const char *)pl.p, (uint64_t)vp * es, s.T}, Wt{(const char *)pl.wt, (uint64_t)vp * es, s.dim};
+            transpose(wv, s.ldw, nv, s.dim, (const uint32_t *)nullptr, 0u, pl.wt, vp, ldp, stream);
+            const Operand P{(const char *)pl.p, ldp * es, s.T}, Wt{(const char *)pl.wt, ldp * es, s.dim};
             rc = pl.large_q ? query_grad_of<Large<E>>(P, Wt, vp / s.kstep(), pl.parts, v0 != 0, pl.dq, s.dim, stream)
                             : query_grad_of<Small<E>>(P, Wt, vp / s.kstep(), pl.parts, v0 != 0, pl.dq, s.dim, stream);
             if (rc) return rc;
