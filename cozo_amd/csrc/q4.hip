@@ -868,7 +868,7 @@ struct Candidates {
 
 // per (chunk of tiles, query): the k nearest rows of the chunk's candidate tiles as a sorted partial list
 template <int LPR>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 3)
 q4_scan_kernel(int metric, Rows t, const float *__restrict__ queries, uint32_t k, uint32_t tiles_per_chunk, Candidates cand,
                uint64_t *__restrict__ part_key, uint32_t *__restrict__ part_id, uint32_t *__restrict__ part_count) {
     extern __shared__ __attribute__((aligned(16))) char smem_raw[];
@@ -878,8 +878,8 @@ q4_scan_kernel(int metric, Rows t, const float *__restrict__ queries, uint32_t k
     double *red = (double *)(tkey + k);           // [4]
     uint32_t *bid = (uint32_t *)(red + 4);        // [256]
     uint32_t *tid_ = bid + 256;                   // [k]
-    uint32_t *list = tid_ + k;                    // [256] candidate tiles
-    uint32_t *cnt = list + 256;                   // [5]
+    uint32_t *list = tid_ + k;                    // [1024] candidate tiles
+    uint32_t *cnt = list + 1024;                  // [5]
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, sub = tid % LPR;
     const uint32_t b = blockIdx.y;
     const uint32_t n_tiles = (uint32_t)(((uint64_t)t.n + kTile - 1) / kTile);
@@ -890,23 +890,37 @@ q4_scan_kernel(int metric, Rows t, const float *__restrict__ queries, uint32_t k
     bool ready = false;
     int tcnt = 0;
     if (tid == 0) cnt[4] = 0;  // rows in the batch
-    for (uint32_t tb = t0; tb < t1; tb += 256) {
-        const uint32_t tile = tb + tid;
-        bool want = tile < t1;
-        if (want && cand.tile_score) {
-            const float s = cand.tile_score[(uint64_t)b * n_tiles + tile];
-            want = !(s + score_error(metric, cand.err, qn, cand.tile_norm[tile]) < need);
+    for (uint32_t tb = t0; tb < t1; tb += 1024) {
+        unsigned long long m[4];
+        uint32_t at = 0, total = 0;
+        bool want[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t tile = tb + 256 * i + tid;
+            want[i] = tile < t1;
+            if (want[i] && cand.tile_score) {
+                const float s = cand.tile_score[(uint64_t)b * n_tiles + tile];
+                want[i] = !(s + score_error(metric, cand.err, qn, cand.tile_norm[tile]) < need);
+            }
         }
-        const unsigned long long m = __ballot(want);
-        if (lane == 0) cnt[wave] = __popcll(m);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            m[i] = __ballot(want[i]);
+            total += __popcll(m[i]);
+        }
+        if (lane == 0) cnt[wave] = total;
         __syncthreads();
-        uint32_t at = __popcll(m & ((1ull << lane) - 1ull)), total = 0;
+        total = 0;
 #pragma unroll
         for (int w = 0; w < 4; w++) {
             if (w < wave) at += cnt[w];
             total += cnt[w];
         }
-        if (want) list[at] = tile;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (want[i]) list[at + __popcll(m[i] & ((1ull << lane) - 1ull))] = tb + 256 * i + tid;
+            at += __popcll(m[i]);
+        }
         __syncthreads();
         if (total && !ready) {  // the query, once there is something to look at
             for (uint32_t i = tid; i < t.chunks * 8; i += 256) {
@@ -1474,7 +1488,7 @@ extern "C" int cz_q4_knn(int metric, const uint8_t *codes, const uint16_t *scale
     if ((rc = cz::scratch_of(ws, ws_bytes, cz_q4_workspace(n, dim, group, B, k), own, &base))) return rc;
     t.codes = codes;
     t.scales = scales;
-    const size_t smem = 256 * 16 + (size_t)k * 12 + 64 + (size_t)t.chunks * 64;
+    const size_t smem = 256 * 12 + 1024 * 4 + (size_t)k * 12 + 64 + (size_t)t.chunks * 64;
     const uint32_t lpr = lanes_per_row(t.chunks);
     const uint32_t turn = turn_of(t);
     for (uint32_t b0 = 0; b0 < B; b0 += turn) {

@@ -259,15 +259,29 @@ xent_query_grad_kernel(Operand P, Operand Wt, uint32_t steps, uint32_t steps_per
     });
 }
 
+// grad_queries: the partial sums added up, four lanes to an element and four sums in flight in each
 template <typename T>
 __global__ void __launch_bounds__(256)
 xent_sum_parts_kernel(const float *__restrict__ parts, uint32_t n_parts, uint64_t n, uint32_t dim, const uint32_t *__restrict__ targets,
                       uint32_t V, T *__restrict__ out) {
-    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (uint64_t)gridDim.x * 256) {
-        float a = 0.f;
-        for (uint32_t p = 0; p < n_parts; p++) a += parts[p * n + i];
-        if (targets && !has_answer(targets[i / dim], V)) a = 0.f;  // (zero weights times a row that is not finite)
-        out[i] = down<T>(a);
+    __shared__ float sums[4][64];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (uint64_t i0 = (uint64_t)blockIdx.x * 64; i0 < n; i0 += (uint64_t)gridDim.x * 64) {
+        const uint64_t i = i0 + lane;
+        float a[4] = {0.f, 0.f, 0.f, 0.f};
+        if (i < n)
+            for (uint32_t p = wave; p < n_parts; p += 16)
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+                    if (p + 4 * u < n_parts) a[u] += parts[(p + 4 * u) * n + i];
+        sums[wave][lane] = (a[0] + a[1]) + (a[2] + a[3]);
+        __syncthreads();
+        if (wave == 0 && i < n) {
+            float v = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
+            if (targets && !has_answer(targets[i / dim], V)) v = 0.f;  // (zero weights times a row that is not finite)
+            out[i] = down<T>(v);
+        }
+        __syncthreads();
     }
 }
 
@@ -341,7 +355,8 @@ Plan make_plan(const Shape &s, bool grad, void *ws) {
         pl.large_w = enough(nv, s.dim);
         pl.large_q = s.T > 128 && s.dim > 128;
         const uint32_t b = pl.large_q ? 256 : 128, tiles = ((s.T + b - 1) / b) * ((s.dim + b - 1) / b);
-        pl.parts = std::max(1u, std::min({(pl.large_q ? 256 : 512) / tiles, 64u, pl.piece / 1024}));
+        // as many stretches of a piece as fill the chip, of at least 8 steps
+        pl.parts = std::max(1u, std::min((pl.large_q ? 256 : 512) / tiles, (uint32_t)(up_to(nv, 256) / s.kstep() / 8)));
         pl.dq = c.take<float>((uint64_t)pl.parts * s.T * s.dim);
     }
     pl.bytes = c.used();
@@ -475,7 +490,7 @@ int backward(const Shape &s, const Plan &pl, const void *q_, const void *w_, con
         }
     }
     if (dq)
-        hipLaunchKernelGGL(xent_sum_parts_kernel<T>, dim3(grid_of((uint64_t)s.T * s.dim)), dim3(256), 0, stream, pl.dq, pl.parts,
+        hipLaunchKernelGGL(xent_sum_parts_kernel<T>, dim3(grid_of((uint64_t)s.T * s.dim * 4)), dim3(256), 0, stream, pl.dq, pl.parts,
                            (uint64_t)s.T * s.dim, s.dim, targets, s.V, (T *)dq);
     return launched("cz_softmax_xent_grad");
 }
@@ -572,10 +587,10 @@ extern "C" int cz_softmax_xent_grad(const void *queries, uint64_t ldq, const voi
         }
         if ((rc = cz::check_device_ptr(grad_table, "grad_table"))) return rc;
         if (s.bf16)
-            hipLaunchKernelGGL(xent_sum_parts_kernel<__bf16>, dim3(grid_of((uint64_t)V * dim)), dim3(256), 0, stream, (const float *)nullptr, 0u,
+            hipLaunchKernelGGL(xent_sum_parts_kernel<__bf16>, dim3(grid_of((uint64_t)V * dim * 4)), dim3(256), 0, stream, (const float *)nullptr, 0u,
                                (uint64_t)V * dim, dim, (const uint32_t *)nullptr, V, (__bf16 *)grad_table);
         else
-            hipLaunchKernelGGL(xent_sum_parts_kernel<float>, dim3(grid_of((uint64_t)V * dim)), dim3(256), 0, stream, (const float *)nullptr, 0u,
+            hipLaunchKernelGGL(xent_sum_parts_kernel<float>, dim3(grid_of((uint64_t)V * dim * 4)), dim3(256), 0, stream, (const float *)nullptr, 0u,
                                (uint64_t)V * dim, dim, (const uint32_t *)nullptr, V, (float *)grad_table);
         return launched("cz_softmax_xent_grad");
     }
