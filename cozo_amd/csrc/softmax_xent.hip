@@ -5,7 +5,8 @@
 // joined once, at the end of a workgroup's stretch of the table.  Stretches are joined in a second launch.
 // Gradient, a piece of the table at a time:  P = grad_loss scale (softmax - onehot) of the piece is computed again and stored in both
 // orders, then  dW = P^T Q  is written and  dq += P W  goes to per-stretch partial sums (each added to by one workgroup only, in
-// a fixed order: no atomics).
+// a fixed order: no atomics).  A bf16 P loses what it rounds off; where that matters most, at the answers -- the largest entries, which may well
+// carry all the same value and so the same error -- the rest is kept in f32 and its term added to dW's row and to dq in f32.
 #include <algorithm>
 #include <cmath>
 
@@ -179,12 +180,12 @@ xent_join_kernel(const float2 *__restrict__ parts, uint32_t n_parts, const T *__
     loss[t] = y == CZ_NONE ? 0.f : y < V ? (float)(e - (double)scale * z) : __builtin_nanf("");
 }
 
-// P of a piece: p[t][v] and pt[v][t], zeros where the piece or the queries (up to tp) end
+// P of a piece: p[t][v] and pt[v][t], zeros where the piece or the queries (up to tp) end; rest[t]: what rounding the answer's entry cut off
 template <class G>
 __global__ void __launch_bounds__(G::kThreads)
 xent_weights_kernel(Operand W, uint32_t v0, uint32_t V, Operand Q, uint32_t steps, float scale, const uint32_t *__restrict__ targets,
                     const float *__restrict__ lse, const float *__restrict__ grad_loss, typename G::Elem::T *__restrict__ p, uint64_t ldp,
-                    typename G::Elem::T *__restrict__ pt, uint32_t tp, uint64_t ldt) {
+                    typename G::Elem::T *__restrict__ pt, uint32_t tp, uint64_t ldt, float *__restrict__ rest) {
     typedef typename G::Elem E;
     constexpr int BM = G::BM, BN = G::BN;
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -209,8 +210,11 @@ xent_weights_kernel(Operand W, uint32_t v0, uint32_t V, Operand Q, uint32_t step
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     float x = exp2_(fmaf(g.acc[i][j][4 * r4 + r], scale2, -l2));
-                    if (v0 + v + r == y) x -= 1.f;
-                    o[r] = down<typename E::T>(on && v + r < W.rows ? x * weight : 0.f);
+                    const bool hit = on && v0 + v + r == y;
+                    if (hit) x -= 1.f;
+                    x = on && v + r < W.rows ? x * weight : 0.f;
+                    o[r] = down<typename E::T>(x);
+                    if (hit && rest) rest[t] = x - up(o[r]);
                 }
                 if (t < Q.rows && p) {
                     typedef typename E::T T4 __attribute__((ext_vector_type(4)));
@@ -223,16 +227,63 @@ xent_weights_kernel(Operand W, uint32_t v0, uint32_t V, Operand Q, uint32_t step
     }
 }
 
-// grad_table rows of a piece: pt [rows][ldt] . qt [dim][ldt]^T
+// what is left of the answers' own terms (rest = null: nothing, P is f32)
+template <typename T>
+struct Answers {
+    const uint32_t *targets;
+    const float *rest;
+    const T *q, *w;
+    uint64_t ldq, ldw;
+    uint32_t T_n, V;
+};
+
+// grad_table rows of a piece (rows v0 ... of the table): pt [rows][ldt] . qt [dim][ldt]^T, and the rest for the queries that the rows answer
 template <class G>
 __global__ void __launch_bounds__(G::kThreads)
-xent_table_grad_kernel(Operand Pt, Operand Qt, uint32_t steps, typename G::Elem::T *__restrict__ out, uint32_t dim) {
-    constexpr int BM = G::BM, BN = G::BN;
+xent_table_grad_kernel(Operand Pt, Operand Qt, uint32_t steps, Answers<typename G::Elem::T> an, uint32_t v0, typename G::Elem::T *__restrict__ out,
+                       uint32_t dim) {
+    constexpr int BM = G::BM, BN = G::BN, kWaves = G::kThreads / 64;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const uint32_t nt = (dim + BN - 1) / BN;
     const uint32_t at = gemm::place_in_order(), n0 = at % nt * BN, m0 = at / nt * BM;
     G g;
     g.run(Pt, m0, Qt, n0, 0, steps, lds);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t *count = (uint32_t *)lds, *list = count + kWaves;  // of each wave; the queries that rows of this tile answer, ascending
+    if (an.rest)
+    for (uint32_t t0 = 0; t0 < an.T_n; t0 += G::kThreads) {
+        const uint32_t t = t0 + threadIdx.x, y = t < an.T_n ? an.targets[t] : CZ_NONE;
+        const bool here = y < an.V && y >= v0 + m0 && y - v0 - m0 < BM;
+        if (!__syncthreads_or(here)) continue;  // (the LDS is free after it: the product's last reads lie before)
+        const unsigned long long m = __ballot(here);
+        if (lane == 0) count[wave] = __popcll(m);
+        __syncthreads();
+        uint32_t first = 0, total = 0;
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) {
+            if (w < wave) first += count[w];
+            total += count[w];
+        }
+        if (here) list[first + __popcll(m & ((1ull << lane) - 1ull))] = t;
+        __syncthreads();
+        for (uint32_t i = 0; i < total; i++) {
+            const uint32_t tq = list[i];
+            const int row = (int)(an.targets[tq] - v0 - m0) - G::wave_row() - 4 * (lane >> 5);
+            if (row < -4 || row >= BM / G::WM) continue;  // (another wave's)
+            const float rest = an.rest[tq];
+#pragma unroll
+            for (int j = 0; j < G::NT; j++) {
+                const uint32_t c = n0 + G::wave_col() + j * 32 + (lane & 31);
+                const float x = c < dim ? up(an.q[tq * an.ldq + c]) * rest : 0.f;
+#pragma unroll
+                for (int k = 0; k < G::MT; k++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++)
+                        if (row == k * 32 + 8 * (r >> 2) + (r & 3)) g.acc[k][j][r] += x;
+            }
+        }
+        __syncthreads();
+    }
     g.each([&](uint32_t r, uint32_t c, float v) {
         if (m0 + r < Pt.rows && n0 + c < dim) out[(uint64_t)(m0 + r) * dim + n0 + c] = down<typename G::Elem::T>(v);
     });
@@ -259,11 +310,10 @@ xent_query_grad_kernel(Operand P, Operand Wt, uint32_t steps, uint32_t steps_per
     });
 }
 
-// grad_queries: the partial sums added up, four lanes to an element and four sums in flight in each
+// grad_queries: the partial sums added up, and the rest for the rows that answer; four lanes to an element and four sums in flight in each
 template <typename T>
 __global__ void __launch_bounds__(256)
-xent_sum_parts_kernel(const float *__restrict__ parts, uint32_t n_parts, uint64_t n, uint32_t dim, const uint32_t *__restrict__ targets,
-                      uint32_t V, T *__restrict__ out) {
+xent_sum_parts_kernel(const float *__restrict__ parts, uint32_t n_parts, uint64_t n, uint32_t dim, Answers<T> an, T *__restrict__ out) {
     __shared__ float sums[4][64];
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (uint64_t i0 = (uint64_t)blockIdx.x * 64; i0 < n; i0 += (uint64_t)gridDim.x * 64) {
@@ -278,7 +328,11 @@ xent_sum_parts_kernel(const float *__restrict__ parts, uint32_t n_parts, uint64_
         __syncthreads();
         if (wave == 0 && i < n) {
             float v = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
-            if (targets && !has_answer(targets[i / dim], V)) v = 0.f;  // (zero weights times a row that is not finite)
+            if (an.targets) {
+                const uint32_t t = (uint32_t)(i / dim), y = an.targets[t];
+                // (without an answer: zero weights, which a table row that is not finite would have made more of)
+                v = !has_answer(y, an.V) ? 0.f : an.rest ? v + an.rest[t] * up(an.w[y * an.ldw + (i - (uint64_t)t * dim)]) : v;
+            }
             out[i] = down<T>(v);
         }
         __syncthreads();
@@ -310,7 +364,7 @@ struct Plan {
     void *q, *w;           // packed copies (unaligned rows or a dim that is no multiple of a step)
     void *qt, *wt, *p, *pt;
     float2 *stats;
-    float *dq;
+    float *dq, *rest;
     size_t bytes;
 };
 
@@ -357,6 +411,7 @@ Plan make_plan(const Shape &s, bool grad, void *ws) {
         const uint32_t b = pl.large_q ? 256 : 128, tiles = ((s.T + b - 1) / b) * ((s.dim + b - 1) / b);
         // as many stretches of a piece as fill the chip, of at least 8 steps
         pl.parts = std::max(1u, std::min((pl.large_q ? 256 : 512) / tiles, (uint32_t)(up_to(nv, 256) / s.kstep() / 8)));
+        pl.rest = s.bf16 ? c.take<float>(s.T) : nullptr;
         pl.dq = c.take<float>((uint64_t)pl.parts * s.T * s.dim);
     }
     pl.bytes = c.used();
@@ -432,14 +487,15 @@ void transpose(const T *x, uint64_t ld, uint32_t n, uint32_t dim, const uint32_t
 
 template <class G>
 int weights_of(const Operand &W, uint32_t v0, uint32_t V, const Operand &Q, uint32_t steps, float scale, const uint32_t *targets, const float *lse,
-               const float *grad_loss, void *p, uint32_t vp, uint64_t ldp, void *pt, uint32_t tp, uint64_t ldt, hipStream_t stream) {
+               const float *grad_loss, void *p, uint32_t vp, uint64_t ldp, void *pt, uint32_t tp, uint64_t ldt, float *rest, hipStream_t stream) {
     typedef typename G::Elem::T T;
     return launch<G>(xent_weights_kernel<G>, tiles_of(vp, G::BM) * tiles_of(tp, G::BN), stream, W, v0, V, Q, steps, scale, targets, lse, grad_loss,
-                     (T *)p, ldp, (T *)pt, tp, ldt);
+                     (T *)p, ldp, (T *)pt, tp, ldt, rest);
 }
 template <class G>
-int table_grad_of(const Operand &Pt, const Operand &Qt, uint32_t steps, typename G::Elem::T *out, uint32_t dim, hipStream_t stream) {
-    return launch<G>(xent_table_grad_kernel<G>, tiles_of(Pt.rows, G::BM) * tiles_of(dim, G::BN), stream, Pt, Qt, steps, out, dim);
+int table_grad_of(const Operand &Pt, const Operand &Qt, uint32_t steps, const Answers<typename G::Elem::T> &an, uint32_t v0,
+                  typename G::Elem::T *out, uint32_t dim, hipStream_t stream) {
+    return launch<G>(xent_table_grad_kernel<G>, tiles_of(Pt.rows, G::BM) * tiles_of(dim, G::BN), stream, Pt, Qt, steps, an, v0, out, dim);
 }
 template <class G>
 int query_grad_of(const Operand &P, const Operand &Wt, uint32_t steps, uint32_t parts, bool add, float *dq, uint32_t dim, hipStream_t stream) {
@@ -460,6 +516,7 @@ int backward(const Shape &s, const Plan &pl, const void *q_, const void *w_, con
     }
     const bool wd = direct(w, s.ldw, s.dim, es);
     const uint64_t ldt = padded(tp, es);
+    const Answers<T> an{targets, pl.rest, q, w, s.ldq, s.ldw, s.T, s.V};
     if (dw) transpose(q, s.ldq, s.T, s.dim, targets, s.V, pl.qt, tp, ldt, stream);
     for (uint32_t v0 = 0; v0 < s.V; v0 += pl.piece) {
         const uint32_t nv = std::min(pl.piece, s.V - v0), vp = (uint32_t)up_to(nv, 256);
@@ -471,14 +528,14 @@ int backward(const Shape &s, const Plan &pl, const void *q_, const void *w_, con
             W = Operand{(const char *)pl.w, (uint64_t)kp * es, nv};
         }
         void *p = dq ? pl.p : nullptr, *pt = dw ? pl.pt : nullptr;
-        int rc = pl.large_p ? weights_of<Large<E>>(W, v0, s.V, Q, steps, scale, targets, lse, grad_loss, p, vp, ldp, pt, tp, ldt, stream)
-                            : weights_of<Small<E>>(W, v0, s.V, Q, steps, scale, targets, lse, grad_loss, p, vp, ldp, pt, tp, ldt, stream);
+        int rc = pl.large_p ? weights_of<Large<E>>(W, v0, s.V, Q, steps, scale, targets, lse, grad_loss, p, vp, ldp, pt, tp, ldt, pl.rest, stream)
+                            : weights_of<Small<E>>(W, v0, s.V, Q, steps, scale, targets, lse, grad_loss, p, vp, ldp, pt, tp, ldt, pl.rest, stream);
         if (rc) return rc;
         if (dw) {
             const Operand Pt{(const char *)pl.pt, ldt * es, nv}, Qt{(const char *)pl.qt, ldt * es, s.dim};
             T *out = (T *)dw + (uint64_t)v0 * s.dim;
-            rc = pl.large_w ? table_grad_of<Large<E>>(Pt, Qt, tp / s.kstep(), out, s.dim, stream)
-                            : table_grad_of<Small<E>>(Pt, Qt, tp / s.kstep(), out, s.dim, stream);
+            rc = pl.large_w ? table_grad_of<Large<E>>(Pt, Qt, tp / s.kstep(), an, v0, out, s.dim, stream)
+                            : table_grad_of<Small<E>>(Pt, Qt, tp / s.kstep(), an, v0, out, s.dim, stream);
             if (rc) return rc;
         }
         if (dq) {
@@ -491,7 +548,7 @@ int backward(const Shape &s, const Plan &pl, const void *q_, const void *w_, con
     }
     if (dq)
         hipLaunchKernelGGL(xent_sum_parts_kernel<T>, dim3(grid_of((uint64_t)s.T * s.dim * 4)), dim3(256), 0, stream, pl.dq, pl.parts,
-                           (uint64_t)s.T * s.dim, s.dim, targets, s.V, (T *)dq);
+                           (uint64_t)s.T * s.dim, s.dim, an, (T *)dq);
     return launched("cz_softmax_xent_grad");
 }
 
@@ -588,10 +645,10 @@ extern "C" int cz_softmax_xent_grad(const void *queries, uint64_t ldq, const voi
         if ((rc = cz::check_device_ptr(grad_table, "grad_table"))) return rc;
         if (s.bf16)
             hipLaunchKernelGGL(xent_sum_parts_kernel<__bf16>, dim3(grid_of((uint64_t)V * dim * 4)), dim3(256), 0, stream, (const float *)nullptr, 0u,
-                               (uint64_t)V * dim, dim, (const uint32_t *)nullptr, V, (__bf16 *)grad_table);
+                               (uint64_t)V * dim, dim, Answers<__bf16>{}, (__bf16 *)grad_table);
         else
             hipLaunchKernelGGL(xent_sum_parts_kernel<float>, dim3(grid_of((uint64_t)V * dim * 4)), dim3(256), 0, stream, (const float *)nullptr, 0u,
-                               (uint64_t)V * dim, dim, (const uint32_t *)nullptr, V, (float *)grad_table);
+                               (uint64_t)V * dim, dim, Answers<float>{}, (float *)grad_table);
         return launched("cz_softmax_xent_grad");
     }
     if (!lse || !grad_loss) return cz::set_error(CZ_E_INVALID, "null buffer");
