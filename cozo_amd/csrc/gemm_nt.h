@@ -60,9 +60,13 @@ __device__ __forceinline__ uint32_t place_in_order() {
 // rows of one operand as a workgroup sees them; rows past the last one are read as the last one (the epilogue drops them)
 struct Operand {
     const char *base;
-    uint64_t ld;     // bytes
+    uint64_t ld;            // bytes from a row to the next
     uint32_t rows;
+    uint64_t step = 128;    // bytes from a step of k to the next: 128 in ordinary rows, more where k is cut into panels
 };
+// k in panels: a step's 128 bytes of every row lie one behind the other, so that a workgroup's step is one run of memory (rows that are 128 KB
+// long put each row of a step into a page of its own: grad_queries of a 65536-row piece took 169 us instead of XXX)
+inline Operand panels(const void *base, uint32_t rows) { return Operand{(const char *)base, 128, rows, (uint64_t)rows * 128}; }
 
 // BM x BN by WM x WN waves.  Measured with 1024 rows of B, 1M rows of A, k = 768, bf16: 128 x 128 by 2 x 2 900 TFLOP/s (32 bytes of copies
 // a clock and CU; its matrix cores are busy 45 % of the time), 256 x 256 by 2 x 4 1185 (52 %; a library's 8192^3 product: 1537).  Zeros for
@@ -145,20 +149,20 @@ struct Tile {
                 __builtin_amdgcn_sched_group_barrier(0x008, E::kPerPiece, 0);
             }
     }
-    // one tile: A rows from m0, B rows from n0, `steps` >= 1 steps from byte k0 of a row on
-    __device__ __forceinline__ void run(const Operand &A, uint32_t m0, const Operand &B, uint32_t n0, uint64_t k0, uint32_t steps, char *lds) {
+    // one tile: A rows from m0, B rows from n0, `steps` >= 1 steps from step s0 on
+    __device__ __forceinline__ void run(const Operand &A, uint32_t m0, const Operand &B, uint32_t n0, uint32_t s0, uint32_t steps, char *lds) {
         const char *sa[NA], *sb[NB];
         rows_of(A, m0, sa);
         rows_of(B, n0, sb);
         zero();
-        copy(sa, k0, lds);
-        copy(sb, k0, lds + BM * 128);
+        copy(sa, s0 * A.step, lds);
+        copy(sb, s0 * B.step, lds + BM * 128);
         for (uint32_t s = 0; s < steps; s++) {
             char *cur = lds + (s & 1) * kBytes, *nxt = lds + (~s & 1) * kBytes;
             arrived();
             if (s + 1 < steps) {
-                copy(sa, k0 + (uint64_t)(s + 1) * 128, nxt);
-                copy(sb, k0 + (uint64_t)(s + 1) * 128, nxt + BM * 128);
+                copy(sa, (s0 + s + 1) * A.step, nxt);
+                copy(sb, (s0 + s + 1) * B.step, nxt + BM * 128);
             }
             step(cur);
         }

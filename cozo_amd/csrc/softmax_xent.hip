@@ -31,6 +31,13 @@ __device__ __forceinline__ bool has_answer(uint32_t y, uint32_t V) { return y < 
 __device__ __forceinline__ float reference(float m) { return fabsf(m) < __builtin_inff() ? m : 0.f; }
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// place of element (row, k) of a matrix of `rows` rows in panels of k (gemm_nt.h)
+template <typename T>
+__device__ __forceinline__ uint64_t in_panels(uint32_t row, uint32_t k, uint32_t rows) {
+    constexpr uint32_t W = 128 / sizeof(T);
+    return ((uint64_t)(k / W) * rows + row) * W + k % W;
+}
+
 // rows [r0, r0 + n) of x, their first dim elements and zeros up to ldo, one 16-byte aligned row behind the other
 template <typename T>
 __global__ void __launch_bounds__(256)
@@ -42,14 +49,13 @@ xent_pack_kernel(const T *__restrict__ x, uint64_t ld, uint32_t n, uint32_t dim,
     }
 }
 
-// out[d][r] = x[r][d] for d < dim, r < n, and zeros up to r = width; rows whose target is no row of the table are zeros too when
-// targets are given (what such a query holds, NaN included, must not reach a product with its zero weight).  HBM bound: 64 x 64 through LDS,
-// 16 bytes of a row read and written at a time.  `wide`: rows of x are 16-byte aligned.  width and ldo are
-// multiples of 128 bytes.
+// out[d][r] = x[r][d] in panels of r, for d < dim, r < n, and zeros up to r = width; rows whose target is no row of the table are zeros too
+// when targets are given (what such a query holds, NaN included, must not reach a product with its zero weight).  HBM bound: 64 x 64 through
+// LDS, 16 bytes of a row read and written at a time.  `wide`: rows of x are 16-byte aligned.  width is a multiple of a panel's.
 template <typename T>
 __global__ void __launch_bounds__(256)
 xent_transpose_kernel(const T *__restrict__ x, uint64_t ld, bool wide, uint32_t n, uint32_t dim, const uint32_t *__restrict__ targets, uint32_t V,
-                      T *__restrict__ out, uint32_t width, uint64_t ldo) {
+                      T *__restrict__ out, uint32_t width) {
     constexpr int P = 16 / sizeof(T);  // elements of 16 bytes
     typedef T Piece __attribute__((ext_vector_type(P)));
     __shared__ T tile[64][64 + 4 / sizeof(T)];
@@ -79,7 +85,7 @@ xent_transpose_kernel(const T *__restrict__ x, uint64_t ld, bool wide, uint32_t 
         Piece v;
 #pragma unroll
         for (int j = 0; j < P; j++) v[j] = tile[c + j][row];
-        *(Piece *)(out + (uint64_t)d * ldo + r) = v;
+        *(Piece *)(out + in_panels<T>(d, r, dim)) = v;
     }
 }
 
@@ -180,12 +186,12 @@ xent_join_kernel(const float2 *__restrict__ parts, uint32_t n_parts, const T *__
     loss[t] = y == CZ_NONE ? 0.f : y < V ? (float)(e - (double)scale * z) : __builtin_nanf("");
 }
 
-// P of a piece: p[t][v] and pt[v][t], zeros where the piece or the queries (up to tp) end; rest[t]: what rounding the answer's entry cut off
+// P of a piece: p[t][v] and pt[v][t], in panels of v and of t, zeros where the piece or the queries (up to tp) end; rest[t]: what rounding the answer's entry cut off
 template <class G>
 __global__ void __launch_bounds__(G::kThreads)
 xent_weights_kernel(Operand W, uint32_t v0, uint32_t V, Operand Q, uint32_t steps, float scale, const uint32_t *__restrict__ targets,
-                    const float *__restrict__ lse, const float *__restrict__ grad_loss, typename G::Elem::T *__restrict__ p, uint64_t ldp,
-                    typename G::Elem::T *__restrict__ pt, uint32_t tp, uint64_t ldt, float *__restrict__ rest) {
+                    const float *__restrict__ lse, const float *__restrict__ grad_loss, typename G::Elem::T *__restrict__ p,
+                    typename G::Elem::T *__restrict__ pt, uint32_t vp, uint32_t tp, float *__restrict__ rest) {
     typedef typename G::Elem E;
     constexpr int BM = G::BM, BN = G::BN;
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -218,11 +224,11 @@ xent_weights_kernel(Operand W, uint32_t v0, uint32_t V, Operand Q, uint32_t step
                 }
                 if (t < Q.rows && p) {
                     typedef typename E::T T4 __attribute__((ext_vector_type(4)));
-                    *(T4 *)(p + t * ldp + v) = T4{o[0], o[1], o[2], o[3]};
+                    *(T4 *)(p + in_panels<typename E::T>(t, v, Q.rows)) = T4{o[0], o[1], o[2], o[3]};
                 }
                 if (t < tp && pt)
 #pragma unroll
-                    for (int r = 0; r < 4; r++) pt[(uint64_t)(v + r) * ldt + t] = o[r];
+                    for (int r = 0; r < 4; r++) pt[in_panels<typename E::T>(v + r, t, vp)] = o[r];
             }
     }
 }
@@ -237,11 +243,11 @@ struct Answers {
     uint32_t T_n, V;
 };
 
-// grad_table rows of a piece (rows v0 ... of the table): pt [rows][ldt] . qt [dim][ldt]^T, and the rest for the queries that the rows answer
+// grad_table rows of a piece (rows v0 ... of the table): pt . qt^T, and the rest for the queries that the rows answer
 template <class G>
 __global__ void __launch_bounds__(G::kThreads)
-xent_table_grad_kernel(Operand Pt, Operand Qt, uint32_t steps, Answers<typename G::Elem::T> an, uint32_t v0, typename G::Elem::T *__restrict__ out,
-                       uint32_t dim) {
+xent_table_grad_kernel(Operand Pt, Operand Qt, uint32_t steps, Answers<typename G::Elem::T> an, uint32_t v0, uint32_t rows,
+                       typename G::Elem::T *__restrict__ out, uint32_t dim) {
     constexpr int BM = G::BM, BN = G::BN, kWaves = G::kThreads / 64;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const uint32_t nt = (dim + BN - 1) / BN;
@@ -285,11 +291,11 @@ xent_table_grad_kernel(Operand Pt, Operand Qt, uint32_t steps, Answers<typename 
         __syncthreads();
     }
     g.each([&](uint32_t r, uint32_t c, float v) {
-        if (m0 + r < Pt.rows && n0 + c < dim) out[(uint64_t)(m0 + r) * dim + n0 + c] = down<typename G::Elem::T>(v);
+        if (m0 + r < rows && n0 + c < dim) out[(uint64_t)(m0 + r) * dim + n0 + c] = down<typename G::Elem::T>(v);
     });
 }
 
-// partial sums of grad_queries: part s gets p [T][k of stretch s] . wt [dim][k]^T, added to what the earlier pieces left there
+// partial sums of grad_queries: part s gets p . wt^T over the steps of stretch s, added to what the earlier pieces left there
 template <class G>
 __global__ void __launch_bounds__(G::kThreads)
 xent_query_grad_kernel(Operand P, Operand Wt, uint32_t steps, uint32_t steps_per_part, int add, float *__restrict__ parts, uint32_t dim) {
@@ -300,7 +306,7 @@ xent_query_grad_kernel(Operand P, Operand Wt, uint32_t steps, uint32_t steps_per
     const uint32_t s0 = s * steps_per_part, s1 = min(steps, s0 + steps_per_part);
     float *out = parts + (uint64_t)s * P.rows * dim;
     G g;
-    if (s0 < s1) g.run(P, m0, Wt, n0, (uint64_t)s0 * 128, s1 - s0, lds);
+    if (s0 < s1) g.run(P, m0, Wt, n0, s0, s1 - s0, lds);
     else g.zero();
     g.each([&](uint32_t r, uint32_t c, float v) {
         if (m0 + r < P.rows && n0 + c < dim) {
@@ -342,10 +348,6 @@ xent_sum_parts_kernel(const float *__restrict__ parts, uint32_t n_parts, uint64_
 // ---- host side -------------------------------------------------------------------------------------------------------
 uint64_t up_to(uint64_t x, uint64_t m) { return (x + m - 1) / m * m; }
 
-// Row length of the matrices in scratch: rows a large power of two apart would all begin in the same few memory channels, and a step of the
-// matrix loop reads the same 128 bytes of 256 rows.
-uint64_t padded(uint64_t n, uint32_t es) { return n + 128 / es; }
-
 struct Shape {
     uint32_t T, V, dim;
     uint64_t ldq, ldw;
@@ -386,7 +388,7 @@ Plan make_plan(const Shape &s, bool grad, void *ws) {
     // the scratch asked for covers packed copies whether or not a call needs them: alignment is not known here
     Plan pl{};
     const uint64_t es = s.es(), kp = s.kp(), tp = s.tp();
-    const uint64_t budget = 128ull << 20;
+    const uint64_t budget = 256ull << 20;
     const uint64_t per_row = es * (grad ? std::max<uint64_t>(tp, kp) : kp);
     pl.piece = (uint32_t)std::min<uint64_t>(up_to(s.V, 256), std::max<uint64_t>(1024, budget / per_row / 1024 * 1024));
     cz::Carve c(ws);
@@ -400,10 +402,10 @@ Plan make_plan(const Shape &s, bool grad, void *ws) {
         pl.parts = std::max(1u, std::min(tiles, resident / qt));
         pl.stats = c.take<float2>((uint64_t)pl.parts * ((s.V + pl.piece - 1) / pl.piece) * s.T);
     } else {
-        pl.qt = c.take<uint8_t>(s.dim * padded(tp, es) * es);
-        pl.wt = c.take<uint8_t>((uint64_t)s.dim * padded(pl.piece, es) * es);
-        pl.p = c.take<uint8_t>((uint64_t)s.T * padded(pl.piece, es) * es);
-        pl.pt = c.take<uint8_t>(pl.piece * padded(tp, es) * es);
+        pl.qt = c.take<uint8_t>(s.dim * tp * es);
+        pl.wt = c.take<uint8_t>((uint64_t)s.dim * pl.piece * es);
+        pl.p = c.take<uint8_t>((uint64_t)s.T * pl.piece * es);
+        pl.pt = c.take<uint8_t>(pl.piece * tp * es);
         const uint32_t nv = std::min(s.V, pl.piece);
         pl.large_p = enough(nv, tp);
         pl.large_w = enough(nv, s.dim);
@@ -478,24 +480,23 @@ int forward(const Shape &s, const Plan &pl, const void *q_, const void *w_, cons
 }
 
 template <typename T>
-void transpose(const T *x, uint64_t ld, uint32_t n, uint32_t dim, const uint32_t *targets, uint32_t V, void *out, uint32_t width, uint64_t ldo,
-               hipStream_t stream) {
+void transpose(const T *x, uint64_t ld, uint32_t n, uint32_t dim, const uint32_t *targets, uint32_t V, void *out, uint32_t width, hipStream_t stream) {
     const bool wide = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && ld * sizeof(T) % 16 == 0;
     hipLaunchKernelGGL(xent_transpose_kernel<T>, dim3((width + 63) / 64, (dim + 63) / 64), dim3(256), 0, stream, x, ld, wide, n, dim, targets, V,
-                       (T *)out, width, ldo);
+                       (T *)out, width);
 }
 
 template <class G>
 int weights_of(const Operand &W, uint32_t v0, uint32_t V, const Operand &Q, uint32_t steps, float scale, const uint32_t *targets, const float *lse,
-               const float *grad_loss, void *p, uint32_t vp, uint64_t ldp, void *pt, uint32_t tp, uint64_t ldt, float *rest, hipStream_t stream) {
+               const float *grad_loss, void *p, uint32_t vp, void *pt, uint32_t tp, float *rest, hipStream_t stream) {
     typedef typename G::Elem::T T;
     return launch<G>(xent_weights_kernel<G>, tiles_of(vp, G::BM) * tiles_of(tp, G::BN), stream, W, v0, V, Q, steps, scale, targets, lse, grad_loss,
-                     (T *)p, ldp, (T *)pt, tp, ldt, rest);
+                     (T *)p, (T *)pt, vp, tp, rest);
 }
 template <class G>
 int table_grad_of(const Operand &Pt, const Operand &Qt, uint32_t steps, const Answers<typename G::Elem::T> &an, uint32_t v0,
-                  typename G::Elem::T *out, uint32_t dim, hipStream_t stream) {
-    return launch<G>(xent_table_grad_kernel<G>, tiles_of(Pt.rows, G::BM) * tiles_of(dim, G::BN), stream, Pt, Qt, steps, an, v0, out, dim);
+                  uint32_t rows, typename G::Elem::T *out, uint32_t dim, hipStream_t stream) {
+    return launch<G>(xent_table_grad_kernel<G>, tiles_of(rows, G::BM) * tiles_of(dim, G::BN), stream, Pt, Qt, steps, an, v0, rows, out, dim);
 }
 template <class G>
 int query_grad_of(const Operand &P, const Operand &Wt, uint32_t steps, uint32_t parts, bool add, float *dq, uint32_t dim, hipStream_t stream) {
@@ -515,12 +516,10 @@ int backward(const Shape &s, const Plan &pl, const void *q_, const void *w_, con
         Q = Operand{(const char *)pl.q, (uint64_t)kp * es, s.T};
     }
     const bool wd = direct(w, s.ldw, s.dim, es);
-    const uint64_t ldt = padded(tp, es);
     const Answers<T> an{targets, pl.rest, q, w, s.ldq, s.ldw, s.T, s.V};
-    if (dw) transpose(q, s.ldq, s.T, s.dim, targets, s.V, pl.qt, tp, ldt, stream);
+    if (dw) transpose(q, s.ldq, s.T, s.dim, targets, s.V, pl.qt, tp, stream);
     for (uint32_t v0 = 0; v0 < s.V; v0 += pl.piece) {
         const uint32_t nv = std::min(pl.piece, s.V - v0), vp = (uint32_t)up_to(nv, 256);
-        const uint64_t ldp = padded(vp, es);
         const T *wv = w + v0 * s.ldw;
         Operand W{(const char *)wv, s.ldw * es, nv};
         if (!wd) {
@@ -528,19 +527,19 @@ int backward(const Shape &s, const Plan &pl, const void *q_, const void *w_, con
             W = Operand{(const char *)pl.w, (uint64_t)kp * es, nv};
         }
         void *p = dq ? pl.p : nullptr, *pt = dw ? pl.pt : nullptr;
-        int rc = pl.large_p ? weights_of<Large<E>>(W, v0, s.V, Q, steps, scale, targets, lse, grad_loss, p, vp, ldp, pt, tp, ldt, pl.rest, stream)
-                            : weights_of<Small<E>>(W, v0, s.V, Q, steps, scale, targets, lse, grad_loss, p, vp, ldp, pt, tp, ldt, pl.rest, stream);
+        int rc = pl.large_p ? weights_of<Large<E>>(W, v0, s.V, Q, steps, scale, targets, lse, grad_loss, p, vp, pt, tp, pl.rest, stream)
+                            : weights_of<Small<E>>(W, v0, s.V, Q, steps, scale, targets, lse, grad_loss, p, vp, pt, tp, pl.rest, stream);
         if (rc) return rc;
         if (dw) {
-            const Operand Pt{(const char *)pl.pt, ldt * es, nv}, Qt{(const char *)pl.qt, ldt * es, s.dim};
+            const Operand Pt = gemm::panels(pl.pt, vp), Qt = gemm::panels(pl.qt, s.dim);
             T *out = (T *)dw + (uint64_t)v0 * s.dim;
-            rc = pl.large_w ? table_grad_of<Large<E>>(Pt, Qt, tp / s.kstep(), an, v0, out, s.dim, stream)
-                            : table_grad_of<Small<E>>(Pt, Qt, tp / s.kstep(), an, v0, out, s.dim, stream);
+            rc = pl.large_w ? table_grad_of<Large<E>>(Pt, Qt, tp / s.kstep(), an, v0, nv, out, s.dim, stream)
+                            : table_grad_of<Small<E>>(Pt, Qt, tp / s.kstep(), an, v0, nv, out, s.dim, stream);
             if (rc) return rc;
         }
         if (dq) {
-            transpose(wv, s.ldw, nv, s.dim, (const uint32_t *)nullptr, 0u, pl.wt, vp, ldp, stream);
-            const Operand P{(const char *)pl.p, ldp * es, s.T}, Wt{(const char *)pl.wt, ldp * es, s.dim};
+            transpose(wv, s.ldw, nv, s.dim, (const uint32_t *)nullptr, 0u, pl.wt, vp, stream);
+            const Operand P = gemm::panels(pl.p, s.T), Wt = gemm::panels(pl.wt, s.dim);
             rc = pl.large_q ? query_grad_of<Large<E>>(P, Wt, vp / s.kstep(), pl.parts, v0 != 0, pl.dq, s.dim, stream)
                             : query_grad_of<Small<E>>(P, Wt, vp / s.kstep(), pl.parts, v0 != 0, pl.dq, s.dim, stream);
             if (rc) return rc;
