@@ -1,5 +1,5 @@
-// gemm_nt.h -- the matrix-core loop that the dense operators share:  C[m][n] = sum_k A[m][k] * B[n][k],  both operands with k
-// contiguous.  A workgroup owns a BM x BN tile; what happens to the accumulators is the caller's epilogue.
+// gemm_nt.h -- the matrix-core loop that the dense operators share:  C[m][n] = sum_k A[m][k] * B[n][k],  operands with k contiguous
+// or (16-bit types) with rows contiguous.  A workgroup owns a BM x BN tile; what happens to the accumulators is the caller's epilogue.
 //
 // * k goes in steps of 128 bytes per row (64 bf16 / 32 f32): a step of A and B goes straight from memory into LDS (16 bytes a lane, no
 //   registers in between), two steps are kept, the next one is on its way while the matrix cores work on this one.
@@ -8,6 +8,9 @@
 // * operand layout of the 32 x 32 matrix instructions: lane l holds row l % 32 and the k that belong to half l / 32; as both
 //   operands are read alike, which k those are does not matter: a half is a 16-byte piece (8 bf16 = one 32x32x16 instruction, 4 f32 =
 //   four 32x32x2 ones).
+// * a turned operand lies in LDS as it does in memory, k by k: a k's rows in pieces of 16 bytes (8 rows), piece p at place p ^ 4 (k & 3).  The
+//   transposing read gives 16 lanes of 8 bytes (4 rows) at 4 k's back as 16 rows at 4 k's; 32 lanes read 64 bytes at each of 4 k's, each
+//   in a quarter of the banks of its own.
 // * accumulators: register r of lane l is C[8 (r / 4) + 4 (l / 32) + r % 4][l % 32] of its 32 x 32 tile.
 #pragma once
 #include <hip/hip_runtime.h>
@@ -66,7 +69,74 @@ struct Operand {
 };
 // k in panels: a step's 128 bytes of every row lie one behind the other, so that a workgroup's step is one run of memory (rows that are 128 KB
 // long put each row of a step into a page of its own: grad_queries of a 65536-row piece took 169 us instead of XXX)
+// the same for an operand of a 16-bit type that lies turned: for each k the rows one behind the other
+struct Turned {
+    const char *base;
+    uint64_t ld;            // bytes from a k to the next
+    uint64_t panel;         // bytes from 64 rows to the next 64: 128 where a k's rows are one run
+    uint32_t rows, ks;      // rows: a multiple of 8, 16-byte aligned; a k past the last one is read as the last one (times zeros of the other side)
+};
 inline Operand panels(const void *base, uint32_t rows) { return Operand{(const char *)base, 128, rows, (uint64_t)rows * 128}; }
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// a workgroup's copies of ROWS rows of an operand into LDS, a step at a time
+template <class O, int ROWS, int THREADS>
+struct Copies;
+template <int ROWS, int THREADS>
+struct Copies<Operand, ROWS, THREADS> {
+    static constexpr int N = ROWS * 8 / THREADS;  // 16-byte pieces of a thread
+    static constexpr int kReads = 1;               // LDS reads of a fragment
+    static_assert(N * THREADS == ROWS * 8, "threads cover the copies");
+    const char *src[N];
+    uint64_t stride;
+    __device__ __forceinline__ Copies(const Operand &o, uint32_t row0) : stride(o.step) {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const uint32_t c = i * THREADS + threadIdx.x, row = c >> 3, piece = (c & 7) ^ ((row >> 1) & 7);
+            src[i] = o.base + (uint64_t)min(row0 + row, o.rows - 1) * o.ld + piece * 16;
+        }
+    }
+    __device__ __forceinline__ const char *from(int i, uint32_t step) const { return src[i] + step * stride; }
+    // rows row0 + 32 i + lane % 32 at the 16 k's `kk` of a step
+    static __device__ __forceinline__ u32x4 fragment(const char *lds, int row0, int i, int kk) {
+        const int lane = threadIdx.x & 63, l32 = lane & 31;
+        return *(const u32x4 *)(lds + (row0 + l32) * 128 + (((2 * kk + (lane >> 5)) ^ ((l32 >> 1) & 7)) * 16) + i * 32 * 128);
+    }
+};
+template <int ROWS, int THREADS>
+struct Copies<Turned, ROWS, THREADS> {
+    static constexpr int N = ROWS * 8 / THREADS, P = ROWS / 8;  // pieces of a thread, of a k
+    static constexpr int kReads = 2;
+    static_assert(N * THREADS == ROWS * 8, "threads cover the copies");
+    const char *src[N];
+    uint64_t ld;
+    uint32_t ks;
+    __device__ __forceinline__ Copies(const Turned &o, uint32_t row0) : ld(o.ld), ks(o.ks) {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const uint32_t c = i * THREADS + threadIdx.x, k = c / P, piece = (c % P) ^ (4 * (k & 3));
+            const uint32_t row = min(row0 + piece * 8, o.rows - 8);
+            src[i] = o.base + (row >> 6) * o.panel + (row & 63) * 2;
+        }
+    }
+    __device__ __forceinline__ const char *from(int i, uint32_t step) const {
+        const uint32_t k = step * 64 + (i * THREADS + threadIdx.x) / P;
+        return src[i] + min(k, ks - 1) * ld;
+    }
+    static __device__ __forceinline__ u32x4 fragment(const char *lds, int row0, int i, int kk) {
+        const int lane = threadIdx.x & 63, l16 = lane & 15;
+        const int k = 16 * kk + 8 * (lane >> 5) + (l16 >> 2), col = row0 + i * 32 + 16 * ((lane >> 4) & 1) + 4 * (l16 & 3);
+        const int at = ((col >> 3) ^ (4 * (l16 >> 2))) * 16 + (col & 7) * 2;
+        typedef __attribute__((address_space(3))) s16x4 *Lds;
+        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(lds + k * P * 16 + at)),
+                    b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(lds + (k + 4) * P * 16 + at));
+        struct {
+            s16x4 a, b;
+        } both = {a, b};
+        return __builtin_bit_cast(u32x4, both);
+    }
+};
 
 // BM x BN by WM x WN waves.  Measured with 1024 rows of B, 1M rows of A, k = 768, bf16: 128 x 128 by 2 x 2 900 TFLOP/s (32 bytes of copies
 // a clock and CU; its matrix cores are busy 45 % of the time), 256 x 256 by 2 x 4 1185 (52 %; a library's 8192^3 product: 1537).  Zeros for
@@ -80,9 +150,7 @@ struct Tile {
     static constexpr int MT = BM / WM / 32, NT = BN / WN / 32;
     static constexpr int kBytes = (BM + BN) * 128;  // LDS of one step
     static constexpr int kLds = 2 * kBytes;
-    static constexpr int NA = BM * 8 / kThreads, NB = BN * 8 / kThreads;  // 16-byte pieces a thread copies per step
     static_assert(MT * WM * 32 == BM && NT * WN * 32 == BN, "waves cover the tile");
-    static_assert(NA * kThreads == BM * 8 && NB * kThreads == BN * 8, "threads cover the copies");
 
     f32x16 acc[MT][NT];
 
@@ -94,21 +162,14 @@ struct Tile {
 #pragma unroll
                 for (int r = 0; r < 16; r++) acc[i][j][r] = 0.f;
     }
-    // where this thread's pieces of a tile that starts at row0 come from (k = 0)
-    template <int N>
-    static __device__ __forceinline__ void rows_of(const Operand &o, uint32_t row0, const char *(&src)[N]) {
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            const uint32_t c = i * kThreads + threadIdx.x, row = c >> 3, piece = (c & 7) ^ ((row >> 1) & 7);
-            src[i] = o.base + (uint64_t)min(row0 + row, o.rows - 1) * o.ld + piece * 16;
-        }
-    }
-    template <int N>
-    static __device__ __forceinline__ void copy(const char *(&src)[N], uint64_t k, char *lds) {
+    typedef Copies<Operand, BM, kThreads> CopiesA;
+    typedef Copies<Operand, BN, kThreads> CopiesB;
+    template <class C>
+    static __device__ __forceinline__ void copy(const C &c, uint32_t step, char *lds) {
         const uint32_t wave = threadIdx.x >> 6;
 #pragma unroll
-        for (int i = 0; i < N; i++)
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(src[i] + k),
+        for (int i = 0; i < C::N; i++)
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)c.from(i, step),
                                              (__attribute__((address_space(3))) void *)(lds + (i * kThreads + wave * 64) * 16), 16, 0, 0);
     }
     // the copies this wave has in flight are in LDS, and every wave is here
@@ -119,52 +180,54 @@ struct Tile {
     static __device__ __forceinline__ int wave_row() { return (int)(threadIdx.x >> 6) / WN * (BM / WM); }
     static __device__ __forceinline__ int wave_col() { return (int)(threadIdx.x >> 6) % WN * (BN / WN); }
 
-    __device__ __forceinline__ void fragments(const char *lds, int kk, u32x4 (&a)[MT], u32x4 (&b)[NT]) const {
-        const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
-        const char *la = lds + (wave_row() + l32) * 128, *lb = lds + BM * 128 + (wave_col() + l32) * 128;
-        const int at = ((2 * kk + half) ^ ((l32 >> 1) & 7)) * 16;
+    template <class CA, class CB>
+    static __device__ __forceinline__ void fragments(const char *lds, int kk, u32x4 (&a)[MT], u32x4 (&b)[NT]) {
 #pragma unroll
-        for (int j = 0; j < NT; j++) b[j] = *(const u32x4 *)(lb + j * 32 * 128 + at);
+        for (int j = 0; j < NT; j++) b[j] = CB::fragment(lds + BM * 128, wave_col(), j, kk);
 #pragma unroll
-        for (int i = 0; i < MT; i++) a[i] = *(const u32x4 *)(la + i * 32 * 128 + at);
+        for (int i = 0; i < MT; i++) a[i] = CA::fragment(lds, wave_row(), i, kk);
     }
+    template <class CA = CopiesA, class CB = CopiesB>
     __device__ __forceinline__ void step(const char *lds) {
         u32x4 a[2][MT], b[2][NT];
-        fragments(lds, 0, a[0], b[0]);
+        fragments<CA, CB>(lds, 0, a[0], b[0]);
 #pragma unroll
         for (int kk = 0; kk < 4; kk++) {
-            if (kk < 3) fragments(lds, kk + 1, a[(kk + 1) & 1], b[(kk + 1) & 1]);
+            if (kk < 3) fragments<CA, CB>(lds, kk + 1, a[(kk + 1) & 1], b[(kk + 1) & 1]);
 #pragma unroll
             for (int i = 0; i < MT; i++)
 #pragma unroll
                 for (int j = 0; j < NT; j++) mma(E{}, a[kk & 1][i], b[kk & 1][j], acc[i][j]);
         }
-        // the next fragments are read between this fragment's matrix instructions, one to one
-        __builtin_amdgcn_sched_group_barrier(0x100, MT + NT, 0);
+        // the next fragments are read between this fragment's matrix instructions
+        constexpr int R = MT * CA::kReads + NT * CB::kReads, X = MT * NT, PER = (R + X - 1) / X;
+        __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
 #pragma unroll
         for (int kk = 0; kk < 4; kk++)
 #pragma unroll
-            for (int x = 0; x < MT * NT; x++) {
-                if (kk < 3 && x < MT + NT) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            for (int x = 0; x < X; x++) {
+                if (kk < 3 && x * PER < R) __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
                 __builtin_amdgcn_sched_group_barrier(0x008, E::kPerPiece, 0);
             }
     }
     // one tile: A rows from m0, B rows from n0, `steps` >= 1 steps from step s0 on
-    __device__ __forceinline__ void run(const Operand &A, uint32_t m0, const Operand &B, uint32_t n0, uint32_t s0, uint32_t steps, char *lds) {
-        const char *sa[NA], *sb[NB];
-        rows_of(A, m0, sa);
-        rows_of(B, n0, sb);
+    template <class OA, class OB>
+    __device__ __forceinline__ void run(const OA &A, uint32_t m0, const OB &B, uint32_t n0, uint32_t s0, uint32_t steps, char *lds) {
+        typedef Copies<OA, BM, kThreads> CA;
+        typedef Copies<OB, BN, kThreads> CB;
+        const CA ca(A, m0);
+        const CB cb(B, n0);
         zero();
-        copy(sa, s0 * A.step, lds);
-        copy(sb, s0 * B.step, lds + BM * 128);
+        copy(ca, s0, lds);
+        copy(cb, s0, lds + BM * 128);
         for (uint32_t s = 0; s < steps; s++) {
             char *cur = lds + (s & 1) * kBytes, *nxt = lds + (~s & 1) * kBytes;
             arrived();
             if (s + 1 < steps) {
-                copy(sa, (s0 + s + 1) * A.step, nxt);
-                copy(sb, (s0 + s + 1) * B.step, nxt + BM * 128);
+                copy(ca, s0 + s + 1, nxt);
+                copy(cb, s0 + s + 1, nxt + BM * 128);
             }
-            step(cur);
+            step<CA, CB>(cur);
         }
     }
     // f(row, col, value) over this thread's accumulators, rows and columns within the tile

@@ -528,8 +528,7 @@ q4_scores_kernel(Rows t, gemm::Operand Q, const int *__restrict__ exponent, uint
         qn[j] = near.qnorm[b];
         qe[j] = exponent[b];
     }
-    const char *src[G::NB];
-    G::rows_of(Q, n0, src);
+    const typename G::CopiesB src(Q, n0);
 #pragma unroll 1
     for (uint32_t blk = k0; blk < k1; blk++) {
         const uint64_t r = (uint64_t)blk * BM + mine, safe = min(r, (uint64_t)t.n - 1);
@@ -593,11 +592,11 @@ q4_scores_kernel(Rows t, gemm::Operand Q, const int *__restrict__ exponent, uint
             if (s + 1 < steps) {
                 if (early) store(nxt);
                 asm volatile("" ::: "memory");  // (in this order: the wait above counts on it)
-                G::copy(src, (uint64_t)(s + 1) * 128, nxt + BM * 128);
+                G::copy(src, s + 1, nxt + BM * 128);
                 asm volatile("" ::: "memory");
                 if (early && s + 2 < steps) load(s + 2);
             }
-            g.step(cur);
+            g.template step<>(cur);
             if (!early && s + 1 < steps) {
                 store(nxt);
                 if (s + 2 < steps) load(s + 2);

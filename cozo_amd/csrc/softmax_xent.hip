@@ -3,8 +3,8 @@
 // Forward: one matrix product per (table tile, query tile) with the softmax's running maximum and sum as its epilogue.  The TABLE rows are
 // the product's m and the queries its n: a lane's accumulators then belong to one query, so maximum and sum run in the lane and lanes are
 // joined once, at the end of a workgroup's stretch of the table.  Stretches are joined in a second launch.
-// Gradient, a piece of the table at a time:  P = grad_loss scale (softmax - onehot) of the piece is computed again and stored in both
-// orders, then  dW = P^T Q  is written and  dq += P W  goes to per-stretch partial sums (each added to by one workgroup only, in
+// Gradient, a piece of the table at a time:  P = grad_loss scale (softmax - onehot) of the piece is computed again and stored (in f32 in both
+// orders, in bf16 once: the matrix loop then reads P, Q and W turned where k is not what is contiguous), then  dW = P^T Q  is written and  dq += P W  goes to per-stretch partial sums (each added to by one workgroup only, in
 // a fixed order: no atomics).  A bf16 P loses what it rounds off; where that matters most, at the answers -- the largest entries, which may well
 // carry all the same value and so the same error -- the rest is kept in f32 and its term added to dW's row and to dq in f32.
 #include <algorithm>
@@ -16,6 +16,7 @@
 using gemm::Bf16;
 using gemm::F32;
 using gemm::Operand;
+using gemm::Turned;
 
 namespace {
 
@@ -38,14 +39,16 @@ __device__ __forceinline__ uint64_t in_panels(uint32_t row, uint32_t k, uint32_t
     return ((uint64_t)(k / W) * rows + row) * W + k % W;
 }
 
-// rows [r0, r0 + n) of x, their first dim elements and zeros up to ldo, one 16-byte aligned row behind the other
+// rows of x, their first dim elements and zeros up to ldo, one 16-byte aligned row behind the other, and rows of zeros up to `rows`; with targets
+// given also for those whose target is no row of the table (as in xent_transpose_kernel)
 template <typename T>
 __global__ void __launch_bounds__(256)
-xent_pack_kernel(const T *__restrict__ x, uint64_t ld, uint32_t n, uint32_t dim, T *__restrict__ out, uint32_t ldo) {
-    const uint64_t total = (uint64_t)n * ldo;
+xent_pack_kernel(const T *__restrict__ x, uint64_t ld, uint32_t n, uint32_t dim, T *__restrict__ out, uint32_t ldo, uint32_t rows,
+                 const uint32_t *__restrict__ targets, uint32_t V) {
+    const uint64_t total = (uint64_t)rows * ldo;
     for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (uint64_t)gridDim.x * 256) {
         const uint32_t r = (uint32_t)(i / ldo), c = (uint32_t)(i - (uint64_t)r * ldo);
-        out[i] = c < dim ? x[r * ld + c] : (T)0.f;
+        out[i] = c < dim && r < n && (!targets || has_answer(targets[r], V)) ? x[r * ld + c] : (T)0.f;
     }
 }
 
@@ -222,9 +225,9 @@ xent_weights_kernel(Operand W, uint32_t v0, uint32_t V, Operand Q, uint32_t step
                     o[r] = down<typename E::T>(x);
                     if (hit && rest) rest[t] = x - up(o[r]);
                 }
-                if (t < Q.rows && p) {
+                if (t < tp && p) {
                     typedef typename E::T T4 __attribute__((ext_vector_type(4)));
-                    *(T4 *)(p + in_panels<typename E::T>(t, v, Q.rows)) = T4{o[0], o[1], o[2], o[3]};
+                    *(T4 *)(p + in_panels<typename E::T>(t, v, tp)) = T4{o[0], o[1], o[2], o[3]};
                 }
                 if (t < tp && pt)
 #pragma unroll
@@ -244,9 +247,9 @@ struct Answers {
 };
 
 // grad_table rows of a piece (rows v0 ... of the table): pt . qt^T, and the rest for the queries that the rows answer
-template <class G>
+template <class G, class O>
 __global__ void __launch_bounds__(G::kThreads)
-xent_table_grad_kernel(Operand Pt, Operand Qt, uint32_t steps, Answers<typename G::Elem::T> an, uint32_t v0, uint32_t rows,
+xent_table_grad_kernel(O Pt, O Qt, uint32_t steps, Answers<typename G::Elem::T> an, uint32_t v0, uint32_t rows,
                        typename G::Elem::T *__restrict__ out, uint32_t dim) {
     constexpr int BM = G::BM, BN = G::BN, kWaves = G::kThreads / 64;
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -296,20 +299,20 @@ xent_table_grad_kernel(Operand Pt, Operand Qt, uint32_t steps, Answers<typename 
 }
 
 // partial sums of grad_queries: part s gets p . wt^T over the steps of stretch s, added to what the earlier pieces left there
-template <class G>
+template <class G, class O>
 __global__ void __launch_bounds__(G::kThreads)
-xent_query_grad_kernel(Operand P, Operand Wt, uint32_t steps, uint32_t steps_per_part, int add, float *__restrict__ parts, uint32_t dim) {
+xent_query_grad_kernel(Operand P, O Wt, uint32_t T, uint32_t steps, uint32_t steps_per_part, int add, float *__restrict__ parts, uint32_t dim) {
     constexpr int BM = G::BM, BN = G::BN;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    const uint32_t nt = (dim + BN - 1) / BN, mt = (P.rows + BM - 1) / BM;
+    const uint32_t nt = (dim + BN - 1) / BN, mt = (T + BM - 1) / BM;
     const uint32_t at = gemm::place_in_order(), n0 = at % nt * BN, m0 = at / nt % mt * BM, s = at / (nt * mt);
     const uint32_t s0 = s * steps_per_part, s1 = min(steps, s0 + steps_per_part);
-    float *out = parts + (uint64_t)s * P.rows * dim;
+    float *out = parts + (uint64_t)s * T * dim;
     G g;
     if (s0 < s1) g.run(P, m0, Wt, n0, s0, s1 - s0, lds);
     else g.zero();
     g.each([&](uint32_t r, uint32_t c, float v) {
-        if (m0 + r < P.rows && n0 + c < dim) {
+        if (m0 + r < T && n0 + c < dim) {
             float *o = out + (uint64_t)(m0 + r) * dim + n0 + c;
             *o = add ? *o + v : v;
         }
@@ -364,7 +367,7 @@ struct Plan {
     int fwd;               // forward's tile: 0 narrow, 1 small, 2 large
     bool large_p, large_w, large_q;  // backward's tiles: of P, of grad_table, of grad_queries
     void *q, *w;           // packed copies (unaligned rows or a dim that is no multiple of a step)
-    void *qt, *wt, *p, *pt;
+    void *qt, *wt, *p, *pt;  // (bf16: qt is a copy of the queries without those that have no answer, wt and pt are not needed)
     float2 *stats;
     float *dq, *rest;
     size_t bytes;
@@ -402,10 +405,12 @@ Plan make_plan(const Shape &s, bool grad, void *ws) {
         pl.parts = std::max(1u, std::min(tiles, resident / qt));
         pl.stats = c.take<float2>((uint64_t)pl.parts * ((s.V + pl.piece - 1) / pl.piece) * s.T);
     } else {
-        pl.qt = c.take<uint8_t>(s.dim * tp * es);
-        pl.wt = c.take<uint8_t>((uint64_t)s.dim * pl.piece * es);
-        pl.p = c.take<uint8_t>((uint64_t)s.T * pl.piece * es);
-        pl.pt = c.take<uint8_t>(pl.piece * tp * es);
+        pl.qt = c.take<uint8_t>(kp * tp * es);
+        pl.p = c.take<uint8_t>(tp * pl.piece * es);
+        if (!s.bf16) {
+            pl.wt = c.take<uint8_t>((uint64_t)s.dim * pl.piece * es);
+            pl.pt = c.take<uint8_t>(pl.piece * tp * es);
+        }
         const uint32_t nv = std::min(s.V, pl.piece);
         pl.large_p = enough(nv, tp);
         pl.large_w = enough(nv, s.dim);
@@ -428,8 +433,10 @@ int launched(const char *what) {
 uint32_t grid_of(uint64_t items) { return (uint32_t)std::min<uint64_t>((items + 255) / 256, 1u << 16); }
 
 template <typename T>
-void pack(const T *x, uint64_t ld, uint32_t n, uint32_t dim, void *out, uint32_t ldo, hipStream_t stream) {
-    hipLaunchKernelGGL(xent_pack_kernel<T>, dim3(grid_of((uint64_t)n * ldo)), dim3(256), 0, stream, x, ld, n, dim, (T *)out, ldo);
+void pack(const T *x, uint64_t ld, uint32_t n, uint32_t dim, void *out, uint32_t ldo, hipStream_t stream, uint32_t rows = 0,
+          const uint32_t *targets = nullptr, uint32_t V = 0) {
+    rows = std::max(n, rows);
+    hipLaunchKernelGGL(xent_pack_kernel<T>, dim3(grid_of((uint64_t)rows * ldo)), dim3(256), 0, stream, x, ld, n, dim, (T *)out, ldo, rows, targets, V);
 }
 
 // a kernel over tiles G, with the LDS that they ask for
@@ -493,14 +500,14 @@ int weights_of(const Operand &W, uint32_t v0, uint32_t V, const Operand &Q, uint
     return launch<G>(xent_weights_kernel<G>, tiles_of(vp, G::BM) * tiles_of(tp, G::BN), stream, W, v0, V, Q, steps, scale, targets, lse, grad_loss,
                      (T *)p, (T *)pt, vp, tp, rest);
 }
-template <class G>
-int table_grad_of(const Operand &Pt, const Operand &Qt, uint32_t steps, const Answers<typename G::Elem::T> &an, uint32_t v0,
+template <class G, class O>
+int table_grad_of(const O &Pt, const O &Qt, uint32_t steps, const Answers<typename G::Elem::T> &an, uint32_t v0,
                   uint32_t rows, typename G::Elem::T *out, uint32_t dim, hipStream_t stream) {
-    return launch<G>(xent_table_grad_kernel<G>, tiles_of(rows, G::BM) * tiles_of(dim, G::BN), stream, Pt, Qt, steps, an, v0, rows, out, dim);
+    return launch<G>(xent_table_grad_kernel<G, O>, tiles_of(rows, G::BM) * tiles_of(dim, G::BN), stream, Pt, Qt, steps, an, v0, rows, out, dim);
 }
-template <class G>
-int query_grad_of(const Operand &P, const Operand &Wt, uint32_t steps, uint32_t parts, bool add, float *dq, uint32_t dim, hipStream_t stream) {
-    return launch<G>(xent_query_grad_kernel<G>, tiles_of(P.rows, G::BM) * tiles_of(dim, G::BN) * parts, stream, P, Wt, steps,
+template <class G, class O>
+int query_grad_of(const Operand &P, const O &Wt, uint32_t T, uint32_t steps, uint32_t parts, bool add, float *dq, uint32_t dim, hipStream_t stream) {
+    return launch<G>(xent_query_grad_kernel<G, O>, tiles_of(T, G::BM) * tiles_of(dim, G::BN) * parts, stream, P, Wt, T, steps,
                      (steps + parts - 1) / parts, add ? 1 : 0, dq, dim);
 }
 
@@ -517,7 +524,11 @@ int backward(const Shape &s, const Plan &pl, const void *q_, const void *w_, con
     }
     const bool wd = direct(w, s.ldw, s.dim, es);
     const Answers<T> an{targets, pl.rest, q, w, s.ldq, s.ldw, s.T, s.V};
-    if (dw) transpose(q, s.ldq, s.T, s.dim, targets, s.V, pl.qt, tp, stream);
+    constexpr bool kTurned = sizeof(T) == 2;  // (there is no transposing read for f32)
+    if (dw) {
+        if (kTurned) pack(q, s.ldq, s.T, s.dim, pl.qt, kp, stream, tp, targets, s.V);
+        else transpose(q, s.ldq, s.T, s.dim, targets, s.V, pl.qt, tp, stream);
+    }
     for (uint32_t v0 = 0; v0 < s.V; v0 += pl.piece) {
         const uint32_t nv = std::min(pl.piece, s.V - v0), vp = (uint32_t)up_to(nv, 256);
         const T *wv = w + v0 * s.ldw;
@@ -526,22 +537,33 @@ int backward(const Shape &s, const Plan &pl, const void *q_, const void *w_, con
             pack(wv, s.ldw, nv, s.dim, pl.w, kp, stream);
             W = Operand{(const char *)pl.w, (uint64_t)kp * es, nv};
         }
-        void *p = dq ? pl.p : nullptr, *pt = dw ? pl.pt : nullptr;
+        void *p = dq || kTurned ? pl.p : nullptr, *pt = dw && !kTurned ? pl.pt : nullptr;
         int rc = pl.large_p ? weights_of<Large<E>>(W, v0, s.V, Q, steps, scale, targets, lse, grad_loss, p, vp, pt, tp, pl.rest, stream)
                             : weights_of<Small<E>>(W, v0, s.V, Q, steps, scale, targets, lse, grad_loss, p, vp, pt, tp, pl.rest, stream);
         if (rc) return rc;
-        if (dw) {
-            const Operand Pt = gemm::panels(pl.pt, vp), Qt = gemm::panels(pl.qt, s.dim);
-            T *out = (T *)dw + (uint64_t)v0 * s.dim;
-            rc = pl.large_w ? table_grad_of<Large<E>>(Pt, Qt, tp / s.kstep(), an, v0, nv, out, s.dim, stream)
-                            : table_grad_of<Small<E>>(Pt, Qt, tp / s.kstep(), an, v0, nv, out, s.dim, stream);
+        const uint32_t vsteps = vp / s.kstep();
+        if (dq) {
+            const Operand P = gemm::panels(pl.p, tp);
+            auto query_grad = [&](const auto &Wt) {
+                return pl.large_q ? query_grad_of<Large<E>>(P, Wt, s.T, vsteps, pl.parts, v0 != 0, pl.dq, s.dim, stream)
+                                  : query_grad_of<Small<E>>(P, Wt, s.T, vsteps, pl.parts, v0 != 0, pl.dq, s.dim, stream);
+            };
+            if constexpr (kTurned) {
+                rc = query_grad(Turned{W.base, W.ld, 128, kp, nv});
+            } else {
+                transpose(wv, s.ldw, nv, s.dim, (const uint32_t *)nullptr, 0u, pl.wt, vp, stream);
+                rc = query_grad(gemm::panels(pl.wt, s.dim));
+            }
             if (rc) return rc;
         }
-        if (dq) {
-            transpose(wv, s.ldw, nv, s.dim, (const uint32_t *)nullptr, 0u, pl.wt, vp, stream);
-            const Operand P = gemm::panels(pl.p, s.T), Wt = gemm::panels(pl.wt, s.dim);
-            rc = pl.large_q ? query_grad_of<Large<E>>(P, Wt, vp / s.kstep(), pl.parts, v0 != 0, pl.dq, s.dim, stream)
-                            : query_grad_of<Small<E>>(P, Wt, vp / s.kstep(), pl.parts, v0 != 0, pl.dq, s.dim, stream);
+        if (dw) {
+            T *out = (T *)dw + (uint64_t)v0 * s.dim;
+            auto table_grad = [&](const auto &Pt, const auto &Qt) {
+                return pl.large_w ? table_grad_of<Large<E>>(Pt, Qt, tp / s.kstep(), an, v0, nv, out, s.dim, stream)
+                                  : table_grad_of<Small<E>>(Pt, Qt, tp / s.kstep(), an, v0, nv, out, s.dim, stream);
+            };
+            if constexpr (kTurned) rc = table_grad(Turned{(const char *)pl.p, 128, tp * 128ull, vp, tp}, Turned{(const char *)pl.qt, (uint64_t)kp * es, 128, kp, tp});
+            else rc = table_grad(gemm::panels(pl.pt, vp), gemm::panels(pl.qt, s.dim));
             if (rc) return rc;
         }
     }
