@@ -75,63 +75,65 @@ __global__ void __launch_bounds__(256)
 q4_quantize_kernel(const E *__restrict__ x, uint64_t ld, bool wide, Rows t, uint8_t *__restrict__ codes, uint16_t *__restrict__ scales,
                    float *__restrict__ sqnorms) {
     const int sub = threadIdx.x % LPR;
-    const uint64_t r = (uint64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
     const int glanes = 1 << (t.gshift - 3);
-    const bool live = r < t.n;
-    double sq = 0.0;
-    bool some = false;
-    for (uint32_t c0 = 0; c0 < t.chunks; c0 += LPR) {  // (uniform: the lanes of a group are active together)
-        const uint32_t c = c0 + sub;
-        const bool on = live && c < t.chunks;
-        float v[8];
+    for (uint64_t r0 = (uint64_t)blockIdx.x * (256 / LPR); r0 < t.n; r0 += (uint64_t)gridDim.x * (256 / LPR)) {
+        const uint64_t r = r0 + threadIdx.x / LPR;
+        const bool live = r < t.n;
+        double sq = 0.0;
+        bool some = false;
+        for (uint32_t c0 = 0; c0 < t.chunks; c0 += LPR) {  // (uniform: the lanes of a group are active together)
+            const uint32_t c = c0 + sub;
+            const bool on = live && c < t.chunks;
+            float v[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = 0.f;
-        if (on) load8(x + r * ld, c * 8, t.dim, wide, v);
-        float m = 0.f;
-        bool bad = false;
+            for (int j = 0; j < 8; j++) v[j] = 0.f;
+            if (on) load8(x + r * ld, c * 8, t.dim, wide, v);
+            float m = 0.f;
+            bool bad = false;
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            m = fmaxf(m, fabsf(v[j]));
-            bad |= !(fabsf(v[j]) < __builtin_inff());
-        }
-        if (bad) m = __builtin_inff();
-        for (int o = 1; o < glanes; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-        uint16_t sb = 0;
-        float inv = 0.f;
-        if (m == __builtin_inff()) {
-            sb = 0x7FC0;  // NaN: the group stands for nothing
-        } else if (m >= 0x1p-60f) {
-            sb = f32_to_bf16(__fdiv_rn(m, 7.0f));
-            inv = __fdiv_rn(1.0f, bf16_to_f32(sb));
-        }
-        uint32_t w = 0;
-        int cc = 0;
+            for (int j = 0; j < 8; j++) {
+                m = fmaxf(m, fabsf(v[j]));
+                bad |= !(fabsf(v[j]) < __builtin_inff());
+            }
+            if (bad) m = __builtin_inff();
+            for (int o = 1; o < glanes; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+            uint16_t sb = 0;
+            float inv = 0.f;
+            if (m == __builtin_inff()) {
+                sb = 0x7FC0;  // NaN: the group stands for nothing
+            } else if (m >= 0x1p-60f) {
+                sb = f32_to_bf16(__fdiv_rn(m, 7.0f));
+                inv = __fdiv_rn(1.0f, bf16_to_f32(sb));
+            }
+            uint32_t w = 0;
+            int cc = 0;
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            float q = rintf(v[j] * inv);
-            q = fminf(fmaxf(q, -7.f), 7.f);
-            const int k = m == __builtin_inff() ? 0 : (int)q;
-            cc += k * k;
-            w |= (uint32_t)(k & 15) << (4 * j);
+            for (int j = 0; j < 8; j++) {
+                float q = rintf(v[j] * inv);
+                q = fminf(fmaxf(q, -7.f), 7.f);
+                const int k = m == __builtin_inff() ? 0 : (int)q;
+                cc += k * k;
+                w |= (uint32_t)(k & 15) << (4 * j);
+            }
+            const double s = (double)bf16_to_f32(sb);
+            if (m == __builtin_inff()) sq += (double)__builtin_nanf("");
+            else sq += (double)cc * (s * s);
+            some |= cc != 0;
+            if (on) {
+                *(uint32_t *)(codes + (r * t.chunks + c) * 4) = w;
+                if ((c & (glanes - 1)) == 0) scales[r * t.groups + (c >> (t.gshift - 3))] = sb;
+            }
         }
-        const double s = (double)bf16_to_f32(sb);
-        if (m == __builtin_inff()) sq += (double)__builtin_nanf("");
-        else sq += (double)cc * (s * s);
-        some |= cc != 0;
-        if (on) {
-            *(uint32_t *)(codes + (r * t.chunks + c) * 4) = w;
-            if ((c & (glanes - 1)) == 0) scales[r * t.groups + (c >> (t.gshift - 3))] = sb;
-        }
-    }
 #pragma unroll
-    for (int o = 1; o < LPR; o <<= 1) {
-        sq += __shfl_xor(sq, o, 64);
-        some |= (bool)__shfl_xor((int)some, o, 64);
-    }
-    if (live && sub == 0) {
-        float f = (float)sq;
-        if (some && f == 0.f) f = __uint_as_float(1);
-        sqnorms[r] = f;
+        for (int o = 1; o < LPR; o <<= 1) {
+            sq += __shfl_xor(sq, o, 64);
+            some |= (bool)__shfl_xor((int)some, o, 64);
+        }
+        if (live && sub == 0) {
+            float f = (float)sq;
+            if (some && f == 0.f) f = __uint_as_float(1);
+            sqnorms[r] = f;
+        }
     }
 }
 
@@ -355,6 +357,11 @@ __device__ __forceinline__ float score_error(int metric, float c, float qnorm, f
     return 2.f * c * qnorm * xnorm + 0x1p-22f * xnorm * xnorm + 0x1p-140f;
 }
 
+// what some row of a tile is sure to reach; a tile with a row whose score says nothing is sure of nothing
+__device__ __forceinline__ float sure_score(int metric, float c, float qnorm, float xnorm, float top) {
+    return top < __builtin_inff() ? top - score_error(metric, c, qnorm, xnorm) : -__builtin_inff();
+}
+
 struct Near {              // what the search takes from the product kernels instead of the products
     int metric;
     const float *sqnorms;
@@ -440,7 +447,7 @@ q4_product_kernel(Rows t, const u32x4 *__restrict__ digits, const int *__restric
             if constexpr (NEAR) {
                 for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
                 if (b < B && col == 0) near.tile_score[(uint64_t)b * near.n_tiles + tile] = top;
-                best[c] = fmaxf(best[c], top - score_error(near.metric, near.err, qn[c], xn));
+                best[c] = fmaxf(best[c], sure_score(near.metric, near.err, qn[c], xn, top));
             }
         }
         tile += stride;
@@ -460,7 +467,7 @@ q4_product_kernel(Rows t, const u32x4 *__restrict__ digits, const int *__restric
 // for.  Both sides are scaled by a power of two to a norm of at most 2^8, so that nothing that matters is below f16's normal range:
 //   error <= |q| |x| (2^-11 of rounding the query + sqrt(dim) 2^-20 of what is flushed + dim 2^-24 of the f32 sums)
 // The loop is that of gemm_nt.h with the table's side made in registers: 16 bytes of codes (32 elements) a thread and step, loaded two steps
-// ahead, four packed f16 operations per 4 elements.  1M x 768, 1024 queries: XXX.
+// ahead, four packed f16 operations per 4 elements.  1M x 768, 1024 queries: 1.9 ms, 0.83 PFLOP/s; the same loop over bf16 rows runs at 1.05.
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 // the element (of 8) at each place of a 16-byte piece: a dword's nibbles are taken 16 bits apart
@@ -630,7 +637,7 @@ q4_scores_kernel(Rows t, gemm::Operand Q, const int *__restrict__ exponent, uint
                 const uint32_t b = n0 + G::wave_col() + j * 32 + (lane & 31);
                 const float v = fmaxf(top[j][x], __shfl_xor(top[j][x], 32, 64));
                 if (b < Q.rows && lane < 32) score[(uint64_t)tile * ldb + b] = v;
-                best[j] = fmaxf(best[j], v - score_error(near.metric, near.err, qn[j], xn));
+                best[j] = fmaxf(best[j], sure_score(near.metric, near.err, qn[j], xn, v));
             }
         }
         __syncthreads();  // LDS is free for the next rows
@@ -680,7 +687,7 @@ q4_need_kernel(Near near, bool by_tile, uint32_t k, float *__restrict__ need, do
     }
     constexpr int R = 16;  // values a thread keeps; more are read again for each 8 bits
     uint32_t kept[R];
-    auto value = [&](uint32_t i) { return order_of(by_tile ? v[i] - score_error(near.metric, near.err, qn, near.tile_norm[i]) : v[i]); };
+    auto value = [&](uint32_t i) { return order_of(by_tile ? sure_score(near.metric, near.err, qn, near.tile_norm[i], v[i]) : v[i]); };
 #pragma unroll
     for (int r = 0; r < R; r++) {
         const uint32_t i = threadIdx.x + r * 1024;
@@ -1099,8 +1106,8 @@ q4_join_kernel(const uint64_t *__restrict__ part_key, const uint32_t *__restrict
 }
 
 // ---- host side -------------------------------------------------------------------------------------------------------
-// lanes that share a row: 16 (a 64-byte piece of its codes), fewer for short rows.  More would spend longer on joining their sums: 64 lanes
-// made the k-NN's f64 distances XXX times as long.
+// lanes that share a row: 16 (a 64-byte piece of its codes), fewer for short rows.  More spend longer on joining their sums: with 64
+// the f64 distances of 1024 queries against 1M x 768 took 690 us instead of 379.
 uint32_t lanes_per_row(uint32_t chunks) { return chunks <= 4 ? 4 : chunks <= 8 ? 8 : 16; }
 #define CZ_Q4_LANES(LPR, CALL)      \
     switch (LPR) {                  \
@@ -1191,7 +1198,7 @@ int launch_product(const Rows &t, const ProductPlan &p, const float *q, uint32_t
     return launch_product_ct<1, NEAR>(t, p, B, out, near, stream);
 }
 
-// Up to so many queries the digits' product (100 us for each 16 of them at 1M x 768) is the faster way to the scores.
+// Up to so many queries the digits' product (100 us for each 16 of them at 1M x 768) is the faster way to the scores; at 48 both take 0.37 ms.
 constexpr uint32_t kDigitQueries = 32;
 using Tile128 = gemm::Tile<gemm::F16, 128, 128, 2, 2>;
 using Tile256 = gemm::Tile<gemm::F16, 256, 256, 2, 4>;
@@ -1239,7 +1246,8 @@ KnnPlan knn_plan(const Rows &t, uint32_t B, uint32_t k, void *ws) {
     p.part_count = c.take<uint32_t>((size_t)B * p.chunks);
     if (p.filtered) {
         p.steps = (t.groups << t.gshift) / 64 + ((t.groups << t.gshift) % 64 != 0);
-        p.halves = B <= kDigitQueries ? 0 : B <= 128 ? 1 : 2;
+        // 256 queries to a tile, unless 128 leave fewer columns unused (384 queries against 1M x 768: 0.93 ms instead of 1.10; 1024: 2.44 and 2.26)
+        p.halves = B <= kDigitQueries ? 0 : (B + 127) / 128 * 128 < (B + 255) / 256 * 256 ? 1 : 2;
         if (p.halves) {
             const uint32_t b = p.halves == 2 ? 256 : 128, qt = (B + b - 1) / b, blocks = (t.n + b - 1) / b, resident = p.halves == 2 ? 256 : 512;
             p.parts = std::max(1u, std::min(blocks, resident / qt));
@@ -1330,13 +1338,14 @@ extern "C" int cz_q4_quantize(const void *vectors, int elem, uint32_t n, uint32_
     }
     const bool wide = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (ld * es) % 16 == 0;
     const uint32_t lpr = std::max(lanes_per_row(t.chunks), group / 8);
+    const uint32_t grid = std::min((n + 256 / lpr - 1) / (256 / lpr), 1u << 22);  // (a launch has fewer than 2^32 threads)
 #define CZ_Q4_CALL(L)                                                                                                              \
     if (elem == CZ_ELEM_F32)                                                                                                       \
-        hipLaunchKernelGGL((q4_quantize_kernel<float, L>), dim3((n + 256 / L - 1) / (256 / L)), dim3(256), 0, stream,              \
-                           (const float *)x, ld, wide, t, codes, scales, sqnorms);                                                 \
+        hipLaunchKernelGGL((q4_quantize_kernel<float, L>), dim3(grid), dim3(256), 0, stream, (const float *)x, ld, wide, t, codes, \
+                           scales, sqnorms);                                                                                       \
     else                                                                                                                           \
-        hipLaunchKernelGGL((q4_quantize_kernel<uint16_t, L>), dim3((n + 256 / L - 1) / (256 / L)), dim3(256), 0, stream,           \
-                           (const uint16_t *)x, ld, wide, t, codes, scales, sqnorms)
+        hipLaunchKernelGGL((q4_quantize_kernel<uint16_t, L>), dim3(grid), dim3(256), 0, stream, (const uint16_t *)x, ld, wide, t,  \
+                           codes, scales, sqnorms)
     CZ_Q4_LANES(lpr, CZ_Q4_CALL);
 #undef CZ_Q4_CALL
     rc = launched("cz_q4_quantize");

@@ -93,7 +93,11 @@ class Q4Table:
         """f32 rows: those that `rows` names (a number that is no row: refused on the host, NaN on the GPU), or all"""
         L = _lib.lib()
         if not self._gpu:
-            r = None if rows is None else np.ascontiguousarray(rows, dtype=np.uint32).reshape(-1)
+            r = None if rows is None else np.asarray(rows).reshape(-1)
+            if r is not None:
+                if r.size and (r.dtype.kind not in "iu" or int(r.min()) < 0 or int(r.max()) >= self.n):
+                    raise ValueError("rows are numbers of rows of the table")
+                r = np.ascontiguousarray(r, dtype=np.uint32)
             m = self.n if r is None else r.size
             out = np.empty((m, self.dim), dtype=np.float32)
             check(L.cz_q4_dequantize(ptr(self.codes), ptr(self.scales), self.n, self.dim, self.group, ptr(r), m, ptr(out), 0, None))
@@ -103,7 +107,12 @@ class Q4Table:
             r = None
             if rows is not None:
                 all_on_gpu(self.codes, rows)
-                r = rows.to(torch.int32).contiguous()  # (a negative number becomes one that is no row)
+                if rows.dtype not in (torch.int32, torch.int64):
+                    raise ValueError(f"rows are int32 or int64, not {rows.dtype}")
+                r = rows.reshape(-1)
+                if r.dtype == torch.int64:  # what does not fit 31 bits is no row
+                    r = torch.where((r >= 0) & (r < 2**31), r, torch.full_like(r, -1)).to(torch.int32)
+                r = r.contiguous()
             m = self.n if r is None else r.numel()
             out = torch.empty((m, self.dim), dtype=torch.float32, device=self.codes.device)
             check(L.cz_q4_dequantize(ptr(self.codes), ptr(self.scales), self.n, self.dim, self.group, ptr(r), m, ptr(out),
