@@ -213,10 +213,13 @@ def test_dots_query_values(gpu_lib):
 METRICS = ["L2", "Cosine", "IP"]
 
 
-def _check_knn(t, q, x, k, metric, radius=None, host=False):
+def _check_knn(t, q, x, k, metric, radius=None, host=False, only=None):
+    """the answer to the whole batch, looked at for all queries or for those that `only` names"""
     ids, dist, cnt = t.knn(q if host else _cuda(q), k, distance=metric, radius=radius)
     if not host:
         ids, dist, cnt = ids.cpu().numpy().view(np.uint32), dist.cpu().numpy(), cnt.cpu().numpy().view(np.uint32)
+    if only is not None:
+        q, ids, dist, cnt = q[only], ids[only], dist[only], cnt[only]
     all_d = R.distances(metric, q, x)
     _, wdist, wcnt = R.nearest(all_d, k, radius)
     assert np.array_equal(cnt, wcnt)
