@@ -8,7 +8,8 @@
 // * operand layout of the 32 x 32 matrix instructions: lane l holds row l % 32 and the k that belong to half l / 32; as both
 //   operands are read alike, which k those are does not matter: a half is a 16-byte piece (8 bf16 = one 32x32x16 instruction, 4 f32 =
 //   four 32x32x2 ones).
-// * a turned operand lies in LDS as it does in memory, k by k: a k's rows in pieces of 16 bytes (8 rows), piece p at place p ^ 4 (k & 3).  The
+// * a turned operand lies in LDS as it does in memory, k by k: a k's rows in pieces of 16 bytes (8 rows), piece p at place p ^ 4 (k & 3)
+//   (64 rows: p ^ 4 (k / 2 & 1)).  The
 //   transposing read gives 16 lanes of 8 bytes (4 rows) at 4 k's back as 16 rows at 4 k's; 32 lanes read 64 bytes at each of 4 k's, each
 //   in a quarter of the banks of its own.
 // * accumulators: register r of lane l is C[8 (r / 4) + 4 (l / 32) + r % 4][l % 32] of its 32 x 32 tile.
@@ -67,6 +68,11 @@ struct Operand {
     uint32_t rows;
     uint64_t step = 128;    // bytes from a step of k to the next: 128 in ordinary rows, more where k is cut into panels
 };
+// ordinary rows of `bytes` bytes (a multiple of 16), read where they are although a step ends behind them: it gets zeros there
+struct Tailed {
+    Operand rows_of;
+    uint32_t rows, bytes;
+};
 // k in panels: a step's 128 bytes of every row lie one behind the other, so that a workgroup's step is one run of memory; in rows of 128 KB each
 // row of a step begins in the same few memory channels (grad_queries of a 65536-row piece: 179 us, with padded rows 168, in panels 164)
 // the same for an operand of a 16-bit type that lies turned: for each k the rows one behind the other
@@ -80,6 +86,8 @@ inline Operand panels(const void *base, uint32_t rows) { return Operand{(const c
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
+static __device__ const u32x4 kZeros = {0, 0, 0, 0};
+
 // a workgroup's copies of ROWS rows of an operand into LDS, a step at a time
 template <class O, int ROWS, int THREADS>
 struct Copies;
@@ -90,18 +98,29 @@ struct Copies<Operand, ROWS, THREADS> {
     static_assert(N * THREADS == ROWS * 8, "threads cover the copies");
     const char *src[N];
     uint64_t stride;
+    static __device__ __forceinline__ uint32_t piece(int i) {  // (of the step's 128 bytes)
+        const uint32_t c = i * THREADS + threadIdx.x;
+        return ((c & 7) ^ ((c >> 4) & 7)) * 16;
+    }
     __device__ __forceinline__ Copies(const Operand &o, uint32_t row0) : stride(o.step) {
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            const uint32_t c = i * THREADS + threadIdx.x, row = c >> 3, piece = (c & 7) ^ ((row >> 1) & 7);
-            src[i] = o.base + (uint64_t)min(row0 + row, o.rows - 1) * o.ld + piece * 16;
-        }
+        for (int i = 0; i < N; i++) src[i] = o.base + (uint64_t)min(row0 + (i * THREADS + threadIdx.x) / 8, o.rows - 1) * o.ld;
     }
-    __device__ __forceinline__ const char *from(int i, uint32_t step) const { return src[i] + step * stride; }
+    __device__ __forceinline__ const char *from(int i, uint32_t step) const { return src[i] + (step * stride + piece(i)); }
     // rows row0 + 32 i + lane % 32 at the 16 k's `kk` of a step
     static __device__ __forceinline__ u32x4 fragment(const char *lds, int row0, int i, int kk) {
         const int lane = threadIdx.x & 63, l32 = lane & 31;
         return *(const u32x4 *)(lds + (row0 + l32) * 128 + (((2 * kk + (lane >> 5)) ^ ((l32 >> 1) & 7)) * 16) + i * 32 * 128);
+    }
+};
+// (a kernel of its own for rows that end inside a step: the comparison in every copy took 10 % of the products that do not need it)
+template <int ROWS, int THREADS>
+struct Copies<Tailed, ROWS, THREADS> : Copies<Operand, ROWS, THREADS> {
+    uint32_t bytes;
+    __device__ __forceinline__ Copies(const Tailed &o, uint32_t row0) : Copies<Operand, ROWS, THREADS>(o.rows_of, row0), bytes(o.bytes) {}
+    __device__ __forceinline__ const char *from(int i, uint32_t step) const {
+        const uint32_t at = step * 128 + this->piece(i);
+        return at < bytes ? this->src[i] + at : reinterpret_cast<const char *>(&kZeros);
     }
 };
 template <int ROWS, int THREADS>
@@ -109,13 +128,16 @@ struct Copies<Turned, ROWS, THREADS> {
     static constexpr int N = ROWS * 8 / THREADS, P = ROWS / 8;  // pieces of a thread, of a k
     static constexpr int kReads = 2;
     static_assert(N * THREADS == ROWS * 8, "threads cover the copies");
+    static_assert(P >= 8, "a k's rows fill half of the banks at least");
+    // what a k's pieces are placed by (64 rows: two k's fill the banks)
+    static __device__ __forceinline__ uint32_t turn(uint32_t k) { return P >= 16 ? 4 * (k & 3) : 4 * ((k >> 1) & 1); }
     const char *src[N];
     uint64_t ld;
     uint32_t ks;
     __device__ __forceinline__ Copies(const Turned &o, uint32_t row0) : ld(o.ld), ks(o.ks) {
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            const uint32_t c = i * THREADS + threadIdx.x, k = c / P, piece = (c % P) ^ (4 * (k & 3));
+            const uint32_t c = i * THREADS + threadIdx.x, k = c / P, piece = (c % P) ^ turn(k);
             const uint32_t row = min(row0 + piece * 8, o.rows - 8);
             src[i] = o.base + (row >> 6) * o.panel + (row & 63) * 2;
         }
@@ -127,7 +149,7 @@ struct Copies<Turned, ROWS, THREADS> {
     static __device__ __forceinline__ u32x4 fragment(const char *lds, int row0, int i, int kk) {
         const int lane = threadIdx.x & 63, l16 = lane & 15;
         const int k = 16 * kk + 8 * (lane >> 5) + (l16 >> 2), col = row0 + i * 32 + 16 * ((lane >> 4) & 1) + 4 * (l16 & 3);
-        const int at = ((col >> 3) ^ (4 * (l16 >> 2))) * 16 + (col & 7) * 2;
+        const int at = ((col >> 3) ^ turn(l16 >> 2)) * 16 + (col & 7) * 2;
         typedef __attribute__((address_space(3))) s16x4 *Lds;
         const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(lds + k * P * 16 + at)),
                     b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(lds + (k + 4) * P * 16 + at));

@@ -6,7 +6,8 @@
 // Gradient, a piece of the table at a time:  P = grad_loss scale (softmax - onehot) of the piece is computed again and stored (in f32 in both
 // orders, in bf16 once: the matrix loop then reads P, Q and W turned where k is not what is contiguous), then  dW = P^T Q  is written and  dq += P W  goes to per-stretch partial sums (each added to by one workgroup only, in
 // a fixed order: no atomics).  A bf16 P loses what it rounds off; where that matters most, at the answers -- the largest entries, which may well
-// carry all the same value and so the same error -- the rest is kept in f32 and its term added to dW's row and to dq in f32.
+// carry all the same value and so the same error -- the rest is kept in f32 and its term added to dW's row and to dq in f32.  In f32 the answer's
+// entry is left out of dq's long sum, which would lose the small terms beside it, and added at its end.
 #include <algorithm>
 #include <cmath>
 
@@ -16,11 +17,13 @@
 using gemm::Bf16;
 using gemm::F32;
 using gemm::Operand;
+using gemm::Tailed;
 using gemm::Turned;
 
 namespace {
 
 constexpr uint32_t kMaxDim = 8192;
+uint32_t tiles_of(uint64_t n, uint32_t b) { return (uint32_t)((n + b - 1) / b); }
 constexpr float kLog2e = 1.44269504088896340736f;
 
 __device__ __forceinline__ float up(float x) { return x; }
@@ -92,9 +95,9 @@ xent_transpose_kernel(const T *__restrict__ x, uint64_t ld, bool wide, uint32_t 
     }
 }
 
-template <class G>
+template <class G, class O>
 __global__ void __launch_bounds__(G::kThreads)
-xent_forward_kernel(Operand W, Operand Q, uint32_t steps, float scale2, uint32_t n_tiles, uint32_t tiles_per_part,
+xent_forward_kernel(O W, Operand Q, uint32_t steps, float scale2, uint32_t n_tiles, uint32_t tiles_per_part,
                     uint32_t part0, float2 *__restrict__ parts) {
     constexpr int BM = G::BM, BN = G::BN, WM = G::WM, WN = G::WN;
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -189,10 +192,11 @@ xent_join_kernel(const float2 *__restrict__ parts, uint32_t n_parts, const T *__
     loss[t] = y == CZ_NONE ? 0.f : y < V ? (float)(e - (double)scale * z) : __builtin_nanf("");
 }
 
-// P of a piece: p[t][v] and pt[v][t], in panels of v and of t, zeros where the piece or the queries (up to tp) end; rest[t]: what rounding the answer's entry cut off
-template <class G>
+// P of a piece: p[t][v] and pt[v][t], in panels of v and of t, zeros where the piece or the queries (up to tp) end; rest[t]: what rounding
+// the answer's entry cut off (bf16), or that entry, which p then has as 0 (f32)
+template <class G, class O>
 __global__ void __launch_bounds__(G::kThreads)
-xent_weights_kernel(Operand W, uint32_t v0, uint32_t V, Operand Q, uint32_t steps, float scale, const uint32_t *__restrict__ targets,
+xent_weights_kernel(O W, uint32_t v0, uint32_t V, Operand Q, uint32_t steps, float scale, const uint32_t *__restrict__ targets,
                     const float *__restrict__ lse, const float *__restrict__ grad_loss, typename G::Elem::T *__restrict__ p,
                     typename G::Elem::T *__restrict__ pt, uint32_t vp, uint32_t tp, float *__restrict__ rest) {
     typedef typename G::Elem E;
@@ -203,31 +207,33 @@ xent_weights_kernel(Operand W, uint32_t v0, uint32_t V, Operand Q, uint32_t step
     const int lane = threadIdx.x & 63;
     G g;
     g.run(W, m0, Q, n0, 0, steps, lds);
-    const float scale2 = scale * kLog2e;
+    constexpr bool kSplit = sizeof(typename E::T) == 2;
 #pragma unroll
     for (int j = 0; j < G::NT; j++) {
         const uint32_t t = n0 + G::wave_col() + j * 32 + (lane & 31);
         const uint32_t y = t < Q.rows ? targets[t] : CZ_NONE;
         const bool on = t < Q.rows && has_answer(y, V);
-        const float l2 = on ? lse[t] * kLog2e : 0.f, weight = on ? grad_loss[t] * scale : 0.f;
+        const float e = on ? lse[t] : 0.f, weight = on ? grad_loss[t] * scale : 0.f;
 #pragma unroll
         for (int i = 0; i < G::MT; i++)
 #pragma unroll
             for (int r4 = 0; r4 < 4; r4++) {
                 const uint32_t v = m0 + G::wave_row() + i * 32 + 8 * r4 + 4 * (lane >> 5);
-                typename E::T o[4];
+                typename E::T o[4], own[4];  // for dW and for dq
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    float x = exp2_(fmaf(g.acc[i][j][4 * r4 + r], scale2, -l2));
+                    // (to base 2 only after the difference: log2(e) lse and log2(e) scale, rounded, would be an error that a query's entries share)
+                    float x = exp2_(fmaf(g.acc[i][j][4 * r4 + r], scale, -e) * kLog2e);
                     const bool hit = on && v0 + v + r == y;
                     if (hit) x -= 1.f;
                     x = on && v + r < W.rows ? x * weight : 0.f;
                     o[r] = down<typename E::T>(x);
-                    if (hit && rest) rest[t] = x - up(o[r]);
+                    if (hit) rest[t] = kSplit ? x - up(o[r]) : x;
+                    own[r] = !kSplit && hit ? (typename E::T)0.f : o[r];
                 }
                 if (t < tp && p) {
                     typedef typename E::T T4 __attribute__((ext_vector_type(4)));
-                    *(T4 *)(p + in_panels<typename E::T>(t, v, tp)) = T4{o[0], o[1], o[2], o[3]};
+                    *(T4 *)(p + in_panels<typename E::T>(t, v, tp)) = T4{own[0], own[1], own[2], own[3]};
                 }
                 if (t < tp && pt)
 #pragma unroll
@@ -236,7 +242,7 @@ xent_weights_kernel(Operand W, uint32_t v0, uint32_t V, Operand Q, uint32_t step
     }
 }
 
-// what is left of the answers' own terms (rest = null: nothing, P is f32)
+// what is left of the answers' own terms
 template <typename T>
 struct Answers {
     const uint32_t *targets;
@@ -259,7 +265,7 @@ xent_table_grad_kernel(O Pt, O Qt, uint32_t steps, Answers<typename G::Elem::T> 
     g.run(Pt, m0, Qt, n0, 0, steps, lds);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint32_t *count = (uint32_t *)lds, *list = count + kWaves;  // of each wave; the queries that rows of this tile answer, ascending
-    if (an.rest)
+    if (sizeof(typename G::Elem::T) == 2 && an.rest)
     for (uint32_t t0 = 0; t0 < an.T_n; t0 += G::kThreads) {
         const uint32_t t = t0 + threadIdx.x, y = t < an.T_n ? an.targets[t] : CZ_NONE;
         const bool here = y < an.V && y >= v0 + m0 && y - v0 - m0 < BM;
@@ -340,7 +346,7 @@ xent_sum_parts_kernel(const float *__restrict__ parts, uint32_t n_parts, uint64_
             if (an.targets) {
                 const uint32_t t = (uint32_t)(i / dim), y = an.targets[t];
                 // (without an answer: zero weights, which a table row that is not finite would have made more of)
-                v = !has_answer(y, an.V) ? 0.f : an.rest ? v + an.rest[t] * up(an.w[y * an.ldw + (i - (uint64_t)t * dim)]) : v;
+                v = has_answer(y, an.V) ? v + an.rest[t] * up(an.w[y * an.ldw + (i - (uint64_t)t * dim)]) : 0.f;
             }
             out[i] = down<T>(v);
         }
@@ -364,8 +370,7 @@ struct Shape {
 struct Plan {
     uint32_t piece;        // table rows worked on at a time
     uint32_t parts;        // forward: stretches of a piece; backward: partial sums of grad_queries
-    int fwd;               // forward's tile: 0 narrow, 1 small, 2 large
-    bool large_p, large_w, large_q;  // backward's tiles: of P, of grad_table, of grad_queries
+    int fwd, of_p, of_w, of_q;  // tiles (TileOf): forward's; backward's of P, of grad_table, of grad_queries
     void *q, *w;           // packed copies (unaligned rows or a dim that is no multiple of a step)
     void *qt, *wt, *p, *pt;  // (bf16: qt is a copy of the queries without those that have no answer, wt and pt are not needed)
     float2 *stats;
@@ -373,18 +378,29 @@ struct Plan {
     size_t bytes;
 };
 
-// Tiles of the four products.  Large: most products per byte of LDS; small: more workgroups when there are few tiles; and for a few
-// queries a narrow one, which does not spend the f32 matrix cores on columns that are not there.
+// Tiles of the four products, table rows (or, for grad_queries, queries) first.  Large: most products for what is read; the smaller ones where
+// large tiles would leave CUs without work; narrow and flat for a few queries, which do not spend the matrix cores on columns that are not there
+// (4 queries, 17601 rows of 840 in f32: 277 us with 128 x 128 throughout, 148 with these).
 template <class E> using Large = gemm::Tile<E, 256, 256, 2, 4>;
 template <class E> using Small = gemm::Tile<E, 128, 128, 2, 2>;
+template <class E> using Tiny = gemm::Tile<E, 64, 64, 2, 2>;
 template <class E> using Narrow = gemm::Tile<E, 128, 32, 4, 1>;
+template <class E> using Flat = gemm::Tile<E, 32, 128, 1, 4>;
+enum TileOf { kLarge, kSmall, kTiny, kNarrow, kFlat };
+constexpr uint32_t kFull = 192;  // tiles (one to a CU) that are taken to fill the chip's 256 CUs
 
-// every tile of `big` x `big` fills the chip's 256 CUs about as well as tiles of half the size would
-bool enough(uint64_t m, uint64_t n) { return ((m + 255) / 256) * ((n + 255) / 256) >= 192 && n > 128 && m > 128; }
+uint32_t rows_of(TileOf t) { return t == kLarge ? 256 : t == kTiny ? 64 : t == kFlat ? 32 : 128; }
+uint32_t cols_of(TileOf t) { return t == kLarge ? 256 : t == kTiny ? 64 : t == kNarrow ? 32 : 128; }
+uint64_t count_of(TileOf t, uint64_t m, uint64_t n) { return (m + rows_of(t) - 1) / rows_of(t) * ((n + cols_of(t) - 1) / cols_of(t)); }
+// the largest tile with which m x n fills the chip
+TileOf filling(uint64_t m, uint64_t n) {
+    if (m > 128 && n > 128 && count_of(kLarge, m, n) >= kFull) return kLarge;
+    return count_of(kSmall, m, n) >= kFull ? kSmall : kTiny;
+}
 
-// rows that the matrix loop can read where they are
+// rows that the matrix loop can read where they are (the queries also need whole steps: theirs are the zeros behind a row)
 bool direct(const void *x, uint64_t ld, uint32_t dim, uint32_t es) {
-    return (reinterpret_cast<uintptr_t>(x) & 15) == 0 && ld * es % 16 == 0 && dim * es % 128 == 0;
+    return (reinterpret_cast<uintptr_t>(x) & 15) == 0 && ld * es % 16 == 0 && dim * es % 16 == 0;
 }
 
 Plan make_plan(const Shape &s, bool grad, void *ws) {
@@ -399,9 +415,10 @@ Plan make_plan(const Shape &s, bool grad, void *ws) {
     pl.w = c.take<uint8_t>((uint64_t)pl.piece * kp * es);
     if (!grad) {
         // a table that can be read where it is goes in one piece, another one packed piece by piece: stretches for the larger
-        pl.fwd = s.T <= 32 ? 0 : s.T > 128 && s.V >= 64 * 256 ? 2 : 1;
-        const uint32_t bm = pl.fwd == 2 ? 256 : 128, bn = pl.fwd == 2 ? 256 : pl.fwd == 1 ? 128 : 32;
-        const uint32_t qt = (s.T + bn - 1) / bn, tiles = (s.V + bm - 1) / bm, resident = pl.fwd == 2 ? 256 : pl.fwd == 1 ? 512 : 1024;
+        pl.fwd = s.T <= 32 ? kNarrow : filling(s.V, s.T);
+        const TileOf f = (TileOf)pl.fwd;
+        const uint32_t qt = tiles_of(s.T, cols_of(f)), tiles = tiles_of(s.V, rows_of(f));
+        const uint32_t resident = f == kLarge ? 256 : f == kSmall ? 512 : 1024;
         pl.parts = std::max(1u, std::min(tiles, resident / qt));
         pl.stats = c.take<float2>((uint64_t)pl.parts * ((s.V + pl.piece - 1) / pl.piece) * s.T);
     } else {
@@ -412,13 +429,13 @@ Plan make_plan(const Shape &s, bool grad, void *ws) {
             pl.pt = c.take<uint8_t>(pl.piece * tp * es);
         }
         const uint32_t nv = std::min(s.V, pl.piece);
-        pl.large_p = enough(nv, tp);
-        pl.large_w = enough(nv, s.dim);
-        pl.large_q = s.T > 128 && s.dim > 128;
-        const uint32_t b = pl.large_q ? 256 : 128, tiles = ((s.T + b - 1) / b) * ((s.dim + b - 1) / b);
-        // as many stretches of a piece as fill the chip, of at least 8 steps
-        pl.parts = std::max(1u, std::min((pl.large_q ? 256 : 512) / tiles, (uint32_t)(up_to(nv, 256) / s.kstep() / 8)));
-        pl.rest = s.bf16 ? c.take<float>(s.T) : nullptr;
+        const uint32_t steps = (uint32_t)up_to(nv, 256) / s.kstep(), most = std::max(1u, steps / 8);  // stretches of at least 8 steps
+        pl.of_p = s.T <= 32 ? kNarrow : filling(nv, tp);
+        pl.of_w = filling(nv, s.dim);
+        pl.of_q = s.T <= 32 ? kFlat : s.T > 128 && s.dim > 128 && count_of(kLarge, s.T, s.dim) * most >= kFull ? kLarge : kSmall;
+        const uint32_t tiles = (uint32_t)count_of((TileOf)pl.of_q, s.T, s.dim), resident = pl.of_q == kLarge ? 256 : pl.of_q == kSmall ? 512 : 1024;
+        pl.parts = std::max(1u, std::min({resident / tiles, most, 256u}));
+        pl.rest = c.take<float>(s.T);
         pl.dq = c.take<float>((uint64_t)pl.parts * s.T * s.dim);
     }
     pl.bytes = c.used();
@@ -446,12 +463,15 @@ int launch(K kernel, uint32_t grid, hipStream_t stream, A... args) {
     hipLaunchKernelGGL(kernel, dim3(grid), dim3(G::kThreads), G::kLds, stream, args...);
     return CZ_OK;
 }
-uint32_t tiles_of(uint64_t n, int b) { return (uint32_t)((n + b - 1) / b); }
-
-template <class G>
-int forward_piece(const Operand &W, const Operand &Q, uint32_t steps, float scale2, uint32_t parts, uint32_t part0, float2 *stats, hipStream_t stream) {
+// f over W as it is, or (tail: bytes of a row that ends inside a step) with zeros behind its rows
+template <class F>
+int over(const Operand &W, uint32_t tail, F f) {
+    return tail ? f(Tailed{W, W.rows, tail}) : f(W);
+}
+template <class G, class O>
+int forward_piece(const O &W, const Operand &Q, uint32_t steps, float scale2, uint32_t parts, uint32_t part0, float2 *stats, hipStream_t stream) {
     const uint32_t tiles = tiles_of(W.rows, G::BM);
-    return launch<G>(xent_forward_kernel<G>, parts * tiles_of(Q.rows, G::BN), stream, W, Q, steps, scale2, tiles, (tiles + parts - 1) / parts, part0, stats);
+    return launch<G>(xent_forward_kernel<G, O>, parts * tiles_of(Q.rows, G::BN), stream, W, Q, steps, scale2, tiles, (tiles + parts - 1) / parts, part0, stats);
 }
 
 template <class E>
@@ -461,7 +481,7 @@ int forward(const Shape &s, const Plan &pl, const void *q_, const void *w_, cons
     const T *q = (const T *)q_, *w = (const T *)w_;
     const uint32_t es = s.es(), kp = s.kp(), steps = kp / s.kstep();
     Operand Q{(const char *)q, s.ldq * es, s.T};
-    if (!direct(q, s.ldq, s.dim, es)) {
+    if (!direct(q, s.ldq, s.dim, es) || s.dim != kp) {
         pack(q, s.ldq, s.T, s.dim, pl.q, kp, stream);
         Q = Operand{(const char *)pl.q, (uint64_t)kp * es, s.T};
     }
@@ -475,9 +495,10 @@ int forward(const Shape &s, const Plan &pl, const void *q_, const void *w_, cons
             pack(w + v0 * s.ldw, s.ldw, nv, s.dim, pl.w, kp, stream);
             W = Operand{(const char *)pl.w, (uint64_t)kp * es, nv};
         }
-        const int rc = pl.fwd == 2   ? forward_piece<Large<E>>(W, Q, steps, scale * kLog2e, pl.parts, parts, pl.stats, stream)
-                       : pl.fwd == 1 ? forward_piece<Small<E>>(W, Q, steps, scale * kLog2e, pl.parts, parts, pl.stats, stream)
-                                     : forward_piece<Narrow<E>>(W, Q, steps, scale * kLog2e, pl.parts, parts, pl.stats, stream);
+        const int rc = over(W, wd && s.dim != kp ? s.dim * es : 0, [&](const auto &O) {
+            auto go = [&](auto g) { return forward_piece<decltype(g)>(O, Q, steps, scale * kLog2e, pl.parts, parts, pl.stats, stream); };
+            return pl.fwd == kLarge ? go(Large<E>{}) : pl.fwd == kSmall ? go(Small<E>{}) : pl.fwd == kTiny ? go(Tiny<E>{}) : go(Narrow<E>{});
+        });
         if (rc) return rc;
         parts += pl.parts;
     }
@@ -493,11 +514,11 @@ void transpose(const T *x, uint64_t ld, uint32_t n, uint32_t dim, const uint32_t
                        (T *)out, width);
 }
 
-template <class G>
-int weights_of(const Operand &W, uint32_t v0, uint32_t V, const Operand &Q, uint32_t steps, float scale, const uint32_t *targets, const float *lse,
+template <class G, class O>
+int weights_of(const O &W, uint32_t v0, uint32_t V, const Operand &Q, uint32_t steps, float scale, const uint32_t *targets, const float *lse,
                const float *grad_loss, void *p, uint32_t vp, void *pt, uint32_t tp, float *rest, hipStream_t stream) {
     typedef typename G::Elem::T T;
-    return launch<G>(xent_weights_kernel<G>, tiles_of(vp, G::BM) * tiles_of(tp, G::BN), stream, W, v0, V, Q, steps, scale, targets, lse, grad_loss,
+    return launch<G>(xent_weights_kernel<G, O>, tiles_of(vp, G::BM) * tiles_of(tp, G::BN), stream, W, v0, V, Q, steps, scale, targets, lse, grad_loss,
                      (T *)p, (T *)pt, vp, tp, rest);
 }
 template <class G, class O>
@@ -518,7 +539,7 @@ int backward(const Shape &s, const Plan &pl, const void *q_, const void *w_, con
     const T *q = (const T *)q_, *w = (const T *)w_;
     const uint32_t es = s.es(), kp = s.kp(), tp = s.tp(), steps = kp / s.kstep();
     Operand Q{(const char *)q, s.ldq * es, s.T};
-    if (!direct(q, s.ldq, s.dim, es)) {
+    if (!direct(q, s.ldq, s.dim, es) || s.dim != kp) {
         pack(q, s.ldq, s.T, s.dim, pl.q, kp, stream);
         Q = Operand{(const char *)pl.q, (uint64_t)kp * es, s.T};
     }
@@ -538,18 +559,20 @@ int backward(const Shape &s, const Plan &pl, const void *q_, const void *w_, con
             W = Operand{(const char *)pl.w, (uint64_t)kp * es, nv};
         }
         void *p = dq || kTurned ? pl.p : nullptr, *pt = dw && !kTurned ? pl.pt : nullptr;
-        int rc = pl.large_p ? weights_of<Large<E>>(W, v0, s.V, Q, steps, scale, targets, lse, grad_loss, p, vp, pt, tp, pl.rest, stream)
-                            : weights_of<Small<E>>(W, v0, s.V, Q, steps, scale, targets, lse, grad_loss, p, vp, pt, tp, pl.rest, stream);
+        int rc = over(W, wd && s.dim != kp ? s.dim * es : 0, [&](const auto &O) {
+            auto go = [&](auto g) { return weights_of<decltype(g)>(O, v0, s.V, Q, steps, scale, targets, lse, grad_loss, p, vp, pt, tp, pl.rest, stream); };
+            return pl.of_p == kLarge ? go(Large<E>{}) : pl.of_p == kSmall ? go(Small<E>{}) : pl.of_p == kTiny ? go(Tiny<E>{}) : go(Narrow<E>{});
+        });
         if (rc) return rc;
         const uint32_t vsteps = vp / s.kstep();
         if (dq) {
             const Operand P = gemm::panels(pl.p, tp);
             auto query_grad = [&](const auto &Wt) {
-                return pl.large_q ? query_grad_of<Large<E>>(P, Wt, s.T, vsteps, pl.parts, v0 != 0, pl.dq, s.dim, stream)
-                                  : query_grad_of<Small<E>>(P, Wt, s.T, vsteps, pl.parts, v0 != 0, pl.dq, s.dim, stream);
+                auto go = [&](auto g) { return query_grad_of<decltype(g)>(P, Wt, s.T, vsteps, pl.parts, v0 != 0, pl.dq, s.dim, stream); };
+                return pl.of_q == kLarge ? go(Large<E>{}) : pl.of_q == kSmall ? go(Small<E>{}) : go(Flat<E>{});
             };
             if constexpr (kTurned) {
-                rc = query_grad(Turned{W.base, W.ld, 128, kp, nv});
+                rc = query_grad(Turned{W.base, W.ld, 128, wd ? s.dim : kp, nv});
             } else {
                 transpose(wv, s.ldw, nv, s.dim, (const uint32_t *)nullptr, 0u, pl.wt, vp, stream);
                 rc = query_grad(gemm::panels(pl.wt, s.dim));
@@ -559,8 +582,8 @@ int backward(const Shape &s, const Plan &pl, const void *q_, const void *w_, con
         if (dw) {
             T *out = (T *)dw + (uint64_t)v0 * s.dim;
             auto table_grad = [&](const auto &Pt, const auto &Qt) {
-                return pl.large_w ? table_grad_of<Large<E>>(Pt, Qt, tp / s.kstep(), an, v0, nv, out, s.dim, stream)
-                                  : table_grad_of<Small<E>>(Pt, Qt, tp / s.kstep(), an, v0, nv, out, s.dim, stream);
+                auto go = [&](auto g) { return table_grad_of<decltype(g)>(Pt, Qt, tp / s.kstep(), an, v0, nv, out, s.dim, stream); };
+                return pl.of_w == kLarge ? go(Large<E>{}) : pl.of_w == kSmall ? go(Small<E>{}) : go(Tiny<E>{});
             };
             if constexpr (kTurned) rc = table_grad(Turned{(const char *)pl.p, 128, tp * 128ull, vp, tp}, Turned{(const char *)pl.qt, (uint64_t)kp * es, 128, kp, tp});
             else rc = table_grad(gemm::panels(pl.pt, vp), gemm::panels(pl.qt, s.dim));

@@ -284,3 +284,30 @@ def test_tables_beyond_four_gigabytes(gpu_lib):
     assert float((dq - wdq).norm() / wdq.norm()) <= 1e-4
     for rows in (at[:2], torch.arange(V - 300, V, device="cuda"), torch.tensor([1_048_575, 1_048_576, 1_048_577], device="cuda")):
         assert float((dw[rows] - p[:, rows].T @ q.double()).norm() / (p[:, rows].T @ q.double()).norm()) <= 1e-4
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dim", [4, 24, 72, 100, 200, 840])
+@pytest.mark.parametrize("T", [3, 40, 200])
+def test_rows_that_end_inside_a_step(gpu_lib, dtype, dim, T):
+    """rows read where they are although they are no whole number of steps: what lies between two rows, or in the next one, is not seen"""
+    import torch
+    from tests.test_softmax_xent import _case, _check, _cuda as cuda, _host, _run
+    V = 333
+    q, w, q64, w64, y, g = _case(T, V, dim, dtype, dim + T)
+    tw, tq = cuda(w), cuda(q)
+    want = _run(tq, tw, cuda(y), cuda(g), 1.5)
+    _check(q, w, q64, w64, y, g, 1.5, dtype, [_host(a) for a in want])
+    wide = torch.full((V, dim + 24), float("nan"), device="cuda").to(tw.dtype)
+    wide[:, :dim] = tw
+    got = _run(tq, wide[:, :dim], cuda(y), cuda(g), 1.5)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    # a row that is not finite is its own affair: the logits of the row before it are not touched (its weight is nothing, as -inf)
+    tw2, tq2 = tw.clone(), tq.abs() + 0.5
+    y2 = torch.where(cuda(y) == 200, torch.full_like(cuda(y), 7), cuda(y))
+    tw2[200] = -float("inf")
+    rest = torch.cat([tw[:200], tw[201:]])
+    y3 = torch.where(y2 > 200, y2 - 1, y2)
+    a, b = _run(tq2, tw2, y2, cuda(g), 1.0)[:2], _run(tq2, rest, y3, cuda(g), 1.0)[:2]
+    assert all(bool(((x - z).abs() <= 1e-4 + 1e-6 * z.abs()).all()) for x, z in zip(a, b))
