@@ -10,6 +10,7 @@
 // entry is left out of dq's long sum, which would lose the small terms beside it, and added at its end.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "call.h"
 #include "gemm_nt.h"
@@ -95,9 +96,60 @@ xent_transpose_kernel(const T *__restrict__ x, uint64_t ld, bool wide, uint32_t 
     }
 }
 
+// scale log2(e) in two parts: a factor rounded to f32 would move all logits alike.  low has high's sign and is not zero where high is not, so that
+// infinite products stay what they are.
+struct Scale2 {
+    float high, low;
+    static Scale2 of(float scale) {
+        const double x = (double)scale * 1.44269504088896340736;
+        if (!(x != 0.0 && std::fabs(x) <= 3e38)) return Scale2{(float)x, (float)x};
+        float high = (float)x;
+        if (std::fabs((double)high) > std::fabs(x)) high = std::nextafter(high, 0.f);
+        return Scale2{high, std::copysign((float)std::max(std::fabs(x - (double)high), 1.2e-38), high)};
+    }
+};
+
+// A tile's products taken into the running maximum m and sum l of each of the lane's queries, to base 2.  The maximum is that of the products (the
+// least one where the scale is negative) and scaled once; a term is then two fused multiply-adds, an exponential and an addition, and no product
+// is rounded before the difference.  PART: only the first `left` rows exist.
+template <class G, bool PART>
+__device__ __forceinline__ void take(const G &g, uint32_t left, Scale2 scale2, float (&m)[G::NT], float (&l)[G::NT]) {
+    const int lane = threadIdx.x & 63;
+    const bool least = scale2.high < 0.f;
+    const float none = least ? __builtin_inff() : -__builtin_inff();
+    auto is_there = [&](int i, int r) { return (uint32_t)(G::wave_row() + i * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3)) < left; };
+#pragma unroll
+    for (int j = 0; j < G::NT; j++) {
+        float top = none;
+        if (least) {
+#pragma unroll
+            for (int i = 0; i < G::MT; i++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) top = fminf(top, !PART || is_there(i, r) ? g.acc[i][j][r] : none);
+        } else {
+#pragma unroll
+            for (int i = 0; i < G::MT; i++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) top = fmaxf(top, !PART || is_there(i, r) ? g.acc[i][j][r] : none);
+        }
+        top = fmaxf(m[j], top * scale2.high);
+        const float ref = reference(top);
+        float sum = m[j] == -__builtin_inff() ? l[j] : l[j] * exp2_(m[j] - ref);
+#pragma unroll
+        for (int i = 0; i < G::MT; i++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const float e = exp2_(fmaf(g.acc[i][j][r], scale2.low, fmaf(g.acc[i][j][r], scale2.high, -ref)));
+                sum += !PART || is_there(i, r) ? e : 0.f;
+            }
+        m[j] = top;
+        l[j] = sum;
+    }
+}
+
 template <class G, class O>
 __global__ void __launch_bounds__(G::kThreads)
-xent_forward_kernel(O W, Operand Q, uint32_t steps, float scale2, uint32_t n_tiles, uint32_t tiles_per_part,
+xent_forward_kernel(O W, Operand Q, uint32_t steps, Scale2 scale2, uint32_t n_tiles, uint32_t tiles_per_part,
                     uint32_t part0, float2 *__restrict__ parts) {
     constexpr int BM = G::BM, BN = G::BN, WM = G::WM, WN = G::WN;
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -112,28 +164,8 @@ xent_forward_kernel(O W, Operand Q, uint32_t steps, float scale2, uint32_t n_til
     for (uint32_t t = t0; t < t1; t++) {
         g.run(W, t * BM, Q, n0, 0, steps, lds);
         const uint32_t left = W.rows - t * BM;  // rows of this tile that exist
-#pragma unroll
-        for (int j = 0; j < G::NT; j++) {
-            float top = m[j];
-#pragma unroll
-            for (int i = 0; i < G::MT; i++)
-#pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    const uint32_t row = G::wave_row() + i * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
-                    const float z = row < left ? g.acc[i][j][r] * scale2 : -__builtin_inff();
-                    g.acc[i][j][r] = z;
-                    top = fmaxf(top, z);
-                }
-            const float ref = reference(top);
-            float sum = l[j] * exp2_(m[j] - ref);
-            if (m[j] == -__builtin_inff()) sum = l[j];
-#pragma unroll
-            for (int i = 0; i < G::MT; i++)
-#pragma unroll
-                for (int r = 0; r < 16; r++) sum += exp2_(g.acc[i][j][r] - ref);
-            m[j] = top;
-            l[j] = sum;
-        }
+        if (left >= BM) take<G, false>(g, left, scale2, m, l);
+        else take<G, true>(g, left, scale2, m, l);
         __syncthreads();  // LDS is free for the next tile
     }
     // lanes that hold the same query: the two halves, then the waves along m
@@ -325,7 +357,8 @@ xent_query_grad_kernel(Operand P, O Wt, uint32_t T, uint32_t steps, uint32_t ste
     });
 }
 
-// grad_queries: the partial sums added up, and the rest for the rows that answer; four lanes to an element and four sums in flight in each
+// grad_queries: the partial sums added up, and the rest for the rows that answer; four lanes to an element, 16 loads on their way in each
+// (255 queries, 96 wide, 256 sums: 8 us; with four loads 32)
 template <typename T>
 __global__ void __launch_bounds__(256)
 xent_sum_parts_kernel(const float *__restrict__ parts, uint32_t n_parts, uint64_t n, uint32_t dim, Answers<T> an, T *__restrict__ out) {
@@ -334,11 +367,17 @@ xent_sum_parts_kernel(const float *__restrict__ parts, uint32_t n_parts, uint64_
     for (uint64_t i0 = (uint64_t)blockIdx.x * 64; i0 < n; i0 += (uint64_t)gridDim.x * 64) {
         const uint64_t i = i0 + lane;
         float a[4] = {0.f, 0.f, 0.f, 0.f};
-        if (i < n)
-            for (uint32_t p = wave; p < n_parts; p += 16)
+        if (i < n) {
+            uint32_t p = wave;
+            for (; p + 4 * 15 < n_parts; p += 64) {  // (16 loads on their way)
+                float v[16];
 #pragma unroll
-                for (int u = 0; u < 4; u++)
-                    if (p + 4 * u < n_parts) a[u] += parts[(p + 4 * u) * n + i];
+                for (int u = 0; u < 16; u++) v[u] = parts[(p + 4 * u) * n + i];
+#pragma unroll
+                for (int u = 0; u < 16; u++) a[u & 3] += v[u];
+            }
+            for (; p < n_parts; p += 4) a[0] += parts[p * n + i];
+        }
         sums[wave][lane] = (a[0] + a[1]) + (a[2] + a[3]);
         __syncthreads();
         if (wave == 0 && i < n) {
@@ -386,6 +425,8 @@ template <class E> using Small = gemm::Tile<E, 128, 128, 2, 2>;
 template <class E> using Tiny = gemm::Tile<E, 64, 64, 2, 2>;
 template <class E> using Narrow = gemm::Tile<E, 128, 32, 4, 1>;
 template <class E> using Flat = gemm::Tile<E, 32, 128, 1, 4>;
+// (in f32 the products over rows and queries have no large tile: see large_in_f32)
+template <class E> using Long = std::conditional_t<sizeof(typename E::T) == 2, Large<E>, Small<E>>;
 enum TileOf { kLarge, kSmall, kTiny, kNarrow, kFlat };
 constexpr uint32_t kFull = 192;  // tiles (one to a CU) that are taken to fill the chip's 256 CUs
 
@@ -393,9 +434,20 @@ uint32_t rows_of(TileOf t) { return t == kLarge ? 256 : t == kTiny ? 64 : t == k
 uint32_t cols_of(TileOf t) { return t == kLarge ? 256 : t == kTiny ? 64 : t == kNarrow ? 32 : 128; }
 uint64_t count_of(TileOf t, uint64_t m, uint64_t n) { return (m + rows_of(t) - 1) / rows_of(t) * ((n + cols_of(t) - 1) / cols_of(t)); }
 // the largest tile with which m x n fills the chip
-TileOf filling(uint64_t m, uint64_t n) {
-    if (m > 128 && n > 128 && count_of(kLarge, m, n) >= kFull) return kLarge;
+TileOf filling(bool large, uint64_t m, uint64_t n) {
+    if (large && m > 128 && n > 128 && count_of(kLarge, m, n) >= kFull) return kLarge;
     return count_of(kSmall, m, n) >= kFull ? kSmall : kTiny;
+}
+
+// f32's matrix instructions take 16 times as long for what is read, so that large tiles are no gain, and with 128 accumulators a lane has no room
+// for more than one sum; but over few steps what a tile costs besides them counts (small and large tiles, 255 queries x 100003 rows, 96 wide:
+// forward 76 and 65 us, weights 100 and 93; loss + gradient of 645 x 32103, 165 wide: 471 and 488)
+bool large_in_f32(uint32_t dim) { return dim <= 128; }
+
+// f of the tile that t says; LARGE, TINY and OTHER: what a product has under these names
+template <class E, class LARGE, class TINY, class OTHER, class F>
+int with_tile(int t, F f) {
+    return t == kLarge ? f(LARGE{}) : t == kSmall ? f(Small<E>{}) : t == kTiny ? f(TINY{}) : f(OTHER{});
 }
 
 // rows that the matrix loop can read where they are (the queries also need whole steps: theirs are the zeros behind a row)
@@ -415,7 +467,7 @@ Plan make_plan(const Shape &s, bool grad, void *ws) {
     pl.w = c.take<uint8_t>((uint64_t)pl.piece * kp * es);
     if (!grad) {
         // a table that can be read where it is goes in one piece, another one packed piece by piece: stretches for the larger
-        pl.fwd = s.T <= 32 ? kNarrow : filling(s.V, s.T);
+        pl.fwd = s.T <= 32 ? kNarrow : filling(s.bf16 || large_in_f32(s.dim), s.V, s.T);
         const TileOf f = (TileOf)pl.fwd;
         const uint32_t qt = tiles_of(s.T, cols_of(f)), tiles = tiles_of(s.V, rows_of(f));
         const uint32_t resident = f == kLarge ? 256 : f == kSmall ? 512 : 1024;
@@ -430,9 +482,9 @@ Plan make_plan(const Shape &s, bool grad, void *ws) {
         }
         const uint32_t nv = std::min(s.V, pl.piece);
         const uint32_t steps = (uint32_t)up_to(nv, 256) / s.kstep(), most = std::max(1u, steps / 8);  // stretches of at least 8 steps
-        pl.of_p = s.T <= 32 ? kNarrow : filling(nv, tp);
-        pl.of_w = filling(nv, s.dim);
-        pl.of_q = s.T <= 32 ? kFlat : s.T > 128 && s.dim > 128 && count_of(kLarge, s.T, s.dim) * most >= kFull ? kLarge : kSmall;
+        pl.of_p = s.T <= 32 ? kNarrow : filling(s.bf16 || large_in_f32(s.dim), nv, tp);
+        pl.of_w = filling(s.bf16, nv, s.dim);
+        pl.of_q = s.T <= 32 ? kFlat : s.bf16 && s.T > 128 && s.dim > 128 && count_of(kLarge, s.T, s.dim) * most >= kFull ? kLarge : kSmall;
         const uint32_t tiles = (uint32_t)count_of((TileOf)pl.of_q, s.T, s.dim), resident = pl.of_q == kLarge ? 256 : pl.of_q == kSmall ? 512 : 1024;
         pl.parts = std::max(1u, std::min({resident / tiles, most, 256u}));
         pl.rest = c.take<float>(s.T);
@@ -469,7 +521,7 @@ int over(const Operand &W, uint32_t tail, F f) {
     return tail ? f(Tailed{W, W.rows, tail}) : f(W);
 }
 template <class G, class O>
-int forward_piece(const O &W, const Operand &Q, uint32_t steps, float scale2, uint32_t parts, uint32_t part0, float2 *stats, hipStream_t stream) {
+int forward_piece(const O &W, const Operand &Q, uint32_t steps, Scale2 scale2, uint32_t parts, uint32_t part0, float2 *stats, hipStream_t stream) {
     const uint32_t tiles = tiles_of(W.rows, G::BM);
     return launch<G>(xent_forward_kernel<G, O>, parts * tiles_of(Q.rows, G::BN), stream, W, Q, steps, scale2, tiles, (tiles + parts - 1) / parts, part0, stats);
 }
@@ -496,8 +548,8 @@ int forward(const Shape &s, const Plan &pl, const void *q_, const void *w_, cons
             W = Operand{(const char *)pl.w, (uint64_t)kp * es, nv};
         }
         const int rc = over(W, wd && s.dim != kp ? s.dim * es : 0, [&](const auto &O) {
-            auto go = [&](auto g) { return forward_piece<decltype(g)>(O, Q, steps, scale * kLog2e, pl.parts, parts, pl.stats, stream); };
-            return pl.fwd == kLarge ? go(Large<E>{}) : pl.fwd == kSmall ? go(Small<E>{}) : pl.fwd == kTiny ? go(Tiny<E>{}) : go(Narrow<E>{});
+            auto go = [&](auto g) { return forward_piece<decltype(g)>(O, Q, steps, Scale2::of(scale), pl.parts, parts, pl.stats, stream); };
+            return with_tile<E, Large<E>, Tiny<E>, Narrow<E>>(pl.fwd, go);
         });
         if (rc) return rc;
         parts += pl.parts;
@@ -561,7 +613,7 @@ int backward(const Shape &s, const Plan &pl, const void *q_, const void *w_, con
         void *p = dq || kTurned ? pl.p : nullptr, *pt = dw && !kTurned ? pl.pt : nullptr;
         int rc = over(W, wd && s.dim != kp ? s.dim * es : 0, [&](const auto &O) {
             auto go = [&](auto g) { return weights_of<decltype(g)>(O, v0, s.V, Q, steps, scale, targets, lse, grad_loss, p, vp, pt, tp, pl.rest, stream); };
-            return pl.of_p == kLarge ? go(Large<E>{}) : pl.of_p == kSmall ? go(Small<E>{}) : pl.of_p == kTiny ? go(Tiny<E>{}) : go(Narrow<E>{});
+            return with_tile<E, Large<E>, Tiny<E>, Narrow<E>>(pl.of_p, go);
         });
         if (rc) return rc;
         const uint32_t vsteps = vp / s.kstep();
@@ -569,7 +621,7 @@ int backward(const Shape &s, const Plan &pl, const void *q_, const void *w_, con
             const Operand P = gemm::panels(pl.p, tp);
             auto query_grad = [&](const auto &Wt) {
                 auto go = [&](auto g) { return query_grad_of<decltype(g)>(P, Wt, s.T, vsteps, pl.parts, v0 != 0, pl.dq, s.dim, stream); };
-                return pl.of_q == kLarge ? go(Large<E>{}) : pl.of_q == kSmall ? go(Small<E>{}) : go(Flat<E>{});
+                return with_tile<E, Long<E>, Flat<E>, Flat<E>>(pl.of_q, go);
             };
             if constexpr (kTurned) {
                 rc = query_grad(Turned{W.base, W.ld, 128, wd ? s.dim : kp, nv});
@@ -583,7 +635,7 @@ int backward(const Shape &s, const Plan &pl, const void *q_, const void *w_, con
             T *out = (T *)dw + (uint64_t)v0 * s.dim;
             auto table_grad = [&](const auto &Pt, const auto &Qt) {
                 auto go = [&](auto g) { return table_grad_of<decltype(g)>(Pt, Qt, tp / s.kstep(), an, v0, nv, out, s.dim, stream); };
-                return pl.of_w == kLarge ? go(Large<E>{}) : pl.of_w == kSmall ? go(Small<E>{}) : go(Tiny<E>{});
+                return with_tile<E, Long<E>, Tiny<E>, Tiny<E>>(pl.of_w, go);
             };
             if constexpr (kTurned) rc = table_grad(Turned{(const char *)pl.p, 128, tp * 128ull, vp, tp}, Turned{(const char *)pl.qt, (uint64_t)kp * es, 128, kp, tp});
             else rc = table_grad(gemm::panels(pl.pt, vp), gemm::panels(pl.qt, s.dim));
