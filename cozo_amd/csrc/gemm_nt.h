@@ -61,7 +61,7 @@ __device__ __forceinline__ uint32_t place_in_order() {
     return x * per + min(x, rest) + blockIdx.x / 8;
 }
 
-// rows of one operand as a workgroup sees them; rows past the last one are read as the last one (the epilogue drops them)
+// rows of one operand as a workgroup sees them, 16-byte aligned; rows past the last one are read as the last one (the epilogue drops them)
 struct Operand {
     const char *base;
     uint64_t ld;            // bytes from a row to the next
@@ -70,6 +70,12 @@ struct Operand {
 };
 // ordinary rows of `bytes` bytes (a multiple of 16), read where they are although a step ends behind them: it gets zeros there
 struct Tailed {
+    Operand rows_of;
+    uint32_t rows, bytes;
+};
+// rows of `bytes` bytes at any place: no 16 bytes of them need be aligned to more than an element T
+template <typename T>
+struct Ragged {
     Operand rows_of;
     uint32_t rows, bytes;
 };
@@ -94,6 +100,7 @@ struct Copies;
 template <int ROWS, int THREADS>
 struct Copies<Operand, ROWS, THREADS> {
     static constexpr int N = ROWS * 8 / THREADS;  // 16-byte pieces of a thread
+    static constexpr bool kHeld = false;           // copies go straight into LDS
     static constexpr int kReads = 1;               // LDS reads of a fragment
     static_assert(N * THREADS == ROWS * 8, "threads cover the copies");
     const char *src[N];
@@ -123,8 +130,44 @@ struct Copies<Tailed, ROWS, THREADS> : Copies<Operand, ROWS, THREADS> {
         return at < bytes ? this->src[i] + at : reinterpret_cast<const char *>(&kZeros);
     }
 };
+// Through registers: the copy into LDS asks for aligned dwords.  A step's loads are on their way while the step before it is worked on.  What
+// ends in a row's last step is read an element at a time, no further than the row.
+// (7 queries, 349365 rows of 1011 in f32: 322 us; packed into aligned rows first, 1315)
+template <typename T, int ROWS, int THREADS>
+struct Copies<Ragged<T>, ROWS, THREADS> : Copies<Operand, ROWS, THREADS> {
+    typedef Copies<Operand, ROWS, THREADS> Base;
+    static constexpr bool kHeld = true;
+    uint32_t bytes;
+    u32x4 held[Base::N];
+    __device__ __forceinline__ Copies(const Ragged<T> &o, uint32_t row0) : Base(o.rows_of, row0), bytes(o.bytes) {}
+    __device__ __forceinline__ void fetch(uint32_t step) {
+        if ((step + 1) * 128 <= bytes) {
+#pragma unroll
+            for (int i = 0; i < Base::N; i++) __builtin_memcpy(&held[i], this->src[i] + (step * 128 + this->piece(i)), 16);
+        } else {
+            constexpr uint32_t P = 16 / sizeof(T);
+            typedef T Piece __attribute__((ext_vector_type(P)));
+#pragma unroll
+            for (int i = 0; i < Base::N; i++) {
+                const uint32_t at = step * 128 + this->piece(i);
+                Piece x;
+#pragma unroll
+                for (uint32_t j = 0; j < P; j++) {
+                    x[j] = (T)0.f;
+                    if (at + j * sizeof(T) < bytes) x[j] = *(const T *)(this->src[i] + at + j * sizeof(T));
+                }
+                held[i] = __builtin_bit_cast(u32x4, x);
+            }
+        }
+    }
+    __device__ __forceinline__ void put(char *lds) const {
+#pragma unroll
+        for (int i = 0; i < Base::N; i++) *(u32x4 *)(lds + (i * THREADS + threadIdx.x) * 16) = held[i];
+    }
+};
 template <int ROWS, int THREADS>
 struct Copies<Turned, ROWS, THREADS> {
+    static constexpr bool kHeld = false;
     static constexpr int N = ROWS * 8 / THREADS, P = ROWS / 8;  // pieces of a thread, of a k
     static constexpr int kReads = 2;
     static_assert(N * THREADS == ROWS * 8, "threads cover the copies");
@@ -246,19 +289,25 @@ struct Tile {
     __device__ __forceinline__ void run(const OA &A, uint32_t m0, const OB &B, uint32_t n0, uint32_t s0, uint32_t steps, char *lds) {
         typedef Copies<OA, BM, kThreads> CA;
         typedef Copies<OB, BN, kThreads> CB;
-        const CA ca(A, m0);
+        CA ca(A, m0);
         const CB cb(B, n0);
         zero();
-        copy(ca, s0, lds);
         copy(cb, s0, lds + BM * 128);
+        if constexpr (CA::kHeld) {
+            ca.fetch(s0);
+            ca.put(lds);
+        } else copy(ca, s0, lds);
         for (uint32_t s = 0; s < steps; s++) {
             char *cur = lds + (s & 1) * kBytes, *nxt = lds + (~s & 1) * kBytes;
             arrived();
             if (s + 1 < steps) {
-                copy(ca, s0 + s + 1, nxt);
+                if constexpr (CA::kHeld) ca.fetch(s0 + s + 1);
+                else copy(ca, s0 + s + 1, nxt);
                 copy(cb, s0 + s + 1, nxt + BM * 128);
             }
             step<CA, CB>(cur);
+            if constexpr (CA::kHeld)
+                if (s + 1 < steps) ca.put(nxt);
         }
 #pragma unroll
         for (int c = 1; c < kChains; c++)

@@ -18,6 +18,7 @@
 using gemm::Bf16;
 using gemm::F32;
 using gemm::Operand;
+using gemm::Ragged;
 using gemm::Tailed;
 using gemm::Turned;
 
@@ -109,6 +110,9 @@ struct Scale2 {
     }
 };
 
+// From here on neighbouring f32 logits are 1 and more apart: what a product's rounding leaves of a difference can be any number.
+constexpr float kCoarse = 16777216.f;
+
 // A tile's products taken into the running maximum m and sum l of each of the lane's queries, to base 2.  The maximum is that of the products (the
 // least one where the scale is negative) and scaled once; a term is then two fused multiply-adds, an exponential and an addition, and no product
 // is rounded before the difference.  PART: only the first `left` rows exist.
@@ -121,7 +125,7 @@ __device__ __forceinline__ void take(const G &g, uint32_t left, Scale2 scale2, f
 #pragma unroll
     for (int j = 0; j < G::NT; j++) {
         float top = none;
-        if (least) {
+        if (__builtin_expect(least, 0)) {
 #pragma unroll
             for (int i = 0; i < G::MT; i++)
 #pragma unroll
@@ -135,13 +139,23 @@ __device__ __forceinline__ void take(const G &g, uint32_t left, Scale2 scale2, f
         top = fmaxf(m[j], top * scale2.high);
         const float ref = reference(top);
         float sum = m[j] == -__builtin_inff() ? l[j] : l[j] * exp2_(m[j] - ref);
+        if (__builtin_expect(!__any(!(fabsf(ref) < kCoarse)), 1)) {
 #pragma unroll
-        for (int i = 0; i < G::MT; i++)
+            for (int i = 0; i < G::MT; i++)
 #pragma unroll
-            for (int r = 0; r < 16; r++) {
-                const float e = exp2_(fmaf(g.acc[i][j][r], scale2.low, fmaf(g.acc[i][j][r], scale2.high, -ref)));
-                sum += !PART || is_there(i, r) ? e : 0.f;
-            }
+                for (int r = 0; r < 16; r++) {
+                    const float e = exp2_(fmaf(g.acc[i][j][r], scale2.low, fmaf(g.acc[i][j][r], scale2.high, -ref)));
+                    sum += !PART || is_there(i, r) ? e : 0.f;
+                }
+        } else {  // the largest term is to be 1 still
+#pragma unroll
+            for (int i = 0; i < G::MT; i++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const float e = exp2_(__fsub_rn(__fmul_rn(g.acc[i][j][r], scale2.high), ref));
+                    sum += !PART || is_there(i, r) ? e : 0.f;
+                }
+        }
         m[j] = top;
         l[j] = sum;
     }
@@ -150,7 +164,7 @@ __device__ __forceinline__ void take(const G &g, uint32_t left, Scale2 scale2, f
 template <class G, class O>
 __global__ void __launch_bounds__(G::kThreads)
 xent_forward_kernel(O W, Operand Q, uint32_t steps, Scale2 scale2, uint32_t n_tiles, uint32_t tiles_per_part,
-                    uint32_t part0, float2 *__restrict__ parts) {
+                    float2 *__restrict__ parts) {
     constexpr int BM = G::BM, BN = G::BN, WM = G::WM, WN = G::WN;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int lane = threadIdx.x & 63;
@@ -164,7 +178,7 @@ xent_forward_kernel(O W, Operand Q, uint32_t steps, Scale2 scale2, uint32_t n_ti
     for (uint32_t t = t0; t < t1; t++) {
         g.run(W, t * BM, Q, n0, 0, steps, lds);
         const uint32_t left = W.rows - t * BM;  // rows of this tile that exist
-        if (left >= BM) take<G, false>(g, left, scale2, m, l);
+        if (__builtin_expect(left >= BM, 1)) take<G, false>(g, left, scale2, m, l);
         else take<G, true>(g, left, scale2, m, l);
         __syncthreads();  // LDS is free for the next tile
     }
@@ -188,7 +202,7 @@ xent_forward_kernel(O W, Operand Q, uint32_t steps, Scale2 scale2, uint32_t n_ti
             a.y = (a.x == -__builtin_inff() ? a.y : a.y * exp2_(a.x - ref)) + (b.x == -__builtin_inff() ? b.y : b.y * exp2_(b.x - ref));
             a.x = top;
         }
-        parts[(uint64_t)(part0 + part) * Q.rows + n0 + c] = a;
+        parts[(uint64_t)part * Q.rows + n0 + c] = a;
     }
 }
 
@@ -246,6 +260,7 @@ xent_weights_kernel(O W, uint32_t v0, uint32_t V, Operand Q, uint32_t steps, flo
         const uint32_t y = t < Q.rows ? targets[t] : CZ_NONE;
         const bool on = t < Q.rows && has_answer(y, V);
         const float e = on ? lse[t] : 0.f, weight = on ? grad_loss[t] * scale : 0.f;
+        const float most = fabsf(e) < kCoarse ? __builtin_inff() : 0.f;  // of z - lse (NaN stays)
 #pragma unroll
         for (int i = 0; i < G::MT; i++)
 #pragma unroll
@@ -255,7 +270,8 @@ xent_weights_kernel(O W, uint32_t v0, uint32_t V, Operand Q, uint32_t steps, flo
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     // (to base 2 only after the difference: log2(e) lse and log2(e) scale, rounded, would be an error that a query's entries share)
-                    float x = exp2_(fmaf(g.acc[i][j][4 * r4 + r], scale, -e) * kLog2e);
+                    const float below = fmaf(g.acc[i][j][4 * r4 + r], scale, -e);
+                    float x = exp2_((below > most ? most : below) * kLog2e);
                     const bool hit = on && v0 + v + r == y;
                     if (hit) x -= 1.f;
                     x = on && v + r < W.rows ? x * weight : 0.f;
@@ -407,10 +423,10 @@ struct Shape {
 };
 
 struct Plan {
-    uint32_t piece;        // table rows worked on at a time
-    uint32_t parts;        // forward: stretches of a piece; backward: partial sums of grad_queries
+    uint32_t piece;        // backward: table rows worked on at a time
+    uint32_t parts;        // forward: stretches of the table; backward: partial sums of grad_queries
     int fwd, of_p, of_w, of_q;  // tiles (TileOf): forward's; backward's of P, of grad_table, of grad_queries
-    void *q, *w;           // packed copies (unaligned rows or a dim that is no multiple of a step)
+    void *q, *w;           // packed copies: of queries that are unaligned or no whole steps wide; of a piece of an unaligned bf16 table (gradient)
     void *qt, *wt, *p, *pt;  // (bf16: qt is a copy of the queries without those that have no answer, wt and pt are not needed)
     float2 *stats;
     float *dq, *rest;
@@ -464,18 +480,17 @@ Plan make_plan(const Shape &s, bool grad, void *ws) {
     pl.piece = (uint32_t)std::min<uint64_t>(up_to(s.V, 256), std::max<uint64_t>(1024, budget / per_row / 1024 * 1024));
     cz::Carve c(ws);
     pl.q = c.take<uint8_t>((uint64_t)s.T * kp * es);
-    pl.w = c.take<uint8_t>((uint64_t)pl.piece * kp * es);
     if (!grad) {
-        // a table that can be read where it is goes in one piece, another one packed piece by piece: stretches for the larger
         pl.fwd = s.T <= 32 ? kNarrow : filling(s.bf16 || large_in_f32(s.dim), s.V, s.T);
         const TileOf f = (TileOf)pl.fwd;
         const uint32_t qt = tiles_of(s.T, cols_of(f)), tiles = tiles_of(s.V, rows_of(f));
         const uint32_t resident = f == kLarge ? 256 : f == kSmall ? 512 : 1024;
         pl.parts = std::max(1u, std::min(tiles, resident / qt));
-        pl.stats = c.take<float2>((uint64_t)pl.parts * ((s.V + pl.piece - 1) / pl.piece) * s.T);
+        pl.stats = c.take<float2>((uint64_t)pl.parts * s.T);
     } else {
         pl.qt = c.take<uint8_t>(kp * tp * es);
         pl.p = c.take<uint8_t>(tp * pl.piece * es);
+        if (s.bf16) pl.w = c.take<uint8_t>((uint64_t)pl.piece * kp * es);
         if (!s.bf16) {
             pl.wt = c.take<uint8_t>((uint64_t)s.dim * pl.piece * es);
             pl.pt = c.take<uint8_t>(pl.piece * tp * es);
@@ -515,15 +530,17 @@ int launch(K kernel, uint32_t grid, hipStream_t stream, A... args) {
     hipLaunchKernelGGL(kernel, dim3(grid), dim3(G::kThreads), G::kLds, stream, args...);
     return CZ_OK;
 }
-// f over W as it is, or (tail: bytes of a row that ends inside a step) with zeros behind its rows
-template <class F>
-int over(const Operand &W, uint32_t tail, F f) {
-    return tail ? f(Tailed{W, W.rows, tail}) : f(W);
+// f over W's rows of dim elements where they are: as they are, with zeros behind rows that end inside a step, or element by element aligned
+template <typename T, class F>
+int over(const Operand &W, uint32_t dim, bool aligned, F f) {
+    const uint32_t bytes = dim * sizeof(T);
+    if (!aligned) return f(Ragged<T>{W, W.rows, bytes});
+    return bytes % 128 ? f(Tailed{W, W.rows, bytes}) : f(W);
 }
 template <class G, class O>
-int forward_piece(const O &W, const Operand &Q, uint32_t steps, Scale2 scale2, uint32_t parts, uint32_t part0, float2 *stats, hipStream_t stream) {
+int forward_over(const O &W, const Operand &Q, uint32_t steps, Scale2 scale2, uint32_t parts, float2 *stats, hipStream_t stream) {
     const uint32_t tiles = tiles_of(W.rows, G::BM);
-    return launch<G>(xent_forward_kernel<G, O>, parts * tiles_of(Q.rows, G::BN), stream, W, Q, steps, scale2, tiles, (tiles + parts - 1) / parts, part0, stats);
+    return launch<G>(xent_forward_kernel<G, O>, parts * tiles_of(Q.rows, G::BN), stream, W, Q, steps, scale2, tiles, (tiles + parts - 1) / parts, stats);
 }
 
 template <class E>
@@ -537,24 +554,13 @@ int forward(const Shape &s, const Plan &pl, const void *q_, const void *w_, cons
         pack(q, s.ldq, s.T, s.dim, pl.q, kp, stream);
         Q = Operand{(const char *)pl.q, (uint64_t)kp * es, s.T};
     }
-    const bool wd = direct(w, s.ldw, s.dim, es);
-    const uint32_t piece = wd ? s.V : pl.piece;
-    uint32_t parts = 0;
-    for (uint32_t v0 = 0; v0 < s.V; v0 += piece) {
-        const uint32_t nv = std::min(piece, s.V - v0);
-        Operand W{(const char *)(w + v0 * s.ldw), s.ldw * es, nv};
-        if (!wd) {
-            pack(w + v0 * s.ldw, s.ldw, nv, s.dim, pl.w, kp, stream);
-            W = Operand{(const char *)pl.w, (uint64_t)kp * es, nv};
-        }
-        const int rc = over(W, wd && s.dim != kp ? s.dim * es : 0, [&](const auto &O) {
-            auto go = [&](auto g) { return forward_piece<decltype(g)>(O, Q, steps, Scale2::of(scale), pl.parts, parts, pl.stats, stream); };
-            return with_tile<E, Large<E>, Tiny<E>, Narrow<E>>(pl.fwd, go);
-        });
-        if (rc) return rc;
-        parts += pl.parts;
-    }
-    hipLaunchKernelGGL(xent_join_kernel<T>, dim3((s.T + 3) / 4), dim3(256), 0, stream, pl.stats, parts, q, s.ldq, w, s.ldw, s.T, s.V, s.dim,
+    const Operand W{(const char *)w, s.ldw * es, s.V};
+    const int rc = over<T>(W, s.dim, direct(w, s.ldw, s.dim, es), [&](const auto &O) {
+        auto go = [&](auto g) { return forward_over<decltype(g)>(O, Q, steps, Scale2::of(scale), pl.parts, pl.stats, stream); };
+        return with_tile<E, Large<E>, Tiny<E>, Narrow<E>>(pl.fwd, go);
+    });
+    if (rc) return rc;
+    hipLaunchKernelGGL(xent_join_kernel<T>, dim3((s.T + 3) / 4), dim3(256), 0, stream, pl.stats, pl.parts, q, s.ldq, w, s.ldw, s.T, s.V, s.dim,
                        targets, scale, loss, lse);
     return launched("cz_softmax_xent");
 }
@@ -606,12 +612,13 @@ int backward(const Shape &s, const Plan &pl, const void *q_, const void *w_, con
         const uint32_t nv = std::min(pl.piece, s.V - v0), vp = (uint32_t)up_to(nv, 256);
         const T *wv = w + v0 * s.ldw;
         Operand W{(const char *)wv, s.ldw * es, nv};
-        if (!wd) {
+        const bool packed = kTurned && !wd;  // (to be read turned, rows of 8 have to be aligned)
+        if (packed) {
             pack(wv, s.ldw, nv, s.dim, pl.w, kp, stream);
             W = Operand{(const char *)pl.w, (uint64_t)kp * es, nv};
         }
         void *p = dq || kTurned ? pl.p : nullptr, *pt = dw && !kTurned ? pl.pt : nullptr;
-        int rc = over(W, wd && s.dim != kp ? s.dim * es : 0, [&](const auto &O) {
+        int rc = over<T>(W, packed ? kp : s.dim, wd || packed, [&](const auto &O) {
             auto go = [&](auto g) { return weights_of<decltype(g)>(O, v0, s.V, Q, steps, scale, targets, lse, grad_loss, p, vp, pt, tp, pl.rest, stream); };
             return with_tile<E, Large<E>, Tiny<E>, Narrow<E>>(pl.of_p, go);
         });

@@ -332,6 +332,8 @@ int cz_q4_knn(int metric, const uint8_t *codes, const uint16_t *scales, const fl
  * otherwise treated like CZ_NONE (host pointers: CZ_E_INVALID).
  *   queries [T] rows of `dim` elements, ldq apart; table [V] rows, ldw apart; both of type `elem`; 1 <= dim <= 8192, V >= 1.
  * Products and sums are f32 (f32 products stay f32; bf16 products are exact).
+ * Logits of 2^24 and more have no fraction in f32: lse is as exact as they are, but which weights exp(z - lse) become 1 and which 0 is
+ * then up to rounding (none is larger than 1).
  *   grad:  G[t][v] = grad_loss[t] * (exp(z[t][v] - lse[t]) - [v = targets[t]]);   grad_queries = scale * G . table,
  *          grad_table = scale * G^T . queries   (contiguous [T][dim] / [V][dim] of type `elem`, each written whole; either may be
  *          NULL).  For bf16, G is rounded to bf16 before the two products.  grad_loss [T] f32; lse as the forward call gave it.

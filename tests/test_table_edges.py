@@ -311,3 +311,31 @@ def test_rows_that_end_inside_a_step(gpu_lib, dtype, dim, T):
     y3 = torch.where(y2 > 200, y2 - 1, y2)
     a, b = _run(tq2, tw2, y2, cuda(g), 1.0)[:2], _run(tq2, rest, y3, cuda(g), 1.0)[:2]
     assert all(bool(((x - z).abs() <= 1e-4 + 1e-6 * z.abs()).all()) for x, z in zip(a, b))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_logits_without_fractions(gpu_lib, dtype, sign):
+    """logits of 1e9 to 1e36, all of one query's alike or nearly so: lse stays as exact as f32 logits are, weights stay within 0 and 1"""
+    import torch
+    from cozo_amd.softmax import softmax_xent, softmax_xent_grad
+    T, V, dim = 5, 700, 40
+    g = torch.Generator().manual_seed(3)
+    q = torch.rand(T, dim, generator=g).add_(0.5) * torch.tensor([1e9, 3e10, 1e15, 1e30, 1e34])[:, None]
+    w = sign * (1.0 + 1e-3 * torch.rand(V, dim, generator=g))
+    w[300:] = w[7]
+    q, w = (a.cuda() if dtype == "f32" else _bf16(a).cuda() for a in (q, w))
+    y = torch.arange(T, dtype=torch.int32, device="cuda")
+    loss, lse = softmax_xent(q, w, y)
+    z = q.double().cpu() @ w.double().cpu().T
+    # a product's f32 additions (dim of them), to base 2 and back, the sum (at most log V, far below an ulp of such a logit), the result's rounding
+    tol = (dim + 4) * 2.0**-24 * (q.double().cpu().abs() @ w.double().cpu().abs().T).amax(1) + np.log(V)
+    assert bool(((lse.double().cpu() - torch.logsumexp(z, 1)).abs() <= tol).all())
+    assert bool(loss.isfinite().all())
+    gl = torch.full((T,), 0.25, device="cuda")
+    dq, dw = softmax_xent_grad(q, w, y, lse, gl)
+    assert bool(dq.isfinite().all()) and bool(dw.isfinite().all())
+    # |G| <= 0.25: a row's gradient is at most that share of all queries, whatever the rounding (of G, of the sum, of the result)
+    most = 0.25 * q.double().cpu().abs().sum(0)
+    assert bool((dw.double().cpu().abs() <= most * (1 + (2.0**-6 if dtype == "bf16" else 2.0**-20))).all())
