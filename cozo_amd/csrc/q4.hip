@@ -1198,8 +1198,9 @@ int launch_product(const Rows &t, const ProductPlan &p, const float *q, uint32_t
     return launch_product_ct<1, NEAR>(t, p, B, out, near, stream);
 }
 
-// Work (queries x rows x dim) from which scores come first.  The f64 distances of all rows run at some 2e12 elements a second, the scores' launches
-// take 30 us whatever they do; 644 x 18221 x 312: 1928 us without scores, 180 with them
+// Saved work (queries x rows x dim) from which scores come first.  Some k of the tiles stay to be looked at.  The f64 distances of all rows run at some 2e12 elements a second, the scores' launches
+// take 30 us whatever they do; 644 x 18221 x 312: 1928 us without scores, 180 with them (k = 11, 285
+// tiles); 569 x 11596 x 584, k = 51, 182 tiles: 1489 and 516
 constexpr double kFilterFrom = 6e7;
 // Up to so many queries the digits' product (100 us for each 16 of them at 1M x 768) is the faster way to the scores; at 48 both take 0.37 ms.
 constexpr uint32_t kDigitQueries = 32;
@@ -1236,7 +1237,7 @@ struct KnnPlan {
 KnnPlan knn_plan(const Rows &t, uint32_t B, uint32_t k, void *ws) {
     KnnPlan p{};
     const uint32_t n_tiles = (uint32_t)(((uint64_t)t.n + kTile - 1) / kTile);
-    p.filtered = n_tiles >= 4 * (uint64_t)k && (double)B * t.n * t.dim >= kFilterFrom;
+    p.filtered = n_tiles > k && (double)B * t.n * t.dim * (n_tiles - k) / n_tiles >= kFilterFrom;
     // enough workgroups to fill the chip, few enough lists to join
     uint32_t chunks = std::min(n_tiles, std::max(1u, (p.filtered ? 512 : 2048) / B));
     if (p.filtered && B > 256) chunks = 2;

@@ -339,3 +339,15 @@ def test_logits_without_fractions(gpu_lib, dtype, sign):
     # |G| <= 0.25: a row's gradient is at most that share of all queries, whatever the rounding (of G, of the sum, of the result)
     most = 0.25 * q.double().cpu().abs().sum(0)
     assert bool((dw.double().cpu().abs() <= most * (1 + (2.0**-6 if dtype == "bf16" else 2.0**-20))).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("metric", METRICS)
+@pytest.mark.parametrize("B,dim,k", [(500, 512, 50), (30, 4096, 45), (500, 512, 57)])
+def test_hardly_more_tiles_than_results(gpu_lib, metric, B, dim, k):
+    """58 tiles of 64 rows: scores say which of them can hold one of k results although there are few, or nearly none, to leave out"""
+    n = 57 * 64 + 3
+    codes, scales, sq, x = _table(n, dim, 64, k)
+    q = np.random.default_rng(B).standard_normal((B, dim)).astype(np.float32)
+    q[3] = x[n - 1]
+    _check_knn(_gpu_table(codes, scales, sq, dim), q, x, k, metric, only=np.arange(0, B, 17 if B > 100 else 1))
