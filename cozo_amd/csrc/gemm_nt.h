@@ -79,15 +79,15 @@ struct Ragged {
     Operand rows_of;
     uint32_t rows, bytes;
 };
-// k in panels: a step's 128 bytes of every row lie one behind the other, so that a workgroup's step is one run of memory; in rows of 128 KB each
-// row of a step begins in the same few memory channels (grad_queries of a 65536-row piece: 179 us, with padded rows 168, in panels 164)
-// the same for an operand of a 16-bit type that lies turned: for each k the rows one behind the other
+// an operand of a 16-bit type that lies turned: for each k the rows one behind the other
 struct Turned {
     const char *base;
     uint64_t ld;            // bytes from a k to the next
     uint64_t panel;         // bytes from 64 rows to the next 64: 128 where a k's rows are one run
     uint32_t rows, ks;      // rows: a multiple of 8, 16-byte aligned; a k past the last one is read as the last one (times zeros of the other side)
 };
+// k in panels: a step's 128 bytes of every row lie one behind the other, so that a workgroup's step is one run of memory; in rows of 128 KB each
+// row of a step begins in the same few memory channels (grad_queries of a 65536-row piece: 179 us, with padded rows 168, in panels 164)
 inline Operand panels(const void *base, uint32_t rows) { return Operand{(const char *)base, 128, rows, (uint64_t)rows * 128}; }
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
