@@ -571,7 +571,9 @@ q4_scores_kernel(Rows t, gemm::Operand Q, const int *__restrict__ exponent, uint
             rowf[mine] = f;
         }
         auto store = [&](char *to) {  // the loaded 32 elements as f16, at their places of the operand's row
-            const _Float16 s = (_Float16)(bf16_to_f32(sb) * down);
+            // (a group with a code that counts has a scale of at most the row's norm, 2^8 here; that of a group of zeros, which the norm does not
+            // bound, is cut, so that none of its 16 codes, the padding's among them, makes an infinity that a zero would turn into NaN)
+            const _Float16 s = (_Float16)fminf(bf16_to_f32(sb) * down, 4096.f);
             const f16x2 s2 = {finite ? s : (_Float16)0.f, finite ? s : (_Float16)0.f}, off = {(_Float16)1032.f, (_Float16)1032.f};
 #pragma unroll
             for (int d = 0; d < 4; d++) {
