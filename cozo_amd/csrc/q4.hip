@@ -174,13 +174,23 @@ q4_dequantize_kernel(Rows t, const uint32_t *__restrict__ rows, uint32_t m, bool
 // a query becomes integers too: fixed point with 31 bits below its largest element, cut into four balanced 8-bit digits.
 //   v_mfma_i32_16x16x64_i8:  A (16 rows) = 4 queries x 4 digits,  B (16 columns) = 16 table rows,  64 elements at a time.
 // Sums within a group are exact.  Lane l of the result holds the four digits of query l / 16 for table row l % 16: they are joined in
-// the lane (two integer shifts-and-adds, two conversions, one fma) and added to one f32 accumulator with the lane's own row's scale.
+// the lane (two integer shifts-and-adds, two conversions, one fma), put into the sums' unit (a power of two, one multiplication) and added to
+// one f32 accumulator with the lane's own row's scale.
 // Rounding: 2^-31 of the query's largest element, and f32 sums over the groups.
 // HBM bound up to about 16 queries: per 512 bytes of codes (16 rows x 64 elements) a wave issues 14 vector instructions and one matrix
 // instruction for each 4 queries.
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kNotFinite = -100000;  // exponent of a query that holds a NaN or an infinity
+
+// The products of a query whose elements are below 2^e are summed in units of 2^(e - sum_exponent(e)):
+//   e >= 0           2^17: a sum leaves the f32 range only 2^17 beyond the largest result
+//   -17 < e < 0      2^(e + 17)
+//   -90 <= e <= -17  1, the result's own
+//   e < -90          2^(e + 90), so that the factor that brings a joined sum to its unit stays a normal number
+// Below e = 0 no sum leaves the range: 8192 elements of 8 times the largest scale are 2^144, times 2^e.  What is lost below the range is at most
+// 2^-133 of the result for each group.
+__device__ __forceinline__ int sum_exponent(int e) { return e >= 0 ? e - 17 : max(min(e, -17), -90); }
 
 // The element (of a step's 64) that byte j of lane l's 16 bytes stands for.  A lane loads 16 bytes of codes, 32 consecutive elements; lanes
 // 0-31 hold a step's 64, lanes 32-63 the next step's, and a swap of half registers gives every lane 16 of either: the first or the second
@@ -291,7 +301,10 @@ struct Product {
     __device__ __forceinline__ static i32x4 unpack(uint32_t w0, uint32_t w1) {
         return i32x4{(int)((w0 << 4) & 0xF0F0F0F0u), (int)(w0 & 0xF0F0F0F0u), (int)((w1 << 4) & 0xF0F0F0F0u), (int)(w1 & 0xF0F0F0F0u)};
     }
-    __device__ __forceinline__ void work(const Batch &x, const u32x4 *lds, uint32_t k, uint32_t steps) {
+    // UNIT: joined sums are multiplied by the query's unit[c] first
+    template <bool UNIT>
+    __device__ __forceinline__ void work(const Batch &x, const u32x4 *lds, uint32_t k, uint32_t steps, const float (&unit)[CT]) {
+        auto add = [&](int i, int c, const i32x4 &d, float s) { acc[i][c] = fmaf(UNIT ? join(d) * unit[c] : join(d), s, acc[i][c]); };
         const int lane = threadIdx.x & 63;
         i32x4 open[RT][CT];  // (a group of 128 is two steps of one batch)
 #pragma unroll
@@ -315,20 +328,20 @@ struct Product {
                     for (int i = 0; i < RT; i++) {
                         const i32x4 d0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(a0, b[i], none, 0, 0, 0);
                         const i32x4 d1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(a1, b[i], none, 0, 0, 0);
-                        acc[i][c] = fmaf(join(d0), scale(x, i, 2 * u), acc[i][c]);
-                        acc[i][c] = fmaf(join(d1), scale(x, i, 2 * u + 1), acc[i][c]);
+                        add(i, c, d0, scale(x, i, 2 * u));
+                        add(i, c, d1, scale(x, i, 2 * u + 1));
                     }
                 } else if constexpr (GS == 6) {
 #pragma unroll
                     for (int i = 0; i < RT; i++) {
                         const i32x4 d = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b[i], none, 0, 0, 0);
-                        acc[i][c] = fmaf(join(d), scale(x, i, u), acc[i][c]);
+                        add(i, c, d, scale(x, i, u));
                     }
                 } else {
 #pragma unroll
                     for (int i = 0; i < RT; i++) {
                         open[i][c] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b[i], (u & 1) ? open[i][c] : none, 0, 0, 0);
-                        if (u & 1) acc[i][c] = fmaf(join(open[i][c]), scale(x, i, u / 2), acc[i][c]);
+                        if (u & 1) add(i, c, open[i][c], scale(x, i, u / 2));
                     }
                 }
             }
@@ -391,12 +404,16 @@ q4_product_kernel(Rows t, const u32x4 *__restrict__ digits, const int *__restric
         const uint32_t c = c0 + i / (steps * 64);
         lds[i] = c < blocks4 ? digits[(uint64_t)c0 * steps * 64 + i] : u32x4{0, 0, 0, 0};
     }
-    int ex[CT];
-    float best[CT], qn[CT];
+    int ex[CT];  // of a sum's unit
+    float best[CT], qn[CT], unit[CT];
 #pragma unroll
     for (int c = 0; c < CT; c++) {
         const uint32_t b = (c0 + c) * 4 + (lane >> 4);
-        ex[c] = b < B ? exponent[b] : 0;
+        const int e = b < B ? exponent[b] : 0;
+        // a joined sum is in units of 2^(e - 34): the fixed point's 30 bits and the codes' 4.  The search keeps that (a score beyond the
+        // range says nothing, and its tile is looked at)
+        ex[c] = e == kNotFinite ? e : NEAR ? e - 34 : e - sum_exponent(e);
+        unit[c] = NEAR || e == kNotFinite ? 1.f : ldexpf(1.f, sum_exponent(e) - 34);
         best[c] = -__builtin_inff();
         qn[c] = NEAR && b < B ? near.qnorm[b] : 0.f;
     }
@@ -415,7 +432,7 @@ q4_product_kernel(Rows t, const u32x4 *__restrict__ digits, const int *__restric
             const bool more = k + P::KU < steps;
             const uint64_t nt = more ? tile : tile + stride;
             if (nt < n_tiles) P::load(nxt, t, nt * kTile, more ? k + P::KU : 0);
-            p.work(cur, lds, k, steps);
+            p.template work<!NEAR>(cur, lds, k, steps, unit);
             cur = nxt;
         }
         float sq[RT], xn = 0.f;
@@ -437,7 +454,7 @@ q4_product_kernel(Rows t, const u32x4 *__restrict__ digits, const int *__restric
 #pragma unroll
             for (int i = 0; i < RT; i++) {
                 const uint64_t r = tile * kTile + 16 * i + col;
-                const float v = ex[c] == kNotFinite ? __builtin_nanf("") : ldexpf(p.acc[i][c], ex[c] - 34);
+                const float v = ex[c] == kNotFinite ? __builtin_nanf("") : ldexpf(p.acc[i][c], ex[c]);
                 if constexpr (NEAR) {
                     if (r < t.n) top = fmaxf(top, score_of(near.metric, v, sq[i]));
                 } else {

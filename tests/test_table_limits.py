@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 from tests import table_ref as R
-from tests.test_quantized import METRICS, _check_knn, _gpu_table
+from tests.test_quantized import METRICS, U32, _check_knn, _cuda, _gpu_table, _table
 
 
 # ---- scores of a large batch ---------------------------------------------------------------------------------------
@@ -40,3 +40,60 @@ def test_groups_of_zeros_with_large_scales(gpu_lib, metric, B):
     for k in (1, 5, 20):
         ids, _ = _check_knn(t, q, x, k, metric, only=look)
         assert np.isin(ids[:, :min(k, 5)], at).all()
+
+
+# ---- products ------------------------------------------------------------------------------------------------------
+def _dots_bound(q, x, group):
+    """|q| |x|: a group's sum is joined with two roundings and added with one, to partial sums of at most that; the fixed point is off by
+    2^-31 of twice the query's largest element; one rounding of the result; 2^-132 for each group where sums leave the f32 range"""
+    groups = -(-x.shape[1] // group)
+    a = np.abs(q.astype(np.float64)) @ np.abs(x).T
+    return 1.01 * ((groups + 4) * U32 * a + 2.0 ** -30 * np.abs(q).max(1).astype(np.float64)[:, None] * np.abs(x).sum(1)[None, :]) + groups * 2.0 ** -132
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("B", [1, 6, 20])
+def test_products_across_the_range(gpu_lib, group, B):
+    """rows from 1e-30 to 1e36 with queries from 1e-44 to 1e30: whatever is finite comes back, with the same relative error"""
+    n, dim = 200, 768
+    codes, scales, sq, x = _table(n, dim, group, B)
+    s = R.bf16_value(scales).astype(np.float64)
+    s *= (10.0 ** np.linspace(-30, 34, n))[:, None]
+    scales = R.bf16_bits(s.astype(np.float32))
+    x = R.decode(codes, R.bf16_value(scales), dim)
+    t = _gpu_table(codes, scales, sq, dim)
+    rng = np.random.default_rng(group)
+    for size in (1e-44, 1e-40, 1e-30, 1e-20, 1e-10, 1e-5, 1.0, 1e5, 1e20, 1e30):
+        q = rng.standard_normal((B, dim)) * size
+        q = q.astype(np.float32)
+        want = q.astype(np.float64) @ x.T
+        # partial sums within the range: a large sum of terms of both signs is a plain f32 sum's own limit
+        fits = np.abs(q.astype(np.float64)) @ np.abs(x).T < 3e38
+        got = t.dots(_cuda(q)).cpu().numpy()
+        assert fits[:, :100].any() and np.isfinite(got[fits]).all(), size
+        err = np.abs(got.astype(np.float64) - want)
+        assert np.all((err <= _dots_bound(q, x, group))[fits]), size
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B", [1, 20])
+def test_products_that_cancel(gpu_lib, B):
+    """partial sums beyond the f32 range whose total is not; the largest rows there are, with small queries"""
+    dim, group = 1024, 32
+    c = np.full((40, dim), 7)
+    c[:, dim // 2:] = -7
+    c[:, 0] = 6
+    s = np.full((40, dim // group), 2.0 ** 122)  # 512 elements of 3.7e37 each, then as many of the other sign
+    codes, scales = R.pack(c), R.bf16_bits(s.astype(np.float32))
+    x = R.decode(codes, s, dim)
+    sq = np.zeros(40, np.float32)
+    t = _gpu_table(codes, scales, sq, dim)
+    for size in (1.0, 0.75, 1e-3, 1e-20):
+        q = np.full((B, dim), size, np.float32)
+        got = t.dots(_cuda(q)).cpu().numpy()
+        want = q.astype(np.float64) @ x.T
+        assert np.all(np.abs(got - want) <= _dots_bound(q, x, group)), size
+    top = R.bf16_bits(np.full((40, dim // group), 2.0 ** 127, np.float32))
+    got = _gpu_table(R.pack(np.full((40, dim), 7)), top, sq, dim).dots(_cuda(np.full((B, dim), 1e-10, np.float32))).cpu().numpy()
+    assert np.allclose(got, dim * 7 * 2.0 ** 127 * np.float64(np.float32(1e-10)), rtol=1e-5)
