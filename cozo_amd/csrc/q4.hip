@@ -375,6 +375,12 @@ __device__ __forceinline__ float sure_score(int metric, float c, float qnorm, fl
     return top < __builtin_inff() ? top - score_error(metric, c, qnorm, xnorm) : -__builtin_inff();
 }
 
+// Products of these norms, or what a score makes of them, may pass the f32 range: no score then says anything (one that was to be near may have
+// become minus infinity).  A cosine's score is at most the query's norm.
+__device__ __forceinline__ bool may_overflow(int metric, float qnorm, float xnorm) {
+    return metric != CZ_COSINE && !((metric == CZ_L2 ? fmaf(2.f, qnorm, xnorm) : qnorm) * xnorm < 0x1p126f);
+}
+
 struct Near {              // what the search takes from the product kernels instead of the products
     int metric;
     const float *sqnorms;
@@ -654,7 +660,8 @@ q4_scores_kernel(Rows t, gemm::Operand Q, const int *__restrict__ exponent, uint
 #pragma unroll
             for (int j = 0; j < G::NT; j++) {
                 const uint32_t b = n0 + G::wave_col() + j * 32 + (lane & 31);
-                const float v = fmaxf(top[j][x], __shfl_xor(top[j][x], 32, 64));
+                float v = fmaxf(top[j][x], __shfl_xor(top[j][x], 32, 64));
+                if (may_overflow(near.metric, qn[j], xn)) v = __builtin_inff();
                 if (b < Q.rows && lane < 32) score[(uint64_t)tile * ldb + b] = v;
                 best[j] = fmaxf(best[j], sure_score(near.metric, near.err, qn[j], xn, v));
             }

@@ -42,6 +42,38 @@ def test_groups_of_zeros_with_large_scales(gpu_lib, metric, B):
         assert np.isin(ids[:, :min(k, 5)], at).all()
 
 
+@pytest.mark.gpu
+def test_scores_beyond_the_range(gpu_lib):
+    """products around -2^128, where the f16 score of the nearer of two rows overflows and that of the farther one does not: the query's first
+    half is rounded down by its f16 form and the second half up, by half a step each"""
+    n, half = 33000, 2.0 ** -11
+    q1 = np.concatenate([np.full(32, 1 + half), np.full(32, 1 + 3 * half)])
+
+    def row(total, scale, first):
+        """32 codes that sum to -total, in the first or the second half, and a scale that puts their sum into [2^57, 2^58)"""
+        c, part = np.zeros(64, np.int64), np.full(32, total // 32)
+        part[:total % 32] += 1
+        c[:32 if first else None][-32:] = -part
+        return c, scale * 2.0 ** (57 - np.floor(np.log2(total * scale)))
+    c = np.full((n, 64), -7)
+    s = np.full((n, 2), 0.8125 * 2.0 ** 50)  # the others: no longer than the two, products of -1.4 times theirs
+    near, far = 6000, 20000
+    for at, (total, scale, first) in ((near, (155, 211, False)), (far, (137, 239, True))):
+        c[at], v = row(total, scale, first)
+        s[at] = v
+    scales = R.bf16_bits(s.astype(np.float32))
+    assert np.array_equal(R.bf16_value(scales), s)
+    codes = R.pack(c)
+    x = R.decode(codes, s, 64)
+    q = np.tile(q1 * 2.0 ** 70, (40, 1)).astype(np.float32)
+    assert np.array_equal(q[0], q1 * 2.0 ** 70)
+    t = _gpu_table(codes, scales, (x ** 2).sum(1).astype(np.float32), 64)
+    ids, _ = _check_knn(t, q, x, 1, "IP")
+    assert (ids == near).all()
+    _check_knn(t, q, x, 3, "IP", only=[0, 39])
+    _check_knn(t, q, x, 2, "L2", only=[0, 39])
+
+
 # ---- products ------------------------------------------------------------------------------------------------------
 def _dots_bound(q, x, group):
     """|q| |x|: a group's sum is joined with two roundings and added with one, to partial sums of at most that; the fixed point is off by
