@@ -181,6 +181,11 @@ q4_dequantize_kernel(Rows t, const uint32_t *__restrict__ rows, uint32_t m, bool
 // instruction for each 4 queries.
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
+// A query whose norm's square is below this has no score (its norm is given as NaN, and every row is looked at in f64): products with rows of 1e-15,
+// the smallest whose cosine has one, would fall under the f32 range's lower end and be off by more than the score's bound says (2^-150 / 1e-15
+// to 2^-20 of a norm of 2^-80).
+constexpr double kLeastSquare = 0x1p-160;
+
 constexpr int kNotFinite = -100000;  // exponent of a query that holds a NaN or an infinity
 
 // The products of a query whose elements are below 2^e are summed in units of 2^(e - sum_exponent(e)):
@@ -230,7 +235,7 @@ q4_digits_kernel(const float *__restrict__ q, uint32_t B, uint32_t dim, uint32_t
         else if (m > 0.f) (void)frexpf(m, &e);
         if (lane == 0 && b < B) {
             exponent[b] = e;
-            if (norm) norm[b] = e == kNotFinite ? __builtin_nanf("") : __double2float_ru(sqrt(s2));
+            if (norm) norm[b] = e == kNotFinite || s2 < kLeastSquare ? __builtin_nanf("") : __double2float_ru(sqrt(s2));
         }
         const bool on = b < B && e != kNotFinite;
         for (uint32_t i = lane; i < width; i += 64) {
@@ -506,10 +511,10 @@ q4_halves_kernel(const float *__restrict__ q, uint32_t B, uint32_t dim, uint32_t
     double s2 = 0.0;
     for (uint32_t i = lane; i < dim; i += 64) s2 = fma((double)row[i], (double)row[i], s2);
     for (int o = 32; o; o >>= 1) s2 += __shfl_xor(s2, o, 64);
-    // (beyond 2^96, an infinity or NaN among it: no score, every row is looked at)
-    const bool fine = s2 < 0x1p192;
+    // (beyond 2^96, an infinity or NaN among it: no score either)
+    const bool fine = s2 >= kLeastSquare && s2 < 0x1p192;
     int e = 0;
-    if (fine && s2 > 0.0) {
+    if (fine) {
         (void)frexp(s2, &e);
         e = ((e + 1) >> 1) - 8;  // norm < 2^(e + 8)
     }

@@ -74,6 +74,28 @@ def test_scores_beyond_the_range(gpu_lib):
     _check_knn(t, q, x, 2, "L2", only=[0, 39])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("metric", METRICS)
+@pytest.mark.parametrize("B", [30, 40])
+@pytest.mark.parametrize("size", [1e-25, 1e-30, 1e-38, 1e-43])
+def test_tiny_queries(gpu_lib, metric, B, size):
+    """queries so small that their products with small rows are below the f32 range, the nearest row among the small ones"""
+    n, dim = 33000, 72
+    codes, scales, _, x = _table(n, dim, 32, B)
+    s = R.bf16_value(scales).astype(np.float64)
+    s[6400:6464] *= 1.03e-15 / np.linalg.norm(x[6400:6464], axis=1)[:, None]  # (all of a tile)
+    scales = R.bf16_bits(s.astype(np.float32))
+    x = R.decode(codes, R.bf16_value(scales), dim)
+    rng = np.random.default_rng(B)
+    d = rng.standard_normal((B, dim))
+    a = x[6400 + np.arange(B)] / np.linalg.norm(x[6400 + np.arange(B)], axis=1)[:, None]
+    d -= (d * a).sum(1)[:, None] * a
+    q = ((0.6 * a + 0.8 * d / np.linalg.norm(d, axis=1)[:, None]) * size).astype(np.float32)
+    t = _gpu_table(codes, scales, (x ** 2).sum(1).astype(np.float32), dim)
+    for k in (1, 7):
+        _check_knn(t, q, x, k, metric, only=np.arange(0, B, 4))
+
+
 # ---- products ------------------------------------------------------------------------------------------------------
 def _dots_bound(q, x, group):
     """|q| |x|: a group's sum is joined with two roundings and added with one, to partial sums of at most that; the fixed point is off by
