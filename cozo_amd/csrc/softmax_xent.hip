@@ -113,11 +113,22 @@ struct Scale2 {
 // From here on neighbouring f32 logits are 1 and more apart: what a product's rounding leaves of a difference can be any number.
 constexpr float kCoarse = 16777216.f;
 
-// A tile's products taken into the running maximum m and sum l of each of the lane's queries, to base 2.  The maximum is that of the products (the
-// least one where the scale is negative) and scaled once; a term is then two fused multiply-adds, an exponential and an addition, and no product
-// is rounded before the difference.  PART: only the first `left` rows exist.
+// l relative to reference m, a whole number or infinite, made relative to ref
+template <typename T>
+__device__ __forceinline__ T moved(T l, float m, float ref) {
+    if (m == -__builtin_inff()) return l;
+    const int by = (int)fminf(fmaxf(m - ref, -1100.f), 1100.f);
+    if constexpr (sizeof(T) == 8) return ldexp(l, by);
+    else return ldexpf(l, by);
+}
+
+// A tile's products taken into the running reference m and sum l of each of the lane's queries, to base 2.  The reference is the largest product (the
+// least one where the scale is negative), scaled once, and from there the next whole number, so that a sum moves from one reference to another
+// without being rounded, however often a table's rows beat the ones before them.  A term is then two fused multiply-adds, an exponential and an addition,
+// and no product is rounded before the difference.  A tile's terms are added in four f32 sums, tiles in f64: a single f32 sum over a stretch lost
+// more with every row (33000 queries, 1M rows: lse off by 9e-4; the time of both is the same).  PART: only the first `left` rows exist.
 template <class G, bool PART>
-__device__ __forceinline__ void take(const G &g, uint32_t left, Scale2 scale2, float (&m)[G::NT], float (&l)[G::NT]) {
+__device__ __forceinline__ void take(const G &g, uint32_t left, Scale2 scale2, float (&m)[G::NT], double (&l)[G::NT]) {
     const int lane = threadIdx.x & 63;
     const bool least = scale2.high < 0.f;
     const float none = least ? __builtin_inff() : -__builtin_inff();
@@ -136,28 +147,28 @@ __device__ __forceinline__ void take(const G &g, uint32_t left, Scale2 scale2, f
 #pragma unroll
                 for (int r = 0; r < 16; r++) top = fmaxf(top, !PART || is_there(i, r) ? g.acc[i][j][r] : none);
         }
-        top = fmaxf(m[j], top * scale2.high);
+        top = ceilf(fmaxf(m[j], top * scale2.high));
         const float ref = reference(top);
-        float sum = m[j] == -__builtin_inff() ? l[j] : l[j] * exp2_(m[j] - ref);
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
         if (__builtin_expect(!__any(!(fabsf(ref) < kCoarse)), 1)) {
 #pragma unroll
             for (int i = 0; i < G::MT; i++)
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
                     const float e = exp2_(fmaf(g.acc[i][j][r], scale2.low, fmaf(g.acc[i][j][r], scale2.high, -ref)));
-                    sum += !PART || is_there(i, r) ? e : 0.f;
+                    sum[r & 3] += !PART || is_there(i, r) ? e : 0.f;
                 }
-        } else {  // the largest term is to be 1 still
+        } else {  // (whole numbers: the largest term is to be 1)
 #pragma unroll
             for (int i = 0; i < G::MT; i++)
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
                     const float e = exp2_(__fsub_rn(__fmul_rn(g.acc[i][j][r], scale2.high), ref));
-                    sum += !PART || is_there(i, r) ? e : 0.f;
+                    sum[r & 3] += !PART || is_there(i, r) ? e : 0.f;
                 }
         }
+        l[j] = moved(l[j], m[j], ref) + (double)((sum[0] + sum[1]) + (sum[2] + sum[3]));
         m[j] = top;
-        l[j] = sum;
     }
 }
 
@@ -171,9 +182,10 @@ xent_forward_kernel(O W, Operand Q, uint32_t steps, Scale2 scale2, uint32_t n_ti
     const uint32_t qt = (Q.rows + BN - 1) / BN, at = gemm::place_in_order();
     const uint32_t n0 = at % qt * BN, part = at / qt;
     const uint32_t t0 = part * tiles_per_part, t1 = min(n_tiles, t0 + tiles_per_part);
-    float m[G::NT], l[G::NT];
+    float m[G::NT];
+    double l[G::NT];
 #pragma unroll
-    for (int j = 0; j < G::NT; j++) m[j] = -__builtin_inff(), l[j] = 0.f;
+    for (int j = 0; j < G::NT; j++) m[j] = -__builtin_inff(), l[j] = 0.0;
     G g;
     for (uint32_t t = t0; t < t1; t++) {
         g.run(W, t * BM, Q, n0, 0, steps, lds);
@@ -186,9 +198,10 @@ xent_forward_kernel(O W, Operand Q, uint32_t steps, Scale2 scale2, uint32_t n_ti
     float2 *red = (float2 *)lds;  // [WM][BN]
 #pragma unroll
     for (int j = 0; j < G::NT; j++) {
-        const float mo = __shfl_xor(m[j], 32, 64), lo = __shfl_xor(l[j], 32, 64);
+        const float mo = __shfl_xor(m[j], 32, 64);
+        const double lo = __shfl_xor(l[j], 32, 64);
         const float top = fmaxf(m[j], mo), ref = reference(top);
-        const float sum = (m[j] == -__builtin_inff() ? l[j] : l[j] * exp2_(m[j] - ref)) + (mo == -__builtin_inff() ? lo : lo * exp2_(mo - ref));
+        const float sum = (float)(moved(l[j], m[j], ref) + moved(lo, mo, ref));
         if (lane < 32) red[(threadIdx.x >> 6) / WN * BN + G::wave_col() + j * 32 + lane] = make_float2(top, sum);
     }
     __syncthreads();
@@ -199,7 +212,7 @@ xent_forward_kernel(O W, Operand Q, uint32_t steps, Scale2 scale2, uint32_t n_ti
         for (int w = 1; w < WM; w++) {
             const float2 b = red[w * BN + c];
             const float top = fmaxf(a.x, b.x), ref = reference(top);
-            a.y = (a.x == -__builtin_inff() ? a.y : a.y * exp2_(a.x - ref)) + (b.x == -__builtin_inff() ? b.y : b.y * exp2_(b.x - ref));
+            a.y = moved(a.y, a.x, ref) + moved(b.y, b.x, ref);
             a.x = top;
         }
         parts[(uint64_t)part * Q.rows + n0 + c] = a;

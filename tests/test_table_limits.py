@@ -151,3 +151,61 @@ def test_products_that_cancel(gpu_lib, B):
     top = R.bf16_bits(np.full((40, dim // group), 2.0 ** 127, np.float32))
     got = _gpu_table(R.pack(np.full((40, dim), 7)), top, sq, dim).dots(_cuda(np.full((B, dim), 1e-10, np.float32))).cpu().numpy()
     assert np.allclose(got, dim * 7 * 2.0 ** 127 * np.float64(np.float32(1e-10)), rtol=1e-5)
+
+
+# ---- the loss ------------------------------------------------------------------------------------------------------
+def _typed(a, dtype):
+    import torch
+    return a.to(torch.bfloat16 if dtype == "bf16" else torch.float32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("T,V", [(40, 1_000_000), (1024, 1_000_000), (33000, 1_000_003)])
+def test_long_sums(gpu_lib, dtype, T, V):
+    """a million equal rows and one that outweighs each of them: the sum of their exponentials does not lose more with every row"""
+    import torch
+    from cozo_amd.softmax import softmax_xent
+    w = torch.zeros(V, 8, device="cuda")
+    w[V // 3, 0] = 1.0
+    w = _typed(w, dtype)
+    q = torch.zeros(T, 8, device="cuda")
+    q[:, 0] = torch.linspace(0.125, 3.0, T, device="cuda")
+    q = _typed(q, dtype)
+    y = torch.full((T,), V // 3, dtype=torch.int32, device="cuda")
+    loss, lse = softmax_xent(q, w, y)
+    z = q[:, 0].double()
+    want = torch.log(torch.exp(z) + (V - 1))
+    # an exponential: 2 ulp, and its argument (at most 5 to base 2, of two products and a difference) 3 roundings; sums of at most 64 of them
+    # before wider ones, 12 joins; lse's own rounding
+    tol = (4 + 15 + 64 + 12) * U32 + U32 * want
+    assert bool(((lse.double() - want).abs() <= tol).all()), float((lse.double() - want).abs().max())
+    assert bool(((loss.double() - (want - z)).abs() <= tol).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("T,step", [(300, 2.0 ** -12), (300, 2.0 ** -7), (33000, 2.0 ** -8)])
+def test_sums_whose_maximum_keeps_rising(gpu_lib, dtype, T, step):
+    """every tile of the table beats the ones before it a little: taking the sum along does not cost a rounding each time"""
+    import torch
+    from cozo_amd.softmax import softmax_xent
+    V = 400_000
+    w = torch.zeros(V, 8, device="cuda")
+    w[:, 0] = torch.floor(torch.arange(V, device="cuda") / 64.0) * step
+    w[:, 1] = w[:, 0] - _typed(w[:, 0], dtype).float()
+    w[:, 0] -= w[:, 1]
+    w[:, 2] = w[:, 1] - _typed(w[:, 1], dtype).float()
+    w[:, 1] -= w[:, 2]
+    w = _typed(w, dtype)
+    q = torch.zeros(T, 8, device="cuda")
+    q[:, :3] = 1.0
+    q = _typed(q, dtype)
+    y = torch.zeros(T, dtype=torch.int32, device="cuda")
+    loss, lse = softmax_xent(q, w, y)
+    z = w.double().sum(1)
+    want = float(torch.logsumexp(z, 0))
+    # (arguments are differences from the maximum: what weighs is within 30 of it; logits of at most 2^7 are off by their roundings)
+    top = float(z.max())
+    tol = (4 + 64 + 12) * U32 + 8 * U32 * max(1.0, top) + U32 * want
+    assert float((lse.double() - want).abs().max()) <= tol
