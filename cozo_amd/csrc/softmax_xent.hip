@@ -98,15 +98,15 @@ xent_transpose_kernel(const T *__restrict__ x, uint64_t ld, bool wide, uint32_t 
 }
 
 // scale log2(e) in two parts: a factor rounded to f32 would move all logits alike.  low has high's sign and is not zero where high is not, so that
-// infinite products stay what they are.
+// infinite products stay what they are; the least f32 there is moves a finite product by less than 1e-6.  (|scale| < 2^127: in the f32 range)
 struct Scale2 {
     float high, low;
     static Scale2 of(float scale) {
         const double x = (double)scale * 1.44269504088896340736;
-        if (!(x != 0.0 && std::fabs(x) <= 3e38)) return Scale2{(float)x, (float)x};
+        if (x == 0.0) return Scale2{0.f, 0.f};
         float high = (float)x;
         if (std::fabs((double)high) > std::fabs(x)) high = std::nextafter(high, 0.f);
-        return Scale2{high, std::copysign((float)std::max(std::fabs(x - (double)high), 1.2e-38), high)};
+        return Scale2{high, std::copysign(std::max((float)std::fabs(x - (double)high), 0x1p-149f), high)};
     }
 };
 
@@ -677,9 +677,11 @@ int check_shape(uint32_t T, uint32_t V, uint32_t dim, int elem) {
 }
 
 // what forward and backward check alike; host arrays are staged
-int prepare_call(Shape &s, int elem, uint32_t flags, const void *&queries, const void *&table, const uint32_t *&targets, cz::HostStage &stage) {
+int prepare_call(Shape &s, int elem, float scale, uint32_t flags, const void *&queries, const void *&table, const uint32_t *&targets,
+                 cz::HostStage &stage) {
     int rc = check_shape(s.T, s.V, s.dim, elem);
     if (rc) return rc;
+    if (!(std::fabs(scale) < 0x1p127f)) return cz::set_error(CZ_E_INVALID, "scale is not below 2^127");
     s.bf16 = elem == CZ_ELEM_BF16;
     if (s.ldq < s.dim || s.ldw < s.dim) return cz::set_error(CZ_E_INVALID, "ldq or ldw is smaller than dim");
     rc = cz::ensure_device();
@@ -718,7 +720,7 @@ extern "C" int cz_softmax_xent(const void *queries, uint64_t ldq, const void *ta
     cz::HostStage stage(stream);
     cz::DevBuf<uint8_t> own;
     Shape s{T, V, dim, ldq, ldw, false};
-    int rc = prepare_call(s, elem, flags, queries, table, targets, stage);
+    int rc = prepare_call(s, elem, scale, flags, queries, table, targets, stage);
     if (rc || T == 0) return rc;
     if (!loss || !lse) return cz::set_error(CZ_E_INVALID, "null buffer");
     const bool dev = flags & CZ_DEVICE_PTRS;
@@ -749,7 +751,7 @@ extern "C" int cz_softmax_xent_grad(const void *queries, uint64_t ldq, const voi
     cz::DevBuf<uint8_t> own;
     Shape s{T, V, dim, ldq, ldw, false};
     const bool dev = flags & CZ_DEVICE_PTRS;
-    int rc = prepare_call(s, elem, flags, queries, table, targets, stage);
+    int rc = prepare_call(s, elem, scale, flags, queries, table, targets, stage);
     if (rc || (!grad_queries && !grad_table)) return rc;
     const uint32_t es = s.es();
     if (T == 0) {  // the table's gradient is written whole all the same

@@ -330,7 +330,7 @@ int cz_q4_knn(int metric, const uint8_t *codes, const uint16_t *scales, const fl
  *   z[t][v] = scale * queries[t] . table[v]       lse[t] = log sum_v exp z[t][v]       loss[t] = lse[t] - z[t][targets[t]]
  * targets[t] = CZ_NONE: no row answers the query, its loss and gradient are 0.  A target that is no row gives a NaN loss and is
  * otherwise treated like CZ_NONE (host pointers: CZ_E_INVALID).
- *   queries [T] rows of `dim` elements, ldq apart; table [V] rows, ldw apart; both of type `elem`; 1 <= dim <= 8192, V >= 1.
+ *   queries [T] rows of `dim` elements, ldq apart; table [V] rows, ldw apart; both of type `elem`; 1 <= dim <= 8192, V >= 1; |scale| < 2^127.
  * Products and sums are f32 (f32 products stay f32; bf16 products are exact).
  * Logits of 2^24 and more have no fraction in f32: lse is as exact as they are, but which weights exp(z - lse) become 1 and which 0 is
  * then up to rounding (none is larger than 1).

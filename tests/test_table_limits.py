@@ -209,3 +209,33 @@ def test_sums_whose_maximum_keeps_rising(gpu_lib, dtype, T, step):
     top = float(z.max())
     tol = (4 + 64 + 12) * U32 + 8 * U32 * max(1.0, top) + U32 * want
     assert float((lse.double() - want).abs().max()) <= tol
+
+
+def test_scales_that_are_no_factor_are_refused():
+    from cozo_amd import _lib
+    L = _lib.lib()
+    p = _lib.ptr(np.zeros(64, np.uint8))
+    for scale in (np.nan, np.inf, -np.inf, 2.0 ** 127, -2.0 ** 127):
+        assert L.cz_softmax_xent(p, 4, p, 4, 0, 1, 1, 4, p, scale, p, p, None, 0, 0, None) == _lib.CZ_E_INVALID
+        assert L.cz_softmax_xent_grad(p, 4, p, 4, 0, 1, 1, 4, p, scale, p, p, p, p, None, 0, 0, None) == _lib.CZ_E_INVALID
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("size,scale", [(1e18, 1e-36), (1e18, 1e-37), (1e18, -1e-37), (1e18, 2e-38), (1e-18, 1.5e38), (1e-18, -1.7e38)])
+def test_scales_at_the_ends_of_the_range(gpu_lib, dtype, size, scale):
+    """products near one end of the f32 range and a scale near the other"""
+    import torch
+    from cozo_amd.softmax import softmax_xent
+    g = torch.Generator().manual_seed(5)
+    q, w = torch.randn(9, 40, generator=g) * size, torch.randn(500, 40, generator=g) * size
+    q, w = _typed(q, dtype).cuda(), _typed(w, dtype).cuda()
+    y = torch.arange(9, dtype=torch.int32, device="cuda")
+    loss, lse = softmax_xent(q, w, y, scale=scale)
+    z = float(np.float32(scale)) * (q.double() @ w.double().T)
+    want = torch.logsumexp(z, 1)
+    # of a logit: 40 products, the factors and the argument; the sum of 500 exponentials; lse's own rounding
+    tol = 48 * U32 * abs(scale) * (q.double().abs() @ w.double().abs().T).amax(1) + 128 * U32 + U32 * want.abs()
+    assert bool(((lse.double() - want).abs() <= tol).all())
+    answer = z.gather(1, y.long()[:, None])[:, 0]
+    assert bool(((loss.double() - (want - answer)).abs() <= tol + U32 * (want - answer).abs()).all())
