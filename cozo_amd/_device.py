@@ -20,6 +20,14 @@ def all_on_gpu(*arrays) -> bool:
     return any(there)
 
 
+def no_graph(*arrays) -> None:
+    """refuses tensors that autograd follows: what a call of the C library makes of them has no gradient, and would not say so"""
+    if any(getattr(a, "requires_grad", False) for a in arrays):
+        import torch
+        if torch.is_grad_enabled():
+            raise ValueError("a tensor requires a gradient, which the result would not carry: detach it, or call under torch.no_grad()")
+
+
 class on_stream:
     """with on_stream(tensor, stream) as raw: the raw stream a call works on -- the caller's (a handle or a torch stream), or torch's
     current one on the tensor's device.  Outputs and scratch allocated inside belong to that stream."""

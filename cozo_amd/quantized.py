@@ -4,6 +4,8 @@
 over the rows as they stand) and `dequantize`.  Arrays are numpy on the host (a call is synchronous) or torch tensors on the GPU
 (a call only enqueues work, on torch's current stream unless told otherwise, and may be captured into a graph).  On the host
 bfloat16 is held as uint16 bits; row numbers in results are uint32 on the host and int32 on the GPU (a missing one is 0xFFFFFFFF / -1).
+Results are no part of an autograd graph: queries that require a gradient are taken under torch.no_grad() only (`quantize`, whose codes have none,
+takes any vectors).
 """
 from __future__ import annotations
 
@@ -13,7 +15,7 @@ from typing import Any, Optional
 import numpy as np
 
 from . import _lib
-from ._device import all_on_gpu, on_stream
+from ._device import all_on_gpu, no_graph, on_stream
 from ._lib import CZ_DEVICE_PTRS, CZ_ELEM_BF16, CZ_ELEM_F32, check, ptr
 from .hnsw import DISTANCES
 
@@ -79,6 +81,7 @@ class Q4Table:
 
     def _queries(self, queries):
         gpu = all_on_gpu(self.codes, queries)
+        no_graph(queries, self.scales)
         if not gpu:
             queries = np.ascontiguousarray(queries, dtype=np.float32)
         elif str(queries.dtype) != "torch.float32":
@@ -92,6 +95,7 @@ class Q4Table:
     def dequantize(self, rows=None, stream=None):
         """f32 rows: those that `rows` names (a number that is no row: refused on the host, NaN on the GPU), or all"""
         L = _lib.lib()
+        no_graph(self.scales)
         if not self._gpu:
             r = None if rows is None else np.asarray(rows).reshape(-1)
             if r is not None:

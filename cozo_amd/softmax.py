@@ -3,14 +3,15 @@ trains the vectors an index holds.  Row targets[t] of `table` is the answer to q
 
 Arrays are numpy on the host (a call is synchronous; bfloat16 as uint16 bits) or torch tensors on the GPU (a call only enqueues
 work, on torch's current stream unless told otherwise, and may be captured into a graph).  A target of -1 (0xFFFFFFFF) is no answer:
-loss and gradient of that query are 0.
+loss and gradient of that query are 0.  The calls are no part of an autograd graph: tensors that require a gradient are taken under
+torch.no_grad() only.
 """
 from __future__ import annotations
 
 import numpy as np
 
 from . import _lib
-from ._device import all_on_gpu, on_stream
+from ._device import all_on_gpu, no_graph, on_stream
 from ._lib import CZ_DEVICE_PTRS, check, ptr
 from .quantized import _elem_of, _rows
 
@@ -36,6 +37,7 @@ def _targets(targets, T: int, gpu: bool):
 
 
 def _inputs(queries, table, *more):
+    no_graph(queries, table, *more)
     gpu = all_on_gpu(queries, table, *more)
     if not gpu:
         queries, table = (a if isinstance(a, np.ndarray) else np.asarray(a, dtype=np.float32) for a in (queries, table))

@@ -239,3 +239,47 @@ def test_scales_at_the_ends_of_the_range(gpu_lib, dtype, size, scale):
     assert bool(((lse.double() - want).abs() <= tol).all())
     answer = z.gather(1, y.long()[:, None])[:, 0]
     assert bool(((loss.double() - (want - answer)).abs() <= tol + U32 * (want - answer).abs()).all())
+
+
+# ---- tensors that require a gradient -------------------------------------------------------------------------------
+def test_tensors_that_require_a_gradient_are_refused():
+    import torch
+    from cozo_amd import softmax
+    from cozo_amd._device import no_graph
+    a, b = torch.zeros(3, 8), torch.zeros(5, 8, requires_grad=True)
+    y = torch.zeros(3, dtype=torch.int64)
+    with pytest.raises(ValueError, match="gradient"):
+        softmax.softmax_xent(a, b, y)
+    with pytest.raises(ValueError, match="gradient"):
+        softmax.softmax_xent(b[:3], a, y)
+    with pytest.raises(ValueError, match="gradient"):
+        softmax.softmax_xent_grad(a, b, y, torch.zeros(3), torch.zeros(3))
+    with pytest.raises(ValueError, match="gradient"):
+        no_graph(None, np.zeros(3), b)
+    with torch.no_grad():
+        no_graph(b)
+    no_graph(b.detach(), a, None)
+
+
+@pytest.mark.gpu
+def test_a_parameter_trains(gpu_lib):
+    import torch
+    from cozo_amd.quantized import quantize
+    from cozo_amd.softmax import softmax_xent, softmax_xent_grad
+    w = torch.nn.Parameter(torch.randn(300, 64, device="cuda"))
+    q, y = torch.randn(5, 64, device="cuda"), torch.arange(5, device="cuda")
+    with pytest.raises(ValueError, match="gradient"):
+        softmax_xent(q, w, y)
+    with torch.no_grad():
+        loss, lse = softmax_xent(q, w, y)
+        w.grad = softmax_xent_grad(q, w, y, lse, torch.ones(5, device="cuda"), want_queries=False)[1]
+        t = quantize(w)
+    ref = w.detach().double().requires_grad_()
+    torch.nn.functional.cross_entropy(q.double() @ ref.T, y, reduction="sum").backward()
+    # a weight's relative error: its logit's (64 products and 8 roundings), twice with lse's, and the sum's and the exponential's
+    off = 2 * 72 * U32 * float((q.double().abs() @ ref.abs().T).max()) + 128 * U32
+    assert bool(((w.grad.double() - ref.grad).abs() <= off * q.double().abs().sum(0)).all())
+    with pytest.raises(ValueError, match="gradient"):
+        t.dots(q.clone().requires_grad_())
+    with pytest.raises(ValueError, match="gradient"):
+        t.knn(q.clone().requires_grad_(), 3)
