@@ -6,6 +6,8 @@ import pytest
 from tests import table_ref as R
 from tests.test_quantized import METRICS, U32, _check_knn, _cuda, _gpu_table, _table
 
+UBF16 = 2.0 ** -8  # half a step, relative
+
 
 # ---- scores of a large batch ---------------------------------------------------------------------------------------
 @pytest.mark.gpu
@@ -153,6 +155,19 @@ def test_products_that_cancel(gpu_lib, B):
     assert np.allclose(got, dim * 7 * 2.0 ** 127 * np.float64(np.float32(1e-10)), rtol=1e-5)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,dim,group,B", [(300, 768, 64, 1), (300, 768, 32, 17), (300, 200, 128, 7), (64, 8192, 64, 5), (100, 33, 32, 70)])
+def test_products_keep_every_digit(gpu_lib, n, dim, group, B):
+    """one large element in each query: the others live in the fixed point's lower digits"""
+    codes, scales, sq, x = _table(n, dim, group, n + dim)
+    rng = np.random.default_rng(B)
+    for spread in (1.0, 1e-3, 1e-6):
+        q = (rng.standard_normal((B, dim)) * spread).astype(np.float32)
+        q[np.arange(B), rng.integers(0, dim, B)] = 1.0
+        got = _gpu_table(codes, scales, sq, dim).dots(_cuda(q)).cpu().numpy()
+        assert np.all(np.abs(got - q.astype(np.float64) @ x.T) <= _dots_bound(q, x, group))
+
+
 # ---- the loss ------------------------------------------------------------------------------------------------------
 def _typed(a, dtype):
     import torch
@@ -241,6 +256,110 @@ def test_scales_at_the_ends_of_the_range(gpu_lib, dtype, size, scale):
     assert bool(((loss.double() - (want - answer)).abs() <= tol + U32 * (want - answer).abs()).all())
 
 
+# ---- the gradient --------------------------------------------------------------------------------------------------
+def _grad_bounds(q, w, y, g, scale, dtype):
+    """the gradient in f64 (tensors on the GPU) and how far off each entry may be: as the bound of the other tests, but an answer's entry of G
+    loses nothing to bf16"""
+    import torch
+    q, w, g = q.double(), w.double(), g.double()
+    live = (y >= 0)
+    at = y.clamp(min=0).long()[:, None]
+    z = scale * (q @ w.T)
+    lse = torch.logsumexp(z, 1)
+    p = torch.exp(z - lse[:, None])
+    lz = ((q.shape[1] + 8) * U32 * scale) * (q.abs() @ w.abs().T).amax(1)
+    ep = 2 * (lz + 128 * U32) + 4 * U32 * (z.abs().amax(1) + lse.abs()) + 2.0 ** -21
+    weight = (g.abs() * live)[:, None]
+    G = p.clone()
+    G.scatter_add_(1, at, -torch.ones_like(at, dtype=torch.float64))
+    G *= (g * live)[:, None]
+    del z
+    cut = G.abs() * (UBF16 if dtype == "bf16" else 0.0)
+    cut.scatter_(1, at, 0.0)
+    eG = weight * (p * ep[:, None] + 2 * U32) + 2 * U32 * G.abs() + cut
+    del p, cut
+    out = UBF16 if dtype == "bf16" else U32
+    dq, dw = scale * (G @ w), scale * (G.T @ q)
+    a = G.abs()
+    tq = scale * (eG @ w.abs()) + (w.shape[0] + 64) * U32 * scale * (a @ w.abs()) + out * dq.abs()
+    tw = scale * (eG.T @ q.abs()) + (q.shape[0] + 64) * U32 * scale * (a.T @ q.abs()) + out * dw.abs()
+    return dq, dw, 1.01 * tq + 1e-37, 1.01 * tw + 1e-37
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("T,V,dim", [(3000, 100_003, 24), (3000, 100_003, 23), (700, 70_001, 4100)])
+def test_gradient_in_pieces(gpu_lib, dtype, T, V, dim):
+    """tables worked on in several pieces, the last one ragged, rows aligned and not, with answers in every piece and at the seams"""
+    import torch
+    from cozo_amd.softmax import softmax_xent, softmax_xent_grad
+    elem = 1 if dtype == "bf16" else 0
+    size = lambda rows: gpu_lib.cz_softmax_xent_workspace(T, rows, dim, elem, 1)  # noqa: E731
+    lo, hi = 1, V  # the rows of a piece: from there on the scratch no longer grows
+    while lo < hi:
+        mid = (lo + hi) // 2
+        lo, hi = (lo, mid) if size(mid) == size(V) else (mid + 1, hi)
+    piece = -(-lo // 256) * 256
+    assert size(2 * V) == size(V) and V > piece + 1 and V % piece
+    gen = torch.Generator(device="cuda").manual_seed(dim)
+    q = _typed(torch.randn(T, dim, device="cuda", generator=gen) / dim ** 0.5, dtype)
+    w = _typed(torch.randn(V, dim, device="cuda", generator=gen), dtype)
+    y = torch.randint(0, V, (T,), device="cuda", generator=gen)
+    y[1::7] = -1
+    seams = [0, piece - 1, piece, piece + 1, V - 1] + [v for k in range(2, -(-V // piece)) for v in (k * piece - 1, k * piece)]
+    y[2:2 + 2 * len(seams):2] = torch.tensor(seams, device="cuda")
+    g = torch.randn(T, device="cuda", generator=gen)
+    loss, lse = softmax_xent(q, w, y, scale=2.0)
+    got_q, got_w = softmax_xent_grad(q, w, y, lse, g, scale=2.0)
+    dq, dw, tq, tw = _grad_bounds(q, w, y, g, 2.0, dtype)
+    assert bool(((got_q.double() - dq).abs() <= tq).all()) and bool(((got_w.double() - dw).abs() <= tw).all())
+    assert not bool(got_q[y < 0].any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,V,dim", [(40, 700, 64), (300, 3000, 128), (5, 2000, 72)])
+def test_answers_lose_nothing_to_rounding(gpu_lib, T, V, dim):
+    """bf16: G is rounded to 8 bits before the products, but not at the answers, whose entries outweigh the others"""
+    import torch
+    from cozo_amd.softmax import softmax_xent, softmax_xent_grad
+    gen = torch.Generator(device="cuda").manual_seed(T)
+    w = torch.randn(V, dim, device="cuda", generator=gen).to(torch.bfloat16)
+    y = torch.randperm(V, device="cuda", generator=gen)[:T]
+    q = (torch.randn(T, dim, device="cuda", generator=gen) * 0.05).to(torch.bfloat16)
+    g = torch.full((T,), 171.45 / 512, device="cuda")  # (rounded to bf16: off by two thirds of what the result's own rounding may be)
+    _, lse = softmax_xent(q, w, y)
+    got_q, got_w = softmax_xent_grad(q, w, y, lse, g)
+    dq, dw, tq, tw = _grad_bounds(q, w, y, g, 1.0, "bf16")
+    assert bool(((got_q.double() - dq).abs() <= tq).all()) and bool(((got_w.double() - dw).abs() <= tw).all())
+
+
+@pytest.mark.gpu
+def test_answers_do_not_drown_the_rest(gpu_lib):
+    """f32: a query's gradient is one large term, of the row that answers it, and a sum of many, each below half a step of that term"""
+    import torch
+    from cozo_amd.softmax import softmax_xent, softmax_xent_grad
+    T, V, dim = 60, 3001, 64
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    w = 0.07 + 0.005 * torch.rand(V, dim, device="cuda", generator=gen)
+    y = torch.randperm(V, device="cuda", generator=gen)[:T]
+    w[y] = 900.0 + 100.0 * torch.rand(T, dim, device="cuda", generator=gen)
+    q = -torch.rand(T, dim, device="cuda", generator=gen) / dim  # (the answers' logits are far below the others: their weights are -1)
+    g = torch.ones(T, device="cuda")
+    _, lse = softmax_xent(q, w, y)
+    got, _ = softmax_xent_grad(q, w, y, lse, g, want_table=False)
+    z = q.double() @ w.double().T
+    p = torch.exp(z - torch.logsumexp(z, 1)[:, None])
+    # of a weight: its logit and lse, each rounded, an exponential; of the sum: V additions
+    ep = 2 * (dim + 8) * U32 * (q.double().abs() @ w.double().abs().T) + 128 * U32 + 12 * U32 * np.log(V)
+    at = torch.arange(T, device="cuda")
+    small = p.clone()
+    small[at, y] = 0
+    hit = (p[at, y] - 1)[:, None] * w[y].double()
+    want = small @ w.double() + hit
+    tol = (small * (ep + (V + 64) * U32)) @ w.double().abs() + 4 * U32 * hit.abs() + 2 * U32 * want.abs()
+    assert bool(((got.double() - want).abs() <= tol).all())
+
+
 # ---- tensors that require a gradient -------------------------------------------------------------------------------
 def test_tensors_that_require_a_gradient_are_refused():
     import torch
@@ -277,7 +396,7 @@ def test_a_parameter_trains(gpu_lib):
     ref = w.detach().double().requires_grad_()
     torch.nn.functional.cross_entropy(q.double() @ ref.T, y, reduction="sum").backward()
     # a weight's relative error: its logit's (64 products and 8 roundings), twice with lse's, and the sum's and the exponential's
-    off = 2 * 72 * U32 * float((q.double().abs() @ ref.abs().T).max()) + 128 * U32
+    off = 2 * 72 * U32 * float((q.double().abs() @ ref.detach().abs().T).max()) + 128 * U32
     assert bool(((w.grad.double() - ref.grad).abs() <= off * q.double().abs().sum(0)).all())
     with pytest.raises(ValueError, match="gradient"):
         t.dots(q.clone().requires_grad_())
