@@ -1018,7 +1018,7 @@ q4_scan_kernel(int metric, Rows t, const float *__restrict__ queries, uint32_t k
 }
 
 // one workgroup per query: the partial lists joined, the radius cut, the padding.  What a list takes in a full batch at a time would be merged for microseconds; the k-th
-// smallest of 256 lists' heads, which k entries are sure not to be behind, leaves few to merge (one query, 157 lists: 76 -> 12 us).
+// smallest of 256 lists' heads, which k entries are sure not to be behind, leaves few to merge (one query, 157 lists: 76 -> 18 us).
 constexpr size_t join_lds(size_t k) { return 256 * 24 + k * 12 + 257 * 4 + 8 * 4 + 8; }
 __global__ void __launch_bounds__(256)
 q4_join_kernel(const uint64_t *__restrict__ part_key, const uint32_t *__restrict__ part_id, const uint32_t *__restrict__ part_count,
@@ -1243,7 +1243,8 @@ float half_error_unit(const Rows &t) {
     return 1.01f * (0x1p-11f + sqrtf((float)t.dim) * 0x1p-20f + (float)t.dim * 0x1p-24f + 0x1p-21f);
 }
 
-// queries of one launch; a larger batch goes in turns through the same scratch (at most 1 GiB of tile scores)
+// queries of one launch; a larger batch goes in turns through the same scratch: 1 GiB of tile scores, twice that where the f16 product turns them, for
+// tables of up to 268M rows; beyond, what 64 queries take (8.6 GB, and as much again, at 2^31 rows)
 uint32_t turn_of(const Rows &t) {
     const uint64_t n_tiles = std::max<uint64_t>(1, ((uint64_t)t.n + kTile - 1) / kTile);
     return (uint32_t)std::min<uint64_t>(4096, std::max<uint64_t>(64, (1ull << 28) / n_tiles));

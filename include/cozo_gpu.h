@@ -297,7 +297,8 @@ int cz_knn_bruteforce(cz_hnsw_index *ix, const float *queries, uint32_t B, uint3
  *
  * `ws` / `ws_bytes`: device scratch of at least cz_q4_workspace() bytes, 256-byte aligned, used by this call alone until its work on
  * `stream` is done; with it and CZ_DEVICE_PTRS a call only enqueues work (it allocates nothing, waits for nothing and may be
- * captured into a graph).  ws = NULL: the library allocates, waits and frees.  Device pointers have to be on the selected GPU.
+ * captured into a graph).  ws = NULL: the library allocates, waits and frees.  Device pointers have to be on the selected GPU.  The search's
+ * scratch holds up to 2 GiB of scores and the lists (more for tables of over 268M rows); a larger batch goes through it in turns.
  * ===================================================================================== */
 typedef enum { CZ_ELEM_F32 = 0, CZ_ELEM_BF16 = 1 } cz_elem; /* element type of rows and queries */
 
@@ -311,7 +312,8 @@ int cz_q4_dequantize(const uint8_t *codes, const uint16_t *scales, uint32_t n, u
 /* bytes of `ws` for cz_q4_dots (k = 0) or cz_q4_knn of these sizes; 0 when the sizes are refused */
 uint64_t cz_q4_workspace(uint32_t n, uint32_t dim, uint32_t group, uint32_t B, uint32_t k);
 /* out f32 [B][n] = queries . rows: the matrix-vector product (B = 1) and its few-column form.  queries f32 [B][dim].  Products are
- * summed in 32 bits or more; a query with a NaN or an infinity gives NaN.                    [all dev-able] */
+ * summed in 32 bits or more, and no sum leaves the f32 range before 2^17 times what a result may be; below 2^-108 a result keeps 2^-132 for each
+ * group.  A query with a NaN or an infinity gives NaN.                                       [all dev-able] */
 int cz_q4_dots(const uint8_t *codes, const uint16_t *scales, uint32_t n, uint32_t dim, uint32_t group, const float *queries,
                uint32_t B, float *out, void *ws, uint64_t ws_bytes, uint32_t flags, void *stream);
 /* exact k-NN over the 4-bit rows (exact: of the rows as they stand, not of the vectors they were made from).  Distances are the
@@ -336,8 +338,10 @@ int cz_q4_knn(int metric, const uint8_t *codes, const uint16_t *scales, const fl
  * then up to rounding (none is larger than 1).
  *   grad:  G[t][v] = grad_loss[t] * (exp(z[t][v] - lse[t]) - [v = targets[t]]);   grad_queries = scale * G . table,
  *          grad_table = scale * G^T . queries   (contiguous [T][dim] / [V][dim] of type `elem`, each written whole; either may be
- *          NULL).  For bf16, G is rounded to bf16 before the two products.  grad_loss [T] f32; lse as the forward call gave it.
- * Results do not depend on the run: no atomics.  ws / ws_bytes as for cz_q4_dots, of cz_softmax_xent_workspace() bytes. [all dev-able]
+ *          NULL).  For bf16, G is rounded to bf16 before the two products, but for the answers' entries.  grad_loss [T] f32; lse as the
+ *          forward call gave it.
+ * Results do not depend on the run: no atomics.  ws / ws_bytes as for cz_q4_dots, of cz_softmax_xent_workspace() bytes: for the gradient some
+ * 256 MiB to 1 GiB and partial sums of grad_queries; past 65536 (f32) or 131072 (bf16) queries 8 or 2 KiB more for each. [all dev-able]
  * ===================================================================================== */
 uint64_t cz_softmax_xent_workspace(uint32_t T, uint32_t V, uint32_t dim, int elem, int grad);
 int cz_softmax_xent(const void *queries, uint64_t ldq, const void *table, uint64_t ldw, int elem, uint32_t T, uint32_t V,
